@@ -368,6 +368,137 @@ FOIL_API int foil_matmul_tiles_noalloc_dev(const uint16_t* a, const uint16_t* b,
                                            const uint16_t* bias, int32_t relu, void* stream,
                                            uint32_t* status_out);
 
+/* ------------------------------------------------------------------------ */
+/* Token-path operators: products of a few rows with 4-bit weights, the norms */
+/* around a residual block, embedding rows, and their gradients.  Row-major   */
+/* tensors (not tile streams) unless an argument says "tiles".  A row stride  */
+/* `ld_*` is in elements, 0 = dense.  Outputs must not overlap inputs or each */
+/* other except where stated (FOIL_ERR_INVALID).  No counterpart in the       */
+/* reference; their numeric types are its bf16 and fp32.  Like the other      */
+/* entry points, the first call on a device may allocate its error word: make */
+/* it before any stream capture.                                              */
+/* ------------------------------------------------------------------------ */
+
+/* 4-bit weights.  A weight matrix W (K x N, the B operand of the products
+ * above) is held as codes q in 0..15 with one bf16 scale s and, if `zeros`
+ * is non-zero, one zero point z in 0..15 for each `group` (32, 64 or 128)
+ * consecutive k of a column n:  W[k][n] = s * (q - z), z = 8 without zero
+ * points.  The last group may be short (K need not be a multiple of it).
+ *
+ * Storage: blocks of 16 columns x 128 k, block (n / 16, k / 128) at index
+ * (n / 16) * ceil(K / 128) + k / 128.  A block holds 1024 bytes of codes as
+ * 32-bit words [n % 16][(k % 32) / 8][(k % 128) / 32], the eight codes of a
+ * word in the order k % 8 = 0 2 4 6 1 3 5 7 from its lowest nibble; then the
+ * scales [(k % 128) / group][n % 16] (bf16); then, if there are any, the
+ * zero points [(k % 128) / group][n % 16] (one byte each).  What lies past K
+ * or N is finite and otherwise free.  16-byte aligned.
+ *
+ * foil_w4_packed_bytes: its size in bytes, 0 for arguments outside the range
+ * (K and N from 1 to 2^24, group 32, 64 or 128). */
+FOIL_API uint64_t foil_w4_packed_bytes(uint32_t K, uint32_t N, uint32_t group, int32_t zeros);
+
+/* Codes (N x K, one byte each, the low four bits count), scales
+ * (N x ceil(K / group) bf16) and zero points (the same shape, one byte each,
+ * or NULL: storage without zero points) into the storage. */
+FOIL_API int foil_w4_pack_dev(const uint8_t* codes, const uint16_t* scales, const uint8_t* zero_points,
+                              void* packed, uint32_t K, uint32_t N, uint32_t group, void* stream);
+
+/* Quantise a tile stream of Kt x Nt tiles (K = 32 Kt, N = 32 Nt) into the
+ * storage, in fp32 arithmetic.  Without zero points: s = bf16(max|w| / 7),
+ * q = 8 + clamp(rint(w / s), -8, 7).  With: lo = min(0, min w), hi = max(0,
+ * max w), s = bf16((hi - lo) / 15), z = clamp(rint(-lo / s), 0, 15),
+ * q = clamp(rint(w / s) + z, 0, 15).  rint rounds ties to even.  A group with
+ * s = 0 gets q = z; one with an infinity or NaN, or whose range overflows
+ * fp32, stands for NaN throughout. */
+FOIL_API int foil_w4_quantize_tiles_dev(const uint16_t* tiles, void* packed, uint32_t Kt, uint32_t Nt,
+                                        uint32_t group, int32_t zeros, void* stream);
+
+/* The weights of the storage, rounded to bf16, as a tile stream: W
+ * (ceil(K / 32) x ceil(N / 32) tiles), or W transposed (ceil(N / 32) x
+ * ceil(K / 32) tiles) if `transpose` is non-zero; zeros past K and N.  W is
+ * the B operand of foil_matmul_tiles_dev for long inputs, its transpose the
+ * one of the input gradient. */
+FOIL_API int foil_w4_dequantize_tiles_dev(const void* packed, uint16_t* tiles, uint32_t K, uint32_t N,
+                                          uint32_t group, int32_t zeros, int32_t transpose, void* stream);
+
+/* y (M x N) = relu?(x (M x K) . W + bias) for a few rows, M from 1 to 64:
+ * one pass over the 4-bit weights for every 16 rows (longer inputs: dequantise
+ * and use foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or
+ * NULL.  fp32 accumulation of unrounded weights, one rounding to bf16 at the
+ * end.  M = 0 or N = 0 does nothing. */
+FOIL_API int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* packed, const uint16_t* bias,
+                                uint16_t* y, uint64_t ld_y, uint32_t M, uint32_t K, uint32_t N,
+                                uint32_t group, int32_t zeros, int32_t relu, void* stream);
+
+/* The norms after one block and before the next, fused with the block's gate,
+ * its scale and the residual addition, for T tokens of D channels (D at most
+ * 16384), N(v) = v / sqrt(mean(v^2) + eps):
+ *
+ *   p = post ? N(u) * w_post : u          the block's output u
+ *   h = resid + scale * act(gate) * p     the residual stream
+ *   y = N(h) * w_pre                      the next block's input
+ *
+ * Weights that are NULL are ones.  gate: bf16 rows of D, token t takes row
+ * t / gate_rows (1: a gate for each token, T: one vector for all); NULL: none.
+ * act: FOIL_GATE_NONE or FOIL_GATE_SIGMOID.  resid and h: bf16, or fp32 if
+ * `fp32` is non-zero.  u NULL: no branch (h = resid).  h or y may be NULL
+ * (not wanted), not both.  rstd_post, rstd_pre: T floats each,
+ * 1 / sqrt(mean + eps), for the gradient, or NULL.  Sums and the value that y
+ * is made from are held in fp32, h is rounded once.  h may be resid and y may
+ * be u (the same buffer with the same stride).  T = 0 or D = 0 does nothing. */
+enum { FOIL_GATE_NONE = 0, FOIL_GATE_SIGMOID = 1 };
+FOIL_API int foil_block_norm_dev(const void* resid, uint64_t ld_resid, const uint16_t* u, uint64_t ld_u,
+                                 int32_t post, const uint16_t* w_post, const uint16_t* gate,
+                                 uint64_t ld_gate, uint32_t gate_rows, int32_t gate_act,
+                                 const uint16_t* w_pre, void* h, uint64_t ld_h, uint16_t* y,
+                                 uint64_t ld_y, float* rstd_post, float* rstd_pre, uint32_t T,
+                                 uint32_t D, int32_t fp32, float scale, float eps, void* stream);
+
+/* Its gradients from those of h (dh, the type of resid) and of y (dy, bf16),
+ * either of which may be NULL (zero): dresid (the type of resid), du (bf16),
+ * dgate (bf16, one row for each gate row, summed over the tokens that share
+ * it), dw_post and dw_pre (D floats each), any of them NULL if not wanted.
+ * With dy, h and rstd_pre are needed; with any of du, dgate and dw_post, u,
+ * and with post also rstd_post: the forward call's outputs.  The sums over
+ * tokens are made in a fixed order.  ws: workspace of at least
+ * foil_block_norm_grad_ws_bytes(T, D, gate_rows or 0) bytes, 16-byte aligned;
+ * calls that may run at the same time need one each.  T = 0 writes zeros to
+ * dw_post and dw_pre. */
+FOIL_API uint64_t foil_block_norm_grad_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows);
+FOIL_API int foil_block_norm_grad_dev(const void* dh, uint64_t ld_dh, const uint16_t* dy, uint64_t ld_dy,
+                                      const void* h, uint64_t ld_h, const float* rstd_pre,
+                                      const uint16_t* w_pre, const uint16_t* u, uint64_t ld_u,
+                                      int32_t post, const float* rstd_post, const uint16_t* w_post,
+                                      const uint16_t* gate, uint64_t ld_gate, uint32_t gate_rows,
+                                      int32_t gate_act, void* dresid, uint64_t ld_dresid, uint16_t* du,
+                                      uint64_t ld_du, uint16_t* dgate, uint64_t ld_dgate,
+                                      float* dw_post, float* dw_pre, void* ws, uint64_t ws_bytes,
+                                      uint32_t T, uint32_t D, int32_t fp32, float scale, void* stream);
+
+/* out[t] = scale * table[ids[t]] for T ids of `id_bytes` (4 or 8, signed)
+ * into a table of V rows of D bf16; out: bf16, or fp32 if `fp32` is non-zero.
+ * A row whose id equals pad_id becomes zeros; so does one whose id is outside
+ * 0 .. V - 1, which also sets FOIL_DEVERR_BAD_INDEX in the device error word.
+ * V and T at most 2^24. */
+FOIL_API int foil_embed_rows_dev(const void* ids, int32_t id_bytes, const uint16_t* table, uint64_t ld_table,
+                                 void* out, uint64_t ld_out, uint32_t T, uint32_t V, uint32_t D,
+                                 int32_t fp32, float scale, int64_t pad_id, void* stream);
+
+/* Its gradient: dtable[v] = scale * sum of dout[t] over the tokens with
+ * ids[t] = v (dout: bf16, or fp32 if `fp32` is non-zero; dtable: fp32 rows).
+ * Every row is written (zeros where no token names it); if `accumulate` is
+ * non-zero the sums are added instead and rows that no token names are left
+ * as they are.  Tokens are sorted by id and the sums made in a fixed order:
+ * the same call gives the same bits.  Rows with pad_id or a bad id count
+ * nowhere, the latter setting FOIL_DEVERR_BAD_INDEX.  ws: workspace of at
+ * least foil_embed_rows_grad_ws_bytes(T, V, D) bytes, 16-byte aligned; calls
+ * that may run at the same time need one each. */
+FOIL_API uint64_t foil_embed_rows_grad_ws_bytes(uint32_t T, uint32_t V, uint32_t D);
+FOIL_API int foil_embed_rows_grad_dev(const void* ids, int32_t id_bytes, const void* dout, uint64_t ld_dout,
+                                      float* dtable, uint64_t ld_dtable, uint32_t T, uint32_t V,
+                                      uint32_t D, int32_t fp32, float scale, int64_t pad_id,
+                                      int32_t accumulate, void* ws, uint64_t ws_bytes, void* stream);
+
 /* Wall-time limit of every bounded device-side wait (mbarrier, flag and
  * counter waits inside the kernels), in nanoseconds, for the launches that
  * follow; process-wide.  A kernel whose wait runs past it records
@@ -383,6 +514,7 @@ FOIL_API uint64_t foil_set_wait_limit_ns(uint64_t ns);
 #define FOIL_DEVERR_WAIT_TIMEOUT 1u /* a bounded wait gave up */
 #define FOIL_DEVERR_BAD_SHAPE 2u    /* a kernel saw a shape it cannot handle */
 #define FOIL_DEVERR_CONFIG 4u       /* launch parameters inconsistent with the kernel; nothing ran */
+#define FOIL_DEVERR_BAD_INDEX 8u    /* a row id outside the table (its row reads as zeros) */
 
 /* Read and clear the device-side error word of the current device: 0 if no
  * kernel reported an error (bounded waits that gave up) since the last call.

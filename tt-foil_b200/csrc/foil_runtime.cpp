@@ -31,6 +31,7 @@
 #include <vector>
 
 #include "../../include/foil_c.h"
+#include "entry.hpp"
 #include "host_logic.hpp"
 #include "kernels/gemm_tc.cuh"
 #include "kernels/conv_tc.cuh"
@@ -182,28 +183,15 @@ uint32_t* error_word_for_current_device() {
 
 int sm_count_current() { return foil_sm_count(); }
 
-template <class F>
-int guarded(F&& f) {
-    try {
-        f();
-        return FOIL_OK;
-    } catch (const FoilError& e) {
-        g_last_error = e.what();
-        return e.status;
-    } catch (const std::bad_alloc&) {
-        g_last_error = "tt-foil: host out of memory";
-        return FOIL_ERR_OOM;
-    } catch (const std::exception& e) {
-        g_last_error = e.what();
-        return FOIL_ERR_INVALID;
-    }
-}
+using foil::guarded;
 
 void throw_status(int st) {
     if (st != FOIL_OK) throw FoilError(st, g_last_error);
 }
 
 }  // namespace
+
+uint32_t* foil_error_word() { return error_word_for_current_device(); }
 
 // ====================================================================== ====
 struct foil_device {

@@ -60,6 +60,7 @@ enum : uint32_t {
     kErrWaitTimeout = 1u,  // a bounded mbarrier wait gave up
     kErrConfig = 4u,       // launch parameters inconsistent with the kernel instantiation (nothing ran)
     kErrBadShape = 2u,     // kernel saw a shape it cannot handle
+    kErrBadIndex = 8u,     // a row id outside the table
 };
 
 // Wall-clock nanoseconds (for bounded waits).

@@ -10,7 +10,9 @@ Two layers, matching the C header:
 * ``tilize`` / ``untilize`` / ``tile_copy`` / ``add_tiles`` / ``relu_tiles`` /
   ``bias_add_tiles`` / ``matmul_tiles`` run the CUDA kernels on tensors that
   already live on the GPU (torch CUDA tensors or raw device pointers), on the
-  current torch stream.
+  current torch stream.  ``w4_*`` (products of a few rows with 4-bit weights),
+  ``block_norm`` (the norms around a residual block) and ``embed_rows``, with
+  their gradients, do the same for row-major tensors.
 
 There is no fallback: if lib/libfoil.so is missing or was built for another
 GPU, importing or calling this module raises.
@@ -60,6 +62,7 @@ class foil_cb_config(ctypes.Structure):
 # Exported C-ABI symbols with their signatures (restype, argtypes).
 _P = ctypes.c_void_p
 _U16P = ctypes.c_void_p
+_U32, _I32, _U64, _F32 = ctypes.c_uint32, ctypes.c_int32, ctypes.c_uint64, ctypes.c_float
 SIGNATURES = {
     "foil_last_error": (ctypes.c_char_p, []),
     "foil_version": (ctypes.c_char_p, []),
@@ -121,10 +124,27 @@ SIGNATURES = {
     "foil_set_wait_limit_ns": (ctypes.c_uint64, [ctypes.c_uint64]),
     "foil_conv2d_chw_dev": (ctypes.c_int, [_U16P, _U16P, _U16P, _U16P] + [ctypes.c_uint32] * 9 +
                             [ctypes.c_int32, _P]),
+    "foil_w4_packed_bytes": (ctypes.c_uint64, [_U32, _U32, _U32, _I32]),
+    "foil_w4_pack_dev": (ctypes.c_int, [_P, _U16P, _P, _P, _U32, _U32, _U32, _P]),
+    "foil_w4_quantize_tiles_dev": (ctypes.c_int, [_U16P, _P, _U32, _U32, _U32, _I32, _P]),
+    "foil_w4_dequantize_tiles_dev": (ctypes.c_int, [_P, _U16P, _U32, _U32, _U32, _I32, _I32, _P]),
+    "foil_w4_matvec_dev": (ctypes.c_int, [_U16P, _U64, _P, _U16P, _U16P, _U64, _U32, _U32, _U32, _U32, _I32,
+                                          _I32, _P]),
+    "foil_block_norm_dev": (ctypes.c_int, [_P, _U64, _U16P, _U64, _I32, _U16P, _U16P, _U64, _U32, _I32, _U16P,
+                                           _P, _U64, _U16P, _U64, _P, _P, _U32, _U32, _I32, _F32, _F32, _P]),
+    "foil_block_norm_grad_ws_bytes": (ctypes.c_uint64, [_U32, _U32, _U32]),
+    "foil_block_norm_grad_dev": (ctypes.c_int, [_P, _U64, _U16P, _U64, _P, _U64, _P, _U16P, _U16P, _U64, _I32,
+                                                _P, _U16P, _U16P, _U64, _U32, _I32, _P, _U64, _U16P, _U64,
+                                                _U16P, _U64, _P, _P, _P, _U64, _U32, _U32, _I32, _F32, _P]),
+    "foil_embed_rows_dev": (ctypes.c_int, [_P, _I32, _U16P, _U64, _P, _U64, _U32, _U32, _U32, _I32, _F32,
+                                           ctypes.c_int64, _P]),
+    "foil_embed_rows_grad_ws_bytes": (ctypes.c_uint64, [_U32, _U32, _U32]),
+    "foil_embed_rows_grad_dev": (ctypes.c_int, [_P, _I32, _P, _U64, _P, _U64, _U32, _U32, _U32, _I32, _F32,
+                                                ctypes.c_int64, _I32, _P, _U64, _P]),
 }
 
 # Bits of the device error word (include/foil_c.h FOIL_DEVERR_*).
-DEVERR_WAIT_TIMEOUT, DEVERR_BAD_SHAPE, DEVERR_CONFIG = 1, 2, 4
+DEVERR_WAIT_TIMEOUT, DEVERR_BAD_SHAPE, DEVERR_CONFIG, DEVERR_BAD_INDEX = 1, 2, 4, 8
 
 _lib = None
 
@@ -279,6 +299,182 @@ def conv2d_chw(x, w, bias, y, N, Cin, H, W, Cout, KH, KW, stride, pad, relu=Fals
     w (Cout, Cin*KH*KW)) + bias), operands re-laid on the device."""
     check(lib().foil_conv2d_chw_dev(_ptr(x), _ptr(w), _ptr(bias), _ptr(y), N, Cin, H, W, Cout, KH, KW, stride,
                                     pad, 1 if relu else 0, _stream(stream)))
+
+
+# ------------------------------------------------------ token-path operators ---
+
+def _on_current(*tensors):
+    """Refuse torch tensors that do not live on the current device (raw
+    pointers and None pass)."""
+    current = None
+    for t in tensors:
+        if t is None or isinstance(t, int):
+            continue
+        if current is None:
+            import torch
+            current = torch.cuda.current_device()
+        if t.get_device() != current:
+            raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
+
+
+def _ld(t, ld):
+    """Row stride in elements: as given, else that of a 2-D torch tensor, else 0 (dense)."""
+    if ld or t is None or isinstance(t, int):
+        return ld
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if (cols > 1 and t.stride(1) != 1) or (rows > 1 and t.stride(0) < cols):
+            raise FoilError(1, "tt-foil: rows of a tensor must be contiguous and must not overlap")
+        return t.stride(0) if rows > 1 else 0
+    if not t.is_contiguous():
+        raise FoilError(1, "tt-foil: a tensor must be contiguous, or a matrix with a row stride")
+    return 0
+
+
+def _dense(*tensors):
+    for t in tensors:
+        if t is not None and not isinstance(t, int) and not t.is_contiguous():
+            raise FoilError(1, "tt-foil: a tensor must be contiguous")
+
+
+def _is_fp32(fp32, *tensors):
+    """The residual stream's type: as given, else from the first torch tensor (float32 or 16-bit)."""
+    for t in tensors:
+        if t is not None and not isinstance(t, int):
+            wide = t.element_size() == 4
+            if fp32 is not None and bool(fp32) != wide:
+                raise FoilError(1, "tt-foil: tensors of one type are mixed with another")
+            fp32 = wide
+    return 1 if fp32 else 0
+
+
+def w4_packed_bytes(K, N, group, zeros=False):
+    """Bytes of the 4-bit storage of a K x N weight matrix (0: sizes out of range)."""
+    return int(lib().foil_w4_packed_bytes(K, N, group, 1 if zeros else 0))
+
+
+def w4_pack(codes, scales, packed, K, N, group, zero_points=None, stream=None):
+    """Codes (N x K, one byte each), scales (N x ceil(K / group) bf16) and zero
+    points (alike, one byte each, or None) -> 4-bit storage."""
+    _on_current(codes, scales, zero_points, packed)
+    _dense(codes, scales, zero_points, packed)
+    check(lib().foil_w4_pack_dev(_ptr(codes), _ptr(scales), _ptr(zero_points), _ptr(packed), K, N, group,
+                                 _stream(stream)))
+
+
+def w4_quantize_tiles(tiles, packed, Kt, Nt, group, zeros=False, stream=None):
+    """Tile stream of Kt x Nt tiles -> 4-bit storage with a scale (and, with
+    `zeros`, a zero point) for each `group` values of a column."""
+    _on_current(tiles, packed)
+    _dense(tiles, packed)
+    check(lib().foil_w4_quantize_tiles_dev(_ptr(tiles), _ptr(packed), Kt, Nt, group, 1 if zeros else 0,
+                                           _stream(stream)))
+
+
+def w4_dequantize_tiles(packed, tiles, K, N, group, zeros=False, transpose=False, stream=None):
+    """4-bit storage -> tile stream of the weights, or of their transpose."""
+    _on_current(packed, tiles)
+    _dense(packed, tiles)
+    check(lib().foil_w4_dequantize_tiles_dev(_ptr(packed), _ptr(tiles), K, N, group, 1 if zeros else 0,
+                                             1 if transpose else 0, _stream(stream)))
+
+
+def w4_matvec(x, packed, y, M, K, N, group, zeros=False, bias=None, relu=False, ld_x=0, ld_y=0, stream=None):
+    """y (M x N) = relu?(x (M x K) . W + bias) with 4-bit W, M at most 64."""
+    _on_current(x, packed, bias, y)
+    _dense(packed, bias)
+    check(lib().foil_w4_matvec_dev(_ptr(x), _ld(x, ld_x), _ptr(packed), _ptr(bias), _ptr(y), _ld(y, ld_y), M, K, N,
+                                   group, 1 if zeros else 0, 1 if relu else 0, _stream(stream)))
+
+
+GATE_ACTS = {"none": 0, "sigmoid": 1}
+
+
+def _gate_act(name):
+    if name not in GATE_ACTS:
+        raise FoilError(1, f"tt-foil: unknown gate activation {name!r}")
+    return GATE_ACTS[name]
+
+
+def block_norm(resid, u, h, y, T, D, w_pre=None, post=False, w_post=None, gate=None, gate_rows=1, gate_act="none",
+               scale=1.0, eps=1e-5, rstd_post=None, rstd_pre=None, fp32=None, ld_resid=0, ld_u=0, ld_gate=0, ld_h=0,
+               ld_y=0, stream=None):
+    """h = resid + scale * act(gate) * (post ? N(u) * w_post : u);
+    y = N(h) * w_pre, with N(v) = v / sqrt(mean(v^2) + eps).  resid and h are
+    bf16 or fp32 (taken from the tensors; `fp32` for raw pointers)."""
+    _on_current(resid, u, h, y, w_pre, w_post, gate, rstd_post, rstd_pre)
+    _dense(w_pre, w_post, rstd_post, rstd_pre)
+    wide = _is_fp32(fp32, resid, h)
+    check(lib().foil_block_norm_dev(
+        _ptr(resid), _ld(resid, ld_resid), _ptr(u), _ld(u, ld_u), 1 if post else 0, _ptr(w_post), _ptr(gate),
+        _ld(gate, ld_gate), gate_rows, _gate_act(gate_act), _ptr(w_pre), _ptr(h), _ld(h, ld_h), _ptr(y),
+        _ld(y, ld_y), _ptr(rstd_post), _ptr(rstd_pre), T, D, wide, scale, eps, _stream(stream)))
+
+
+def block_norm_grad_ws_bytes(T, D, gate_rows=0):
+    """Workspace bytes of block_norm_grad (gate_rows 0: no gate)."""
+    return int(lib().foil_block_norm_grad_ws_bytes(T, D, gate_rows))
+
+
+def block_norm_grad(dh, dy, h, u, dresid, du, T, D, ws, rstd_pre=None, w_pre=None, dw_pre=None, post=False,
+                    rstd_post=None, w_post=None, dw_post=None, gate=None, dgate=None, gate_rows=1, gate_act="none",
+                    scale=1.0, fp32=None, ws_bytes=None, ld_dh=0, ld_dy=0, ld_h=0, ld_u=0, ld_gate=0, ld_dresid=0,
+                    ld_du=0, ld_dgate=0, stream=None):
+    """Gradients of block_norm from those of h (dh) and y (dy); outputs that
+    are None are not made.  `ws`: a workspace of block_norm_grad_ws_bytes."""
+    _on_current(dh, dy, h, u, dresid, du, ws, rstd_pre, w_pre, dw_pre, rstd_post, w_post, dw_post, gate, dgate)
+    _dense(ws, rstd_pre, w_pre, dw_pre, rstd_post, w_post, dw_post)
+    wide = _is_fp32(fp32, dh, h, dresid)
+    check(lib().foil_block_norm_grad_dev(
+        _ptr(dh), _ld(dh, ld_dh), _ptr(dy), _ld(dy, ld_dy), _ptr(h), _ld(h, ld_h), _ptr(rstd_pre), _ptr(w_pre),
+        _ptr(u), _ld(u, ld_u), 1 if post else 0, _ptr(rstd_post), _ptr(w_post), _ptr(gate), _ld(gate, ld_gate),
+        gate_rows, _gate_act(gate_act), _ptr(dresid), _ld(dresid, ld_dresid), _ptr(du), _ld(du, ld_du),
+        _ptr(dgate), _ld(dgate, ld_dgate), _ptr(dw_post), _ptr(dw_pre), _ptr(ws), _ws_bytes(ws, ws_bytes), T, D,
+        wide, scale, _stream(stream)))
+
+
+def _ws_bytes(ws, ws_bytes):
+    if ws_bytes is not None:
+        return ws_bytes
+    if ws is None or isinstance(ws, int):
+        return 0
+    return ws.numel() * ws.element_size()
+
+
+def _id_bytes(ids, id_bytes):
+    if isinstance(ids, int) or ids is None:
+        return id_bytes
+    if ids.is_floating_point() or ids.element_size() not in (4, 8):
+        raise FoilError(1, "tt-foil: ids must be 32- or 64-bit integers")
+    return ids.element_size()
+
+
+def embed_rows(ids, table, out, T, V, D, scale=1.0, pad_id=-1, id_bytes=4, fp32=None, ld_table=0, ld_out=0,
+               stream=None):
+    """out[t] = scale * table[ids[t]]; zeros where ids[t] is pad_id.  A bad id
+    gives zeros and DEVERR_BAD_INDEX (see device_error)."""
+    _on_current(ids, table, out)
+    _dense(ids)
+    check(lib().foil_embed_rows_dev(_ptr(ids), _id_bytes(ids, id_bytes), _ptr(table), _ld(table, ld_table), _ptr(out),
+                                    _ld(out, ld_out), T, V, D, _is_fp32(fp32, out), scale, pad_id, _stream(stream)))
+
+
+def embed_rows_grad_ws_bytes(T, V, D):
+    """Workspace bytes of embed_rows_grad."""
+    return int(lib().foil_embed_rows_grad_ws_bytes(T, V, D))
+
+
+def embed_rows_grad(ids, dout, dtable, T, V, D, ws, scale=1.0, pad_id=-1, accumulate=False, id_bytes=4, fp32=None,
+                    ws_bytes=None, ld_dout=0, ld_dtable=0, stream=None):
+    """dtable[v] (fp32) = scale * sum of dout[t] over ids[t] = v, or with
+    `accumulate` added to what is there.  `ws`: a workspace of
+    embed_rows_grad_ws_bytes."""
+    _on_current(ids, dout, dtable, ws)
+    _dense(ids, ws)
+    check(lib().foil_embed_rows_grad_dev(_ptr(ids), _id_bytes(ids, id_bytes), _ptr(dout), _ld(dout, ld_dout),
+                                         _ptr(dtable), _ld(dtable, ld_dtable), T, V, D, _is_fp32(fp32, dout), scale,
+                                         pad_id, 1 if accumulate else 0, _ptr(ws), _ws_bytes(ws, ws_bytes),
+                                         _stream(stream)))
 
 
 def matmul_tiles_host(device, a, b, c, Mt, Kt, Nt, bias=None, relu=False, chunk_rows=0):
