@@ -3,11 +3,20 @@
 // foil_w4_pack_dev in include/foil_c.h.
 #include "w4.cuh"
 
-#include "common.cuh"
+#include "gemm_ptx.cuh"
 
 namespace foil {
 namespace w4 {
 namespace {
+
+using gemm::bulk_load;
+using gemm::cluster_sync;
+using gemm::map_to_rank;
+using gemm::mbar_drain;
+using gemm::mbar_expect_tx;
+using gemm::mbar_init;
+using gemm::mbar_wait;
+using gemm::smem_u32;
 
 // Element index of (row r, column c) in a tile stream of ct tile columns.
 __device__ __forceinline__ uint64_t tile_index(uint32_t r, uint32_t c, uint32_t ct) {
@@ -116,22 +125,294 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* 
     tiles[i] = (uint16_t)bits;
 }
 
-// One warp for each column n and row m.
-__global__ void matvec_kernel(const uint16_t* __restrict__ x, uint64_t ld_x, const uint8_t* __restrict__ packed,
-                              const uint16_t* __restrict__ bias, uint16_t* __restrict__ y, uint64_t ld_y, uint32_t M,
-                              Weights w, uint32_t kb, uint32_t relu) {
-    const uint32_t n = blockIdx.x * (blockDim.x / 32u) + threadIdx.x / 32u, m = blockIdx.y, lane = threadIdx.x % 32u;
-    if (n >= w.N) return;
-    float acc = 0.0f;
-    const uint32_t bytes = block_bytes(w.group, w.zeros);
-    for (uint32_t k = lane; k < w.K; k += 32)
-        acc += bf16_bits_to_f32(x[m * ld_x + k]) * weight(packed, n, k, w, kb, bytes);
-    for (int o = 16; o; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) {
-        if (bias) acc += bf16_bits_to_f32(bias[n]);
-        if (relu && acc < 0.0f) acc = 0.0f;
-        y[m * ld_y + n] = (uint16_t)(cvt_bf16x2(acc, 0.0f) & 0xffffu);
+// ------------------------------------------------------------------ matvec ---
+// y = x W for up to 16 rows of x at a time.  HBM-bound: 4-bit weights are read
+// once, so everything else is laid around that stream.
+//
+//  * A warp takes a tile of 16 columns n and a run of its storage blocks along
+//    k, one contiguous piece of memory, through a ring of its own: bulk copies
+//    of one block each (1056 to 1216 bytes: codes, scales, zero points) into
+//    shared memory, kStages deep, no other warp involved.
+//  * mma.m16n8k16 with the weights as the 16-row operand: 16 + q is made in
+//    bf16 by one shift and one logical operation for two codes (0x4180 is 16,
+//    a code at bits 3..6 of its mantissa adds q, exact), laid out in storage
+//    so that a lane's 16-byte words are its operand registers.  x is the other
+//    operand, one 16-byte shared-memory read for two MMAs.
+//  * The group's scale and zero point come after the MMAs in fp32:
+//    s * (sum (16 + q) x - (16 + z) sum x), sum x of each group made once when
+//    x is staged.  Nothing is rounded to fewer than 32 bits before the output.
+//  * K is split over the CTAs of a cluster (S) where x would not fit one SM's
+//    shared memory, and over the warps of a CTA (WK) where there are few
+//    columns; the parts are added in a fixed order through (distributed)
+//    shared memory.  Clusters take contiguous, near-equal runs of tiles: the
+//    grid is one CTA per SM, whatever N is.
+constexpr int kMvWarps = 16;
+constexpr int kMvThreads = 32 * kMvWarps;
+constexpr uint32_t kMaxSmem = 232448;
+
+struct Matvec {
+    const uint16_t* x;
+    const uint8_t* packed;
+    const uint16_t* bias;
+    uint16_t* y;
+    uint64_t ld_x, ld_y;
+    uint32_t M, K, N, kb, tiles;
+    uint32_t S, WK, stages, pass_tiles;  // split and shared-memory plan (host)
+    uint32_t ks;                         // blocks of k of a CTA, at most
+    uint32_t x_pitch, off_sum, off_red, off_ring, off_bar;
+    uint32_t relu, x_vec;
+    uint32_t* err;
+    uint64_t wait_ns;
+};
+
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Codes number I and I + 4 of a word as 16 + q in bf16.
+template <int I>
+__device__ __forceinline__ uint32_t codes16(uint32_t w) {
+    const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
+    return (v & 0x00780078u) | 0x41804180u;
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
+    asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
+                 : "memory");
+}
+
+// The x rows of this CTA's blocks into shared memory (zeros past M and K) and
+// the sum of each group of each row.
+template <int NT, int GROUP>
+__device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb) {
+    float* sums = reinterpret_cast<float*>(smem + p.off_sum);
+    const uint32_t per_row = nkb * 16u, total = 8u * NT * per_row;  // 16-byte pieces
+    const uint32_t rows = min(p.M - m0, 8u * NT);
+    for (uint32_t i0 = 0; i0 < total; i0 += kMvThreads) {
+        const uint32_t i = i0 + threadIdx.x, row = i / per_row, c = i - row * per_row;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        const uint32_t k = kb0 * kBlockK + c * 8u;
+        if (row < rows && k < p.K) {  // false for i >= total: row >= 8 NT >= rows
+            const uint16_t* src = p.x + (m0 + row) * p.ld_x + k;
+            if (p.x_vec && k + 8u <= p.K) {
+                v = *reinterpret_cast<const uint4*>(src);
+            } else {
+                uint32_t e[8];
+#pragma unroll
+                for (uint32_t j = 0; j < 8; ++j) e[j] = k + j < p.K ? src[j] : 0u;
+                v = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                               pack_bf16x2(e[6], e[7]));
+            }
+        }
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = word_of(v, j);
+            s += bf16_bits_to_f32(w & 0xffffu) + bf16_bits_to_f32(w >> 16);
+        }
+#pragma unroll
+        for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (i < total) {
+            *reinterpret_cast<uint4*>(smem + row * p.x_pitch + c * 16u) = v;
+            if (c % (GROUP / 8) == 0) sums[c / (GROUP / 8) * (8u * NT) + row] = s;
+        }
     }
+}
+
+template <int NT>
+__device__ __forceinline__ void put(const Matvec& p, uint32_t m0, uint32_t tile, uint32_t nt, uint32_t lane,
+                                    const float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t n = tile * 16u + lane / 4u + (j / 2) * 8u, m = m0 + nt * 8u + lane % 4u * 2u + j % 2;
+        if (n >= p.N || m >= p.M) continue;
+        float o = v[j];
+        if (p.bias) o += bf16_bits_to_f32(p.bias[n]);
+        if (p.relu && o < 0.0f) o = 0.0f;
+        p.y[m * p.ld_y + n] = (uint16_t)(cvt_bf16x2(o, 0.0f) & 0xffffu);
+    }
+}
+
+template <int NT, int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_constant__ Matvec p) {
+    constexpr uint32_t kBytes = block_bytes(GROUP, ZEROS);
+    constexpr int kGroups = 128 / GROUP;  // groups of a block
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint32_t abort_word;
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, g = lane / 4u, t = lane % 4u;
+    const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = gridDim.x / p.S;
+    const uint32_t m0 = blockIdx.y * 8u * NT;
+    // This CTA's blocks of k and its cluster's tiles.
+    const uint32_t kb0 = (uint32_t)((uint64_t)p.kb * rank / p.S);
+    const uint32_t nkb = (uint32_t)((uint64_t)p.kb * (rank + 1) / p.S) - kb0;
+    const uint32_t t0 = (uint32_t)((uint64_t)p.tiles * cluster / clusters);
+    const uint32_t t1 = (uint32_t)((uint64_t)p.tiles * (cluster + 1) / clusters);
+    // This warp's share: tiles t0 + wn, + WN, ... and blocks [b0, b1) of kb0 ...
+    const uint32_t WN = kMvWarps / p.WK, wn = warp / p.WK, wk = warp % p.WK;
+    const uint32_t b0 = nkb * wk / p.WK, nb = nkb * (wk + 1) / p.WK - b0;
+    const bool joined = p.S * p.WK > 1;
+
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + p.off_bar) + warp * p.stages;
+    uint8_t* ring = smem + p.off_ring + warp * p.stages * kBytes;
+    volatile uint32_t* abort_flag = &abort_word;
+    if (lane == 0)
+        for (uint32_t i = 0; i < p.stages; ++i) mbar_init(&bar[i], 1);
+    if (threadIdx.x == 0) abort_word = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncwarp();
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+
+    // The warp's blocks in order: (tile, block) -> load counter.
+    const uint32_t my_tiles = t0 + wn < t1 ? (t1 - t0 - wn + WN - 1) / WN : 0u;
+    const uint64_t loads = (uint64_t)my_tiles * nb;
+    uint64_t issued = 0;
+    uint32_t is_tile = t0 + wn, is_block = 0, is_stage = 0;
+    auto issue = [&] {  // lane 0
+        const uint8_t* src = p.packed + ((uint64_t)is_tile * p.kb + kb0 + b0 + is_block) * kBytes;
+        mbar_expect_tx(&bar[is_stage], kBytes);
+        bulk_load(smem_u32(ring + is_stage * kBytes), src, kBytes, &bar[is_stage]);
+        if (++is_block == nb) is_block = 0, is_tile += WN;
+        if (++is_stage == p.stages) is_stage = 0;
+        ++issued;
+    };
+    if (lane == 0)
+        while (issued < loads && issued < p.stages) issue();
+
+    stage_x<NT, GROUP>(p, smem, m0, kb0, nkb);
+    if (p.S > 1)
+        cluster_sync();  // also: every CTA of the cluster runs before its memory is written
+    else
+        __syncthreads();
+
+    const float* sums = reinterpret_cast<const float*>(smem + p.off_sum);
+    const uint8_t* xrow = smem + g * p.x_pitch + t * 16u;
+    uint32_t stage = 0, parity = 0;
+    uint64_t used = 0;
+    bool alive = true;
+    for (uint32_t pass = t0; pass < t1; pass += p.pass_tiles) {
+        const uint32_t pass_end = min(t1, pass + p.pass_tiles);
+        // pass_tiles is a multiple of WN, so a warp's tiles keep their stride.
+        for (uint32_t tile = pass + wn; tile < pass_end; tile += WN) {
+            float acc[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
+#pragma unroll 1
+            for (uint32_t b = 0; b < nb; ++b) {
+                if (alive) alive = mbar_wait(&bar[stage], parity, abort_flag, p.err, p.wait_ns);
+                if (!__all_sync(0xffffffffu, alive)) {  // gave up: no more reads, the barriers below still met
+                    alive = false;
+                    break;
+                }
+                const uint8_t* blk = ring + stage * kBytes;
+                const uint4 wa = *reinterpret_cast<const uint4*>(blk + lane * 16u);
+                const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512u + lane * 16u);
+#pragma unroll
+                for (int gi = 0; gi < kGroups; ++gi) {
+                    float part[NT][4];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
+#pragma unroll
+                    for (int q = gi * (GROUP / 32); q < (gi + 1) * (GROUP / 32); ++q) {
+                        const uint32_t a = word_of(wa, q), c = word_of(wb, q);
+                        const uint32_t a0 = codes16<0>(a), a1 = codes16<1>(a), a2 = codes16<2>(a), a3 = codes16<3>(a);
+                        const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c), c3 = codes16<3>(c);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const uint4 xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch +
+                                                                             (b0 + b) * 256u + q * 64u);
+                            mma_bf16(part[n], a0, c0, a1, c1, xv.x, xv.y);
+                            mma_bf16(part[n], a2, c2, a3, c3, xv.z, xv.w);
+                        }
+                    }
+                    const uint16_t* sc = reinterpret_cast<const uint16_t*>(blk + kCodeBytes) + gi * 16;
+                    const float s0 = bf16_bits_to_f32(sc[g]), s1 = bf16_bits_to_f32(sc[g + 8]);
+                    float z0 = 24.0f, z1 = 24.0f;
+                    if constexpr (ZEROS) {
+                        const uint8_t* zp = blk + kCodeBytes + 32 * kGroups + gi * 16;
+                        z0 = 16.0f + (float)zp[g], z1 = 16.0f + (float)zp[g + 8];
+                    }
+                    const float* xs = sums + ((b0 + b) * kGroups + gi) * (8u * NT) + 2u * t;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 x2 = *reinterpret_cast<const float2*>(xs + 8 * n);
+                        acc[n][0] = fmaf(s0, fmaf(-z0, x2.x, part[n][0]), acc[n][0]);
+                        acc[n][1] = fmaf(s0, fmaf(-z0, x2.y, part[n][1]), acc[n][1]);
+                        acc[n][2] = fmaf(s1, fmaf(-z1, x2.x, part[n][2]), acc[n][2]);
+                        acc[n][3] = fmaf(s1, fmaf(-z1, x2.y, part[n][3]), acc[n][3]);
+                    }
+                }
+                __syncwarp();  // every lane has read the stage
+                ++used;
+                if (lane == 0 && issued < loads) issue();
+                if (++stage == p.stages) stage = 0, parity ^= 1u;
+            }
+            if (!joined) {
+                if (alive)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) put<NT>(p, m0, tile, n, lane, acc[n]);
+                continue;
+            }
+            // Tile i of the pass belongs to CTA i % S, place i / S, part rank * WK + wk.
+            const uint32_t i = tile - pass;
+            uint8_t* slot = smem + p.off_red + (((i / p.S) * p.S + rank) * p.WK + wk) * (512u * NT) + lane * 16u;
+            if (p.S > 1) {
+                const uint32_t dst = map_to_rank(slot, i % p.S);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) st_cluster_f4(dst + 512u * n, acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+            } else {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    *reinterpret_cast<float4*>(slot + 512u * n) =
+                        make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+            }
+        }
+        if (!joined) continue;
+        if (p.S > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+        // Add the parts of this CTA's tiles in order and finish them.
+        const uint32_t n_pass = pass_end - pass;
+        const uint32_t mine = n_pass > rank ? (n_pass - rank + p.S - 1) / p.S : 0u, parts = p.S * p.WK;
+        for (uint32_t i = warp; i < mine * NT; i += kMvWarps) {
+            const uint8_t* slot = smem + p.off_red + (i / NT) * parts * (512u * NT) + (i % NT) * 512u + lane * 16u;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (uint32_t k = 0; k < parts; ++k) {
+                const float4 f = *reinterpret_cast<const float4*>(slot + k * (512u * NT));
+                v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
+            }
+            if (*abort_flag == 0u) put<NT>(p, m0, pass + (i / NT) * p.S + rank, i % NT, lane, v);
+        }
+        if (pass_end < t1) {  // the places are free again
+            if (p.S > 1)
+                cluster_sync();
+            else
+                __syncthreads();
+        }
+    }
+    // After a wait that gave up: this warp's copies in flight, bounded.
+    if (lane == 0)
+        for (; used < issued; ++used) {
+            mbar_drain(&bar[used % p.stages], (uint32_t)(used / p.stages) & 1u, p.wait_ns);
+        }
+}
+
+using MatvecKernel = void (*)(const Matvec);
+template <int NT>
+MatvecKernel pick_matvec(const Weights& w) {
+    if (w.group == 32) return w.zeros ? matvec_kernel<NT, 32, true> : matvec_kernel<NT, 32, false>;
+    if (w.group == 64) return w.zeros ? matvec_kernel<NT, 64, true> : matvec_kernel<NT, 64, false>;
+    return w.zeros ? matvec_kernel<NT, 128, true> : matvec_kernel<NT, 128, false>;
 }
 
 uint32_t blocks_k(const Weights& w) { return (w.K + kBlockK - 1) / kBlockK; }
@@ -165,12 +446,78 @@ cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weigh
     return count(cudaGetLastError());
 }
 
+// The split of K over the CTAs of a cluster (S) and the warps of a CTA (WK):
+// the one whose busiest warp reads the fewest storage blocks, among those
+// whose slice of x fits.  A cluster barrier costs about as much as two blocks
+// a warp, the join of a CTA's warps about half a block.
+static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, uint32_t sms) {
+    const uint32_t width = 8 * nt;
+    float best = 0.0f;
+    for (uint32_t S = 1; S <= 8; S *= 2) {
+        const uint32_t ks = (p.kb + S - 1) / S;
+        if (S > 1 && S > p.kb) break;
+        const uint32_t pitch = ks * 256 + 64;  // 64 bytes more: rows of an 8-lane read phase on distinct banks
+        const uint32_t off_sum = width * pitch, sums = ks * (128 / group) * width * 4;
+        const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
+        const uint32_t clusters = sms / S < p.tiles ? sms / S : p.tiles;
+        const uint32_t tc = (p.tiles + clusters - 1) / clusters;
+        for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
+            const uint32_t wn = kMvWarps / wk, units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk);
+            // Ring: up to 6 stages a warp, at least 2; the rest joins tiles.
+            const uint32_t slot = S * wk * 512 * nt;  // one tile's parts
+            const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * slot : 0;
+            const uint32_t per_stage = kMvWarps * (bytes + 8);
+            if (off_red + min_red + 2 * per_stage > kMaxSmem - 1024) continue;
+            uint32_t stages = (kMaxSmem - 1024 - off_red - min_red) / per_stage;
+            stages = stages > 6 ? 6 : stages;
+            uint32_t red = kMaxSmem - 1024 - off_red - stages * per_stage;
+            uint32_t tiles_pass = tc;
+            if (S * wk > 1) {
+                const uint32_t cap = red / slot * S;
+                if (cap < tc) tiles_pass = cap / wn * wn;
+                red = (tiles_pass + S - 1) / S * slot;
+            } else {
+                red = 0;
+            }
+            const uint32_t passes = (tc + tiles_pass - 1) / tiles_pass;
+            const float cost = units + passes * (S > 1 ? 2.0f : wk > 1 ? 0.5f : 0.0f);
+            if (best > 0.0f && cost >= best) continue;
+            best = cost;
+            p.S = S, p.WK = wk, p.stages = stages, p.ks = ks, p.x_pitch = pitch, p.off_sum = off_sum;
+            p.off_red = off_red, p.off_ring = (off_red + red + 127) / 128 * 128;
+            p.off_bar = p.off_ring + (kMvWarps * stages * bytes + 7) / 8 * 8;
+            p.pass_tiles = tiles_pass < tc ? tiles_pass : (tc + wn - 1) / wn * wn;
+        }
+    }
+    return best > 0.0f;
+}
+
 cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, const uint16_t* bias, uint16_t* y,
                    uint64_t ld_y, uint32_t M, const Weights& w, bool relu, uint32_t* err, cudaStream_t s) {
-    (void)err;
-    matvec_kernel<<<dim3((w.N + 7) / 8, M), 256, 0, s>>>(x, ld_x, packed, bias, y, ld_y, M, w, blocks_k(w),
-                                                         relu ? 1u : 0u);
-    return count(cudaGetLastError());
+    Matvec p{};
+    p.x = x, p.packed = packed, p.bias = bias, p.y = y, p.ld_x = ld_x, p.ld_y = ld_y, p.M = M, p.K = w.K, p.N = w.N;
+    p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0, p.err = err;
+    p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0, p.wait_ns = foil_wait_limit_ns();
+    const uint32_t nt = M > 8 ? 2 : 1, bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
+    if (!plan_matvec(p, nt, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    const uint32_t smem = p.off_bar + kMvWarps * p.stages * 8;
+    const MatvecKernel kernel = nt == 2 ? pick_matvec<2>(w) : pick_matvec<1>(w);
+    const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512);
+    if (e != cudaSuccess) return e;
+    const uint32_t clusters = sms / p.S < p.tiles ? sms / p.S : p.tiles;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(clusters * p.S, (M + 8 * nt - 1) / (8 * nt), 1);
+    cfg.blockDim = dim3(kMvThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute la[2]{};
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = p.S, la[1].val.clusterDim.y = 1, la[1].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = p.S > 1 ? 2 : 1;
+    return count(cudaLaunchKernelEx(&cfg, kernel, p));
 }
 
 }  // namespace w4
