@@ -9,13 +9,9 @@ namespace foil {
 namespace w4 {
 namespace {
 
-using gemm::bulk_load;
 using gemm::cluster_sync;
+using gemm::cp_async16;
 using gemm::map_to_rank;
-using gemm::mbar_drain;
-using gemm::mbar_expect_tx;
-using gemm::mbar_init;
-using gemm::mbar_wait;
 using gemm::smem_u32;
 
 // Element index of (row r, column c) in a tile stream of ct tile columns.
@@ -130,9 +126,12 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* 
 // once, so everything else is laid around that stream.
 //
 //  * A warp takes a tile of 16 columns n and a run of its storage blocks along
-//    k, one contiguous piece of memory, through a ring of its own: bulk copies
-//    of one block each (1056 to 1216 bytes: codes, scales, zero points) into
-//    shared memory, kStages deep, no other warp involved.
+//    k, one contiguous piece of memory, through a ring of its own: 16-byte
+//    asynchronous copies, one commit group a block (1056 to 1216 bytes: codes,
+//    scales, zero points), 6 blocks ahead (3 where x takes the memory), no
+//    other warp involved.
+//    (Bulk copies of one block each, measured: 80 to 140 ns of an SM's copy
+//    engine apiece, 1.2 to 2 TB/s in all.)
 //  * mma.m16n8k16 with the weights as the 16-row operand: 16 + q is made in
 //    bf16 by one shift and one logical operation for two codes (0x4180 is 16,
 //    a code at bits 3..6 of its mantissa adds q, exact), laid out in storage
@@ -148,6 +147,7 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* 
 //    grid is one CTA per SM, whatever N is.
 constexpr int kMvWarps = 16;
 constexpr int kMvThreads = 32 * kMvWarps;
+constexpr int kMvAhead = 6, kMvAheadShort = 3;  // blocks in flight of a warp
 constexpr uint32_t kMaxSmem = 232448;
 
 struct Matvec {
@@ -159,10 +159,8 @@ struct Matvec {
     uint32_t M, K, N, kb, tiles;
     uint32_t S, WK, stages, pass_tiles;  // split and shared-memory plan (host)
     uint32_t ks;                         // blocks of k of a CTA, at most
-    uint32_t x_pitch, off_sum, off_red, off_ring, off_bar;
+    uint32_t x_pitch, off_sum, off_red, off_ring;
     uint32_t relu, x_vec;
-    uint32_t* err;
-    uint64_t wait_ns;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -186,18 +184,19 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, f
                  : "memory");
 }
 
-// The x rows of this CTA's blocks into shared memory (zeros past M and K) and
-// the sum of each group of each row.
-template <int NT, int GROUP>
+// The x rows of this CTA's blocks into shared memory (zeros past K) and the sum
+// of each group of each row, times -24 (codes stand as 16 + q, and q - 8 is
+// wanted) where there are no zero points.
+template <int NT, int GROUP, bool ZEROS>
 __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb) {
     float* sums = reinterpret_cast<float*>(smem + p.off_sum);
-    const uint32_t per_row = nkb * 16u, total = 8u * NT * per_row;  // 16-byte pieces
     const uint32_t rows = min(p.M - m0, 8u * NT);
+    const uint32_t per_row = nkb * 16u, total = rows * per_row;  // 16-byte pieces
     for (uint32_t i0 = 0; i0 < total; i0 += kMvThreads) {
         const uint32_t i = i0 + threadIdx.x, row = i / per_row, c = i - row * per_row;
         uint4 v = make_uint4(0, 0, 0, 0);
         const uint32_t k = kb0 * kBlockK + c * 8u;
-        if (row < rows && k < p.K) {  // false for i >= total: row >= 8 NT >= rows
+        if (i < total && k < p.K) {
             const uint16_t* src = p.x + (m0 + row) * p.ld_x + k;
             if (p.x_vec && k + 8u <= p.K) {
                 v = *reinterpret_cast<const uint4*>(src);
@@ -219,7 +218,7 @@ __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t
         for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         if (i < total) {
             *reinterpret_cast<uint4*>(smem + row * p.x_pitch + c * 16u) = v;
-            if (c % (GROUP / 8) == 0) sums[c / (GROUP / 8) * (8u * NT) + row] = s;
+            if (c % (GROUP / 8) == 0) sums[c / (GROUP / 8) * (8u * NT) + row] = ZEROS ? s : -24.0f * s;
         }
     }
 }
@@ -238,12 +237,15 @@ __device__ __forceinline__ void put(const Matvec& p, uint32_t m0, uint32_t tile,
     }
 }
 
+// -(16 + z) for a zero point z, in the bits of a float: 16 + z is 16 with z at
+// bits 19..22 of the mantissa.
+__device__ __forceinline__ float minus16(uint32_t z) { return __uint_as_float(0xc1800000u | (z & 15u) << 19); }
+
 template <int NT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_constant__ Matvec p) {
     constexpr uint32_t kBytes = block_bytes(GROUP, ZEROS);
     constexpr int kGroups = 128 / GROUP;  // groups of a block
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ uint32_t abort_word;
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, g = lane / 4u, t = lane % 4u;
     const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = gridDim.x / p.S;
     const uint32_t m0 = blockIdx.y * 8u * NT;
@@ -257,34 +259,32 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
     const uint32_t b0 = nkb * wk / p.WK, nb = nkb * (wk + 1) / p.WK - b0;
     const bool joined = p.S * p.WK > 1;
 
-    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + p.off_bar) + warp * p.stages;
-    uint8_t* ring = smem + p.off_ring + warp * p.stages * kBytes;
-    volatile uint32_t* abort_flag = &abort_word;
-    if (lane == 0)
-        for (uint32_t i = 0; i < p.stages; ++i) mbar_init(&bar[i], 1);
-    if (threadIdx.x == 0) abort_word = 0u;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncwarp();
+    const uint32_t ring = smem_u32(smem + p.off_ring) + warp * p.stages * kBytes;
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
 
-    // The warp's blocks in order: (tile, block) -> load counter.
-    const uint32_t my_tiles = t0 + wn < t1 ? (t1 - t0 - wn + WN - 1) / WN : 0u;
-    const uint64_t loads = (uint64_t)my_tiles * nb;
-    uint64_t issued = 0;
-    uint32_t is_tile = t0 + wn, is_block = 0, is_stage = 0;
-    auto issue = [&] {  // lane 0
-        const uint8_t* src = p.packed + ((uint64_t)is_tile * p.kb + kb0 + b0 + is_block) * kBytes;
-        mbar_expect_tx(&bar[is_stage], kBytes);
-        bulk_load(smem_u32(ring + is_stage * kBytes), src, kBytes, &bar[is_stage]);
-        if (++is_block == nb) is_block = 0, is_tile += WN;
-        if (++is_stage == p.stages) is_stage = 0;
-        ++issued;
+    // The warp's blocks in order, one commit group each (empty past the end).
+    const uint8_t* src = p.packed + ((uint64_t)(t0 + wn) * p.kb + kb0 + b0) * kBytes + lane * 16u;
+    const uint64_t next_tile = (uint64_t)WN * p.kb * kBytes;
+    uint32_t left = nb ? (t0 + wn < t1 ? (t1 - t0 - wn + WN - 1) / WN : 0u) * nb : 0u;
+    uint32_t is_block = 0, is_dst = ring + lane * 16u;
+    const uint32_t dst_end = is_dst + p.stages * kBytes;
+    auto issue = [&] {
+        if (left) {
+            cp_async16(is_dst, src, 16);
+            cp_async16(is_dst + 512u, src + 512, 16);
+            if (lane < (kBytes - kCodeBytes) / 16u) cp_async16(is_dst + kCodeBytes, src + kCodeBytes, 16);
+            src += kBytes;
+            if (++is_block == nb) is_block = 0, src += next_tile - (uint64_t)nb * kBytes;
+            is_dst += kBytes;
+            if (is_dst == dst_end) is_dst = ring + lane * 16u;
+            --left;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    if (lane == 0)
-        while (issued < loads && issued < p.stages) issue();
+    for (uint32_t i = 0; i < p.stages; ++i) issue();
 
-    stage_x<NT, GROUP>(p, smem, m0, kb0, nkb);
+    stage_x<NT, GROUP, ZEROS>(p, smem, m0, kb0, nkb);
     if (p.S > 1)
         cluster_sync();  // also: every CTA of the cluster runs before its memory is written
     else
@@ -292,9 +292,10 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 
     const float* sums = reinterpret_cast<const float*>(smem + p.off_sum);
     const uint8_t* xrow = smem + g * p.x_pitch + t * 16u;
-    uint32_t stage = 0, parity = 0;
-    uint64_t used = 0;
-    bool alive = true;
+    bool has[NT];  // rows past M: zeros instead of a read
+#pragma unroll
+    for (int n = 0; n < NT; ++n) has[n] = m0 + 8u * n + g < p.M;
+    uint32_t stage = 0;
     for (uint32_t pass = t0; pass < t1; pass += p.pass_tiles) {
         const uint32_t pass_end = min(t1, pass + p.pass_tiles);
         // pass_tiles is a multiple of WN, so a warp's tiles keep their stride.
@@ -306,21 +307,30 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                 for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
 #pragma unroll 1
             for (uint32_t b = 0; b < nb; ++b) {
-                if (alive) alive = mbar_wait(&bar[stage], parity, abort_flag, p.err, p.wait_ns);
-                if (!__all_sync(0xffffffffu, alive)) {  // gave up: no more reads, the barriers below still met
-                    alive = false;
-                    break;
-                }
-                const uint8_t* blk = ring + stage * kBytes;
+                if (p.stages == kMvAhead)
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kMvAhead - 1) : "memory");
+                else
+                    asm volatile("cp.async.wait_group %0;" ::"n"(kMvAheadShort - 1) : "memory");
+                __syncwarp();  // every lane's copies of this block have landed
+                const uint8_t* blk = smem + p.off_ring + (warp * p.stages + stage) * kBytes;
                 const uint4 wa = *reinterpret_cast<const uint4*>(blk + lane * 16u);
                 const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512u + lane * 16u);
 #pragma unroll
                 for (int gi = 0; gi < kGroups; ++gi) {
+                    // Start from minus (16 + z) times the group's sum of x.
+                    const float* xs = sums + ((b0 + b) * kGroups + gi) * (8u * NT) + 2u * t;
                     float part[NT][4];
+                    float z0 = 1.0f, z1 = 1.0f;
+                    if constexpr (ZEROS) {
+                        const uint8_t* zp = blk + kCodeBytes + 32 * kGroups + gi * 16;
+                        z0 = minus16(zp[g]), z1 = minus16(zp[g + 8]);
+                    }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) part[n][j] = 0.0f;
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 x2 = *reinterpret_cast<const float2*>(xs + 8 * n);
+                        part[n][0] = z0 * x2.x, part[n][1] = z0 * x2.y;
+                        part[n][2] = z1 * x2.x, part[n][3] = z1 * x2.y;
+                    }
 #pragma unroll
                     for (int q = gi * (GROUP / 32); q < (gi + 1) * (GROUP / 32); ++q) {
                         const uint32_t a = word_of(wa, q), c = word_of(wb, q);
@@ -328,38 +338,31 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                         const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c), c3 = codes16<3>(c);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const uint4 xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch +
-                                                                             (b0 + b) * 256u + q * 64u);
+                            uint4 xv = make_uint4(0, 0, 0, 0);
+                            if (has[n])
+                                xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch + (b0 + b) * 256u +
+                                                                     q * 64u);
                             mma_bf16(part[n], a0, c0, a1, c1, xv.x, xv.y);
                             mma_bf16(part[n], a2, c2, a3, c3, xv.z, xv.w);
                         }
                     }
                     const uint16_t* sc = reinterpret_cast<const uint16_t*>(blk + kCodeBytes) + gi * 16;
                     const float s0 = bf16_bits_to_f32(sc[g]), s1 = bf16_bits_to_f32(sc[g + 8]);
-                    float z0 = 24.0f, z1 = 24.0f;
-                    if constexpr (ZEROS) {
-                        const uint8_t* zp = blk + kCodeBytes + 32 * kGroups + gi * 16;
-                        z0 = 16.0f + (float)zp[g], z1 = 16.0f + (float)zp[g + 8];
-                    }
-                    const float* xs = sums + ((b0 + b) * kGroups + gi) * (8u * NT) + 2u * t;
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        const float2 x2 = *reinterpret_cast<const float2*>(xs + 8 * n);
-                        acc[n][0] = fmaf(s0, fmaf(-z0, x2.x, part[n][0]), acc[n][0]);
-                        acc[n][1] = fmaf(s0, fmaf(-z0, x2.y, part[n][1]), acc[n][1]);
-                        acc[n][2] = fmaf(s1, fmaf(-z1, x2.x, part[n][2]), acc[n][2]);
-                        acc[n][3] = fmaf(s1, fmaf(-z1, x2.y, part[n][3]), acc[n][3]);
+                        acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
+                        acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
+                        acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
+                        acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
                     }
                 }
-                __syncwarp();  // every lane has read the stage
-                ++used;
-                if (lane == 0 && issued < loads) issue();
-                if (++stage == p.stages) stage = 0, parity ^= 1u;
+                __syncwarp();  // every lane has read the block
+                issue();
+                if (++stage == p.stages) stage = 0;
             }
             if (!joined) {
-                if (alive)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) put<NT>(p, m0, tile, n, lane, acc[n]);
+                for (int n = 0; n < NT; ++n) put<NT>(p, m0, tile, n, lane, acc[n]);
                 continue;
             }
             // Tile i of the pass belongs to CTA i % S, place i / S, part rank * WK + wk.
@@ -391,7 +394,7 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                 const float4 f = *reinterpret_cast<const float4*>(slot + k * (512u * NT));
                 v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
             }
-            if (*abort_flag == 0u) put<NT>(p, m0, pass + (i / NT) * p.S + rank, i % NT, lane, v);
+            put<NT>(p, m0, pass + (i / NT) * p.S + rank, i % NT, lane, v);
         }
         if (pass_end < t1) {  // the places are free again
             if (p.S > 1)
@@ -400,11 +403,6 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                 __syncthreads();
         }
     }
-    // After a wait that gave up: this warp's copies in flight, bounded.
-    if (lane == 0)
-        for (; used < issued; ++used) {
-            mbar_drain(&bar[used % p.stages], (uint32_t)(used / p.stages) & 1u, p.wait_ns);
-        }
 }
 
 using MatvecKernel = void (*)(const Matvec);
@@ -462,15 +460,15 @@ static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, 
         const uint32_t clusters = sms / S < p.tiles ? sms / S : p.tiles;
         const uint32_t tc = (p.tiles + clusters - 1) / clusters;
         for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
-            const uint32_t wn = kMvWarps / wk, units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk);
-            // Ring: up to 6 stages a warp, at least 2; the rest joins tiles.
+            // A tile's set-up and join cost about as much as one block.
+            const uint32_t wn = kMvWarps / wk, units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk + 1);
+            // What the ring leaves joins tiles.
             const uint32_t slot = S * wk * 512 * nt;  // one tile's parts
             const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * slot : 0;
-            const uint32_t per_stage = kMvWarps * (bytes + 8);
-            if (off_red + min_red + 2 * per_stage > kMaxSmem - 1024) continue;
-            uint32_t stages = (kMaxSmem - 1024 - off_red - min_red) / per_stage;
-            stages = stages > 6 ? 6 : stages;
-            uint32_t red = kMaxSmem - 1024 - off_red - stages * per_stage;
+            uint32_t stages = kMvAhead, ring = kMvWarps * stages * bytes;
+            if (off_red + min_red + ring > kMaxSmem - 1024) stages = kMvAheadShort, ring = kMvWarps * stages * bytes;
+            if (off_red + min_red + ring > kMaxSmem - 1024) continue;
+            uint32_t red = kMaxSmem - 1024 - off_red - ring;
             uint32_t tiles_pass = tc;
             if (S * wk > 1) {
                 const uint32_t cap = red / slot * S;
@@ -485,7 +483,6 @@ static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, 
             best = cost;
             p.S = S, p.WK = wk, p.stages = stages, p.ks = ks, p.x_pitch = pitch, p.off_sum = off_sum;
             p.off_red = off_red, p.off_ring = (off_red + red + 127) / 128 * 128;
-            p.off_bar = p.off_ring + (kMvWarps * stages * bytes + 7) / 8 * 8;
             p.pass_tiles = tiles_pass < tc ? tiles_pass : (tc + wn - 1) / wn * wn;
         }
     }
@@ -493,14 +490,14 @@ static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, 
 }
 
 cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, const uint16_t* bias, uint16_t* y,
-                   uint64_t ld_y, uint32_t M, const Weights& w, bool relu, uint32_t* err, cudaStream_t s) {
+                   uint64_t ld_y, uint32_t M, const Weights& w, bool relu, cudaStream_t s) {
     Matvec p{};
     p.x = x, p.packed = packed, p.bias = bias, p.y = y, p.ld_x = ld_x, p.ld_y = ld_y, p.M = M, p.K = w.K, p.N = w.N;
-    p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0, p.err = err;
-    p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0, p.wait_ns = foil_wait_limit_ns();
+    p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0;
+    p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0;
     const uint32_t nt = M > 8 ? 2 : 1, bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
     if (!plan_matvec(p, nt, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
-    const uint32_t smem = p.off_bar + kMvWarps * p.stages * 8;
+    const uint32_t smem = p.off_ring + kMvWarps * p.stages * bytes;
     const MatvecKernel kernel = nt == 2 ? pick_matvec<2>(w) : pick_matvec<1>(w);
     const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512);
     if (e != cudaSuccess) return e;

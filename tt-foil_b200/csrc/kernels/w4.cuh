@@ -33,7 +33,7 @@ cudaError_t quantize_tiles(const uint16_t* tiles, uint8_t* packed, const Weights
 cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weights& w, bool transpose,
                              cudaStream_t s);
 cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, const uint16_t* bias, uint16_t* y,
-                   uint64_t ld_y, uint32_t M, const Weights& w, bool relu, uint32_t* err, cudaStream_t s);
+                   uint64_t ld_y, uint32_t M, const Weights& w, bool relu, cudaStream_t s);
 
 }  // namespace w4
 }  // namespace foil
