@@ -174,7 +174,9 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
 template <int I>
 __device__ __forceinline__ uint32_t codes16(uint32_t w) {
     const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
-    return (v & 0x00780078u) | 0x41804180u;
+    uint32_t r;  // (v & mask) | magic in one instruction
+    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(0x00780078u), "r"(0x41804180u));
+    return r;
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -184,14 +186,16 @@ __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, f
                  : "memory");
 }
 
-// The x rows of this CTA's blocks into shared memory (zeros past K) and the sum
-// of each group of each row, times -24 (codes stand as 16 + q, and q - 8 is
+// The x rows of this CTA's blocks into shared memory (zeros past M and K) and
+// the sum of each group of each row, times -24 (codes stand as 16 + q, and q - 8 is
 // wanted) where there are no zero points.
 template <int NT, int GROUP, bool ZEROS>
 __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb) {
     float* sums = reinterpret_cast<float*>(smem + p.off_sum);
     const uint32_t rows = min(p.M - m0, 8u * NT);
     const uint32_t per_row = nkb * 16u, total = rows * per_row;  // 16-byte pieces
+    for (uint32_t i = rows * p.x_pitch + threadIdx.x * 16u; i < 8u * NT * p.x_pitch; i += kMvThreads * 16u)
+        *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
     for (uint32_t i0 = 0; i0 < total; i0 += kMvThreads) {
         const uint32_t i = i0 + threadIdx.x, row = i / per_row, c = i - row * per_row;
         uint4 v = make_uint4(0, 0, 0, 0);
@@ -292,9 +296,6 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 
     const float* sums = reinterpret_cast<const float*>(smem + p.off_sum);
     const uint8_t* xrow = smem + g * p.x_pitch + t * 16u;
-    bool has[NT];  // rows past M: zeros instead of a read
-#pragma unroll
-    for (int n = 0; n < NT; ++n) has[n] = m0 + 8u * n + g < p.M;
     uint32_t stage = 0;
     for (uint32_t pass = t0; pass < t1; pass += p.pass_tiles) {
         const uint32_t pass_end = min(t1, pass + p.pass_tiles);
@@ -338,10 +339,8 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                         const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c), c3 = codes16<3>(c);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            uint4 xv = make_uint4(0, 0, 0, 0);
-                            if (has[n])
-                                xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch + (b0 + b) * 256u +
-                                                                     q * 64u);
+                            const uint4 xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch +
+                                                                             (b0 + b) * 256u + q * 64u);
                             mma_bf16(part[n], a0, c0, a1, c1, xv.x, xv.y);
                             mma_bf16(part[n], a2, c2, a3, c3, xv.z, xv.w);
                         }
