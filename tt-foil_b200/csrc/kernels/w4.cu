@@ -3,6 +3,8 @@
 // foil_w4_pack_dev in include/foil_c.h.
 #include "w4.cuh"
 
+#include <atomic>
+
 #include "gemm_ptx.cuh"
 
 namespace foil {
@@ -125,12 +127,11 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* 
 // y = x W for up to 16 rows of x at a time.  HBM-bound: 4-bit weights are read
 // once, so everything else is laid around that stream.
 //
-//  * A warp takes a tile of 16 columns n and a run of its storage blocks along
-//    k, one contiguous piece of memory, through a ring of its own: 16-byte
-//    asynchronous copies, one commit group a block (1056 to 1216 bytes: codes,
-//    scales, zero points), 6 blocks ahead (3 where x takes the memory), no
-//    other warp involved.
-//    (Bulk copies of one block each, measured: 80 to 140 ns of an SM's copy
+//  * A warp takes one or two tiles of 16 columns n (what it reads of x serves
+//    both) and a run of their storage blocks along k, one contiguous piece of
+//    memory each, through a ring of its own: 16-byte asynchronous copies, 4 to
+//    6 blocks (1056 to 1216 bytes each: codes, scales, zero points) ahead, no
+//    other warp involved.  (Bulk copies of one block each, measured: 80 to 140 ns of an SM's copy
 //    engine apiece, 1.2 to 2 TB/s in all.)
 //  * mma.m16n8k16 with the weights as the 16-row operand: 16 + q is made in
 //    bf16 by one shift and one logical operation for two codes (0x4180 is 16,
@@ -147,7 +148,10 @@ __global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* 
 //    grid is one CTA per SM, whatever N is.
 constexpr int kMvWarps = 16;
 constexpr int kMvThreads = 32 * kMvWarps;
-constexpr int kMvAhead = 6, kMvAheadShort = 3;  // blocks in flight of a warp
+// Tiles of a warp at a time: two for up to 8 rows of x, one for up to 16 (the
+// accumulators of two would not fit the registers); and the slots in flight.
+__host__ __device__ constexpr int mv_tiles(int nt) { return nt == 1 ? 2 : 1; }
+__host__ __device__ constexpr int mv_ahead(int rt) { return rt == 2 ? 3 : 4; }
 constexpr uint32_t kMaxSmem = 232448;
 
 struct Matvec {
@@ -157,9 +161,8 @@ struct Matvec {
     uint16_t* y;
     uint64_t ld_x, ld_y;
     uint32_t M, K, N, kb, tiles;
-    uint32_t S, WK, stages, pass_tiles;  // split and shared-memory plan (host)
-    uint32_t ks;                         // blocks of k of a CTA, at most
-    uint32_t x_pitch, off_sum, off_red, off_ring;
+    uint32_t S, WK, clusters, pass_runs;           // split (host)
+    uint32_t x_pitch, off_sum, off_red, off_ring;  // shared-memory plan (host)
     uint32_t relu, x_vec;
 };
 
@@ -245,48 +248,56 @@ __device__ __forceinline__ void put(const Matvec& p, uint32_t m0, uint32_t tile,
 // bits 19..22 of the mantissa.
 __device__ __forceinline__ float minus16(uint32_t z) { return __uint_as_float(0xc1800000u | (z & 15u) << 19); }
 
-template <int NT, int GROUP, bool ZEROS>
+template <int NT, int RT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_constant__ Matvec p) {
     constexpr uint32_t kBytes = block_bytes(GROUP, ZEROS);
     constexpr int kGroups = 128 / GROUP;  // groups of a block
+    constexpr int kAhead = mv_ahead(RT);
+    constexpr uint32_t kSlot = RT * kBytes, kPlace = 512 * RT * NT;
     extern __shared__ __align__(128) uint8_t smem[];
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, g = lane / 4u, t = lane % 4u;
-    const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = gridDim.x / p.S;
+    const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = p.clusters;
     const uint32_t m0 = blockIdx.y * 8u * NT;
-    // This CTA's blocks of k and its cluster's tiles.
+    // This CTA's blocks of k and its cluster's tiles, in runs of RT.
     const uint32_t kb0 = (uint32_t)((uint64_t)p.kb * rank / p.S);
     const uint32_t nkb = (uint32_t)((uint64_t)p.kb * (rank + 1) / p.S) - kb0;
     const uint32_t t0 = (uint32_t)((uint64_t)p.tiles * cluster / clusters);
     const uint32_t t1 = (uint32_t)((uint64_t)p.tiles * (cluster + 1) / clusters);
-    // This warp's share: tiles t0 + wn, + WN, ... and blocks [b0, b1) of kb0 ...
+    const uint32_t runs = (t1 - t0 + RT - 1) / RT;
+    // This warp's share: runs wn, wn + WN, ... and blocks [b0, b0 + nb) of kb0 ...
     const uint32_t WN = kMvWarps / p.WK, wn = warp / p.WK, wk = warp % p.WK;
     const uint32_t b0 = nkb * wk / p.WK, nb = nkb * (wk + 1) / p.WK - b0;
     const bool joined = p.S * p.WK > 1;
+    const uint64_t tile_bytes = (uint64_t)p.kb * kBytes;
 
-    const uint32_t ring = smem_u32(smem + p.off_ring) + warp * p.stages * kBytes;
+    uint8_t* const ring = smem + p.off_ring + warp * (kAhead * kSlot);
+    uint8_t* const ring_end = ring + kAhead * kSlot;
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
 
-    // The warp's blocks in order, one commit group each (empty past the end).
-    const uint8_t* src = p.packed + ((uint64_t)(t0 + wn) * p.kb + kb0 + b0) * kBytes + lane * 16u;
-    const uint64_t next_tile = (uint64_t)WN * p.kb * kBytes;
-    uint32_t left = nb ? (t0 + wn < t1 ? (t1 - t0 - wn + WN - 1) / WN : 0u) * nb : 0u;
-    uint32_t is_block = 0, is_dst = ring + lane * 16u;
-    const uint32_t dst_end = is_dst + p.stages * kBytes;
-    auto issue = [&] {
-        if (left) {
-            cp_async16(is_dst, src, 16);
-            cp_async16(is_dst + 512u, src + 512, 16);
-            if (lane < (kBytes - kCodeBytes) / 16u) cp_async16(is_dst + kCodeBytes, src + kCodeBytes, 16);
+    // The warp's blocks in order, one commit group for a block of each tile of
+    // the run (empty past the end).
+    uint32_t is_run = wn, is_block = 0;
+    const uint8_t* src = p.packed + (uint64_t)(t0 + RT * wn) * tile_bytes + (uint64_t)(kb0 + b0) * kBytes + lane * 16u;
+    auto issue = [&](uint8_t* slot) {
+        if (is_run < runs && nb) {
+            const uint32_t dst = smem_u32(slot) + lane * 16u;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                if (r && t0 + RT * is_run + r >= t1) break;
+                const uint8_t* s = src + r * tile_bytes;
+                cp_async16(dst + r * kBytes, s, 16);
+                cp_async16(dst + r * kBytes + 512u, s + 512, 16);
+                if (lane < (kBytes - kCodeBytes) / 16u)
+                    cp_async16(dst + r * kBytes + kCodeBytes, s + kCodeBytes, 16);
+            }
             src += kBytes;
-            if (++is_block == nb) is_block = 0, src += next_tile - (uint64_t)nb * kBytes;
-            is_dst += kBytes;
-            if (is_dst == dst_end) is_dst = ring + lane * 16u;
-            --left;
+            if (++is_block == nb) is_block = 0, is_run += WN, src += RT * WN * tile_bytes - (uint64_t)nb * kBytes;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (uint32_t i = 0; i < p.stages; ++i) issue();
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) issue(ring + i * kSlot);
 
     stage_x<NT, GROUP, ZEROS>(p, smem, m0, kb0, nkb);
     if (p.S > 1)
@@ -294,108 +305,124 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
     else
         __syncthreads();
 
-    const float* sums = reinterpret_cast<const float*>(smem + p.off_sum);
-    const uint8_t* xrow = smem + g * p.x_pitch + t * 16u;
-    uint32_t stage = 0;
-    for (uint32_t pass = t0; pass < t1; pass += p.pass_tiles) {
-        const uint32_t pass_end = min(t1, pass + p.pass_tiles);
-        // pass_tiles is a multiple of WN, so a warp's tiles keep their stride.
-        for (uint32_t tile = pass + wn; tile < pass_end; tile += WN) {
-            float acc[NT][4];
+    const uint8_t* const xrow = smem + g * p.x_pitch + t * 16u + b0 * 256u;
+    const float* const sums =
+        reinterpret_cast<const float*>(smem + p.off_sum) + b0 * kGroups * (8u * NT) + 2u * t;
+    uint8_t* slot = ring;
+    for (uint32_t pass = 0; pass < runs; pass += p.pass_runs) {
+        const uint32_t pass_end = min(runs, pass + p.pass_runs);
+        // pass_runs is a multiple of WN, so a warp's runs keep their stride.
+        for (uint32_t run = pass + wn; run < pass_end; run += WN) {
+            const uint32_t tile = t0 + RT * run, n_tiles = min((uint32_t)RT, t1 - tile);
+            float acc[RT][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[n][j] = 0.0f;
+            for (int i = 0; i < 4 * RT * NT; ++i) acc[i / (4 * NT)][i / 4 % NT][i % 4] = 0.0f;
+            const uint8_t* xb = xrow;
+            const float* xs = sums;
 #pragma unroll 1
-            for (uint32_t b = 0; b < nb; ++b) {
-                if (p.stages == kMvAhead)
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kMvAhead - 1) : "memory");
-                else
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kMvAheadShort - 1) : "memory");
-                __syncwarp();  // every lane's copies of this block have landed
-                const uint8_t* blk = smem + p.off_ring + (warp * p.stages + stage) * kBytes;
-                const uint4 wa = *reinterpret_cast<const uint4*>(blk + lane * 16u);
-                const uint4 wb = *reinterpret_cast<const uint4*>(blk + 512u + lane * 16u);
+            for (uint32_t b = 0; b < nb; ++b, xb += 256, xs += kGroups * 8 * NT) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+                __syncwarp();  // every lane's copies have landed
+                uint4 wa[RT], wb[RT];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    wa[r] = *reinterpret_cast<const uint4*>(slot + r * kBytes + lane * 16u);
+                    wb[r] = *reinterpret_cast<const uint4*>(slot + r * kBytes + 512u + lane * 16u);
+                }
 #pragma unroll
                 for (int gi = 0; gi < kGroups; ++gi) {
-                    // Start from minus (16 + z) times the group's sum of x.
-                    const float* xs = sums + ((b0 + b) * kGroups + gi) * (8u * NT) + 2u * t;
-                    float part[NT][4];
-                    float z0 = 1.0f, z1 = 1.0f;
-                    if constexpr (ZEROS) {
-                        const uint8_t* zp = blk + kCodeBytes + 32 * kGroups + gi * 16;
-                        z0 = minus16(zp[g]), z1 = minus16(zp[g + 8]);
-                    }
+                    float part[RT][NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        const float2 x2 = *reinterpret_cast<const float2*>(xs + 8 * n);
-                        part[n][0] = z0 * x2.x, part[n][1] = z0 * x2.y;
-                        part[n][2] = z1 * x2.x, part[n][3] = z1 * x2.y;
+                    for (int r = 0; r < RT; ++r) {
+                        // Start from minus (16 + z) times the group's sum of x.
+                        float z0 = 1.0f, z1 = 1.0f;
+                        if constexpr (ZEROS) {
+                            const uint8_t* zp = slot + r * kBytes + kCodeBytes + 32 * kGroups + gi * 16;
+                            z0 = minus16(zp[g]), z1 = minus16(zp[g + 8]);
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            const float2 x2 = *reinterpret_cast<const float2*>(xs + (gi * NT + n) * 8);
+                            part[r][n][0] = z0 * x2.x, part[r][n][1] = z0 * x2.y;
+                            part[r][n][2] = z1 * x2.x, part[r][n][3] = z1 * x2.y;
+                        }
                     }
 #pragma unroll
                     for (int q = gi * (GROUP / 32); q < (gi + 1) * (GROUP / 32); ++q) {
-                        const uint32_t a = word_of(wa, q), c = word_of(wb, q);
-                        const uint32_t a0 = codes16<0>(a), a1 = codes16<1>(a), a2 = codes16<2>(a), a3 = codes16<3>(a);
-                        const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c), c3 = codes16<3>(c);
+                        uint4 xv[NT];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            const uint4 xv = *reinterpret_cast<const uint4*>(xrow + n * 8u * p.x_pitch +
-                                                                             (b0 + b) * 256u + q * 64u);
-                            mma_bf16(part[n], a0, c0, a1, c1, xv.x, xv.y);
-                            mma_bf16(part[n], a2, c2, a3, c3, xv.z, xv.w);
+                        for (int n = 0; n < NT; ++n)
+                            xv[n] = *reinterpret_cast<const uint4*>(xb + n * 8u * p.x_pitch + q * 64u);
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) {
+                            if (r && r >= (int)n_tiles) break;
+                            const uint32_t a = word_of(wa[r], q), c = word_of(wb[r], q);
+                            const uint32_t a0 = codes16<0>(a), a1 = codes16<1>(a), a2 = codes16<2>(a),
+                                           a3 = codes16<3>(a);
+                            const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c),
+                                           c3 = codes16<3>(c);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma_bf16(part[r][n], a0, c0, a1, c1, xv[n].x, xv[n].y);
+                                mma_bf16(part[r][n], a2, c2, a3, c3, xv[n].z, xv[n].w);
+                            }
                         }
                     }
-                    const uint16_t* sc = reinterpret_cast<const uint16_t*>(blk + kCodeBytes) + gi * 16;
-                    const float s0 = bf16_bits_to_f32(sc[g]), s1 = bf16_bits_to_f32(sc[g + 8]);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        acc[n][0] = fmaf(s0, part[n][0], acc[n][0]);
-                        acc[n][1] = fmaf(s0, part[n][1], acc[n][1]);
-                        acc[n][2] = fmaf(s1, part[n][2], acc[n][2]);
-                        acc[n][3] = fmaf(s1, part[n][3], acc[n][3]);
+                    for (int r = 0; r < RT; ++r) {
+                        const uint16_t* sc = reinterpret_cast<const uint16_t*>(slot + r * kBytes + kCodeBytes) + gi * 16;
+                        const float s0 = bf16_bits_to_f32(sc[g]), s1 = bf16_bits_to_f32(sc[g + 8]);
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            acc[r][n][0] = fmaf(s0, part[r][n][0], acc[r][n][0]);
+                            acc[r][n][1] = fmaf(s0, part[r][n][1], acc[r][n][1]);
+                            acc[r][n][2] = fmaf(s1, part[r][n][2], acc[r][n][2]);
+                            acc[r][n][3] = fmaf(s1, part[r][n][3], acc[r][n][3]);
+                        }
                     }
                 }
-                __syncwarp();  // every lane has read the block
-                issue();
-                if (++stage == p.stages) stage = 0;
+                __syncwarp();  // every lane has read the slot
+                issue(slot);
+                slot += kSlot;
+                if (slot == ring_end) slot = ring;
             }
             if (!joined) {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) put<NT>(p, m0, tile, n, lane, acc[n]);
+                for (int r = 0; r < RT; ++r)
+                    if (r < (int)n_tiles)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) put<NT>(p, m0, tile + r, n, lane, acc[r][n]);
                 continue;
             }
-            // Tile i of the pass belongs to CTA i % S, place i / S, part rank * WK + wk.
-            const uint32_t i = tile - pass;
-            uint8_t* slot = smem + p.off_red + (((i / p.S) * p.S + rank) * p.WK + wk) * (512u * NT) + lane * 16u;
-            if (p.S > 1) {
-                const uint32_t dst = map_to_rank(slot, i % p.S);
+            // Run i of the pass belongs to CTA i % S, place i / S, part rank * WK + wk.
+            const uint32_t i = run - pass;
+            uint8_t* place = smem + p.off_red + (((i / p.S) * p.S + rank) * p.WK + wk) * kPlace + lane * 16u;
+            const uint32_t dst = p.S > 1 ? map_to_rank(place, i % p.S) : smem_u32(place);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) st_cluster_f4(dst + 512u * n, acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-            } else {
+            for (int r = 0; r < RT; ++r)
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
-                    *reinterpret_cast<float4*>(slot + 512u * n) =
-                        make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-            }
+                    st_cluster_f4(dst + 512u * (r * NT + n), acc[r][n][0], acc[r][n][1], acc[r][n][2], acc[r][n][3]);
         }
         if (!joined) continue;
         if (p.S > 1)
             cluster_sync();
         else
             __syncthreads();
-        // Add the parts of this CTA's tiles in order and finish them.
+        // Add the parts of this CTA's runs in order and finish them.
         const uint32_t n_pass = pass_end - pass;
         const uint32_t mine = n_pass > rank ? (n_pass - rank + p.S - 1) / p.S : 0u, parts = p.S * p.WK;
-        for (uint32_t i = warp; i < mine * NT; i += kMvWarps) {
-            const uint8_t* slot = smem + p.off_red + (i / NT) * parts * (512u * NT) + (i % NT) * 512u + lane * 16u;
+        for (uint32_t i = warp; i < mine * RT * NT; i += kMvWarps) {
+            const uint32_t place = i / (RT * NT), tile = t0 + RT * (pass + place * p.S + rank) + i / NT % RT;
+            const uint8_t* part = smem + p.off_red + place * parts * kPlace + i % (RT * NT) * 512u + lane * 16u;
             float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             for (uint32_t k = 0; k < parts; ++k) {
-                const float4 f = *reinterpret_cast<const float4*>(slot + k * (512u * NT));
+                const float4 f = *reinterpret_cast<const float4*>(part + k * kPlace);
                 v[0] += f.x, v[1] += f.y, v[2] += f.z, v[3] += f.w;
             }
-            put<NT>(p, m0, pass + (i / NT) * p.S + rank, i % NT, lane, v);
+            if (tile < t1) put<NT>(p, m0, tile, i % NT, lane, v);
         }
-        if (pass_end < t1) {  // the places are free again
+        if (pass_end < runs) {  // the places are free again
             if (p.S > 1)
                 cluster_sync();
             else
@@ -407,9 +434,10 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 using MatvecKernel = void (*)(const Matvec);
 template <int NT>
 MatvecKernel pick_matvec(const Weights& w) {
-    if (w.group == 32) return w.zeros ? matvec_kernel<NT, 32, true> : matvec_kernel<NT, 32, false>;
-    if (w.group == 64) return w.zeros ? matvec_kernel<NT, 64, true> : matvec_kernel<NT, 64, false>;
-    return w.zeros ? matvec_kernel<NT, 128, true> : matvec_kernel<NT, 128, false>;
+    constexpr int RT = mv_tiles(NT);
+    if (w.group == 32) return w.zeros ? matvec_kernel<NT, RT, 32, true> : matvec_kernel<NT, RT, 32, false>;
+    if (w.group == 64) return w.zeros ? matvec_kernel<NT, RT, 64, true> : matvec_kernel<NT, RT, 64, false>;
+    return w.zeros ? matvec_kernel<NT, RT, 128, true> : matvec_kernel<NT, RT, 128, false>;
 }
 
 uint32_t blocks_k(const Weights& w) { return (w.K + kBlockK - 1) / kBlockK; }
@@ -443,12 +471,41 @@ cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weigh
     return count(cudaGetLastError());
 }
 
+// Clusters of S CTAs, one CTA on an SM, that run at the same time (74, 33 and
+// 15 of 2, 4 and 8 on 148 SMs: a cluster stays inside a GPC); asked for once
+// for each device.
+static uint32_t resident_clusters(uint32_t S, uint32_t sms) {
+    static std::atomic<uint32_t> known[64][4];
+    int dev = 0;
+    if (S == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / S;
+    std::atomic<uint32_t>& k = known[dev][S == 2 ? 1 : S == 4 ? 2 : 3];
+    uint32_t n = k.load(std::memory_order_relaxed);
+    if (n == 0) {
+        const MatvecKernel kernel = matvec_kernel<1, mv_tiles(1), 128, false>;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(sms / S * S, 1, 1), cfg.blockDim = dim3(kMvThreads, 1, 1);
+        cfg.dynamicSmemBytes = 150000;
+        cudaLaunchAttribute la[1]{};
+        la[0].id = cudaLaunchAttributeClusterDimension;
+        la[0].val.clusterDim.x = S, la[0].val.clusterDim.y = 1, la[0].val.clusterDim.z = 1;
+        cfg.attrs = la, cfg.numAttrs = 1;
+        int got = 0;
+        if (foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512) != cudaSuccess ||
+            cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess || got <= 0) {
+            cudaGetLastError();
+            got = (int)(sms / S);
+        }
+        k.store(n = (uint32_t)got, std::memory_order_relaxed);
+    }
+    return n;
+}
+
 // The split of K over the CTAs of a cluster (S) and the warps of a CTA (WK):
 // the one whose busiest warp reads the fewest storage blocks, among those
 // whose slice of x fits.  A cluster barrier costs about as much as two blocks
 // a warp, the join of a CTA's warps about half a block.
 static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, uint32_t sms) {
-    const uint32_t width = 8 * nt;
+    const uint32_t width = 8 * nt, rt = mv_tiles((int)nt), ring = kMvWarps * mv_ahead((int)rt) * rt * bytes;
     float best = 0.0f;
     for (uint32_t S = 1; S <= 8; S *= 2) {
         const uint32_t ks = (p.kb + S - 1) / S;
@@ -456,33 +513,30 @@ static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, 
         const uint32_t pitch = ks * 256 + 64;  // 64 bytes more: rows of an 8-lane read phase on distinct banks
         const uint32_t off_sum = width * pitch, sums = ks * (128 / group) * width * 4;
         const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
-        const uint32_t clusters = sms / S < p.tiles ? sms / S : p.tiles;
-        const uint32_t tc = (p.tiles + clusters - 1) / clusters;
+        const uint32_t fit = resident_clusters(S, sms), clusters = fit < p.tiles ? fit : p.tiles;
+        const uint32_t tc = ((p.tiles + clusters - 1) / clusters + rt - 1) / rt;  // runs of rt tiles
         for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
-            // A tile's set-up and join cost about as much as one block.
+            // A run's set-up and join cost about as much as one of its steps.
             const uint32_t wn = kMvWarps / wk, units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk + 1);
-            // What the ring leaves joins tiles.
-            const uint32_t slot = S * wk * 512 * nt;  // one tile's parts
-            const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * slot : 0;
-            uint32_t stages = kMvAhead, ring = kMvWarps * stages * bytes;
-            if (off_red + min_red + ring > kMaxSmem - 1024) stages = kMvAheadShort, ring = kMvWarps * stages * bytes;
+            const uint32_t place = S * wk * 512 * rt * nt;  // one run's parts
+            const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * place : 0;
             if (off_red + min_red + ring > kMaxSmem - 1024) continue;
-            uint32_t red = kMaxSmem - 1024 - off_red - ring;
-            uint32_t tiles_pass = tc;
+            // What the ring leaves joins tiles.
+            uint32_t red = kMaxSmem - 1024 - off_red - ring, pass = tc;
             if (S * wk > 1) {
-                const uint32_t cap = red / slot * S;
-                if (cap < tc) tiles_pass = cap / wn * wn;
-                red = (tiles_pass + S - 1) / S * slot;
+                const uint32_t cap = red / place * S;
+                if (cap < tc) pass = cap / wn * wn;
+                red = (pass + S - 1) / S * place;
             } else {
                 red = 0;
             }
-            const uint32_t passes = (tc + tiles_pass - 1) / tiles_pass;
+            const uint32_t passes = (tc + pass - 1) / pass;
             const float cost = units + passes * (S > 1 ? 2.0f : wk > 1 ? 0.5f : 0.0f);
             if (best > 0.0f && cost >= best) continue;
             best = cost;
-            p.S = S, p.WK = wk, p.stages = stages, p.ks = ks, p.x_pitch = pitch, p.off_sum = off_sum;
-            p.off_red = off_red, p.off_ring = (off_red + red + 127) / 128 * 128;
-            p.pass_tiles = tiles_pass < tc ? tiles_pass : (tc + wn - 1) / wn * wn;
+            p.S = S, p.WK = wk, p.clusters = clusters, p.x_pitch = pitch, p.off_sum = off_sum, p.off_red = off_red;
+            p.off_ring = (off_red + red + 127) / 128 * 128;
+            p.pass_runs = pass < tc ? pass : (tc + wn - 1) / wn * wn;
         }
     }
     return best > 0.0f;
@@ -494,15 +548,16 @@ cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, cons
     p.x = x, p.packed = packed, p.bias = bias, p.y = y, p.ld_x = ld_x, p.ld_y = ld_y, p.M = M, p.K = w.K, p.N = w.N;
     p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0;
     p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0;
-    const uint32_t nt = M > 8 ? 2 : 1, bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
-    if (!plan_matvec(p, nt, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
-    const uint32_t smem = p.off_ring + kMvWarps * p.stages * bytes;
+    const uint32_t bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
+    // 16 rows at a time where there are more than 8 and their x fits, else 8.
+    const uint32_t nt = M > 8 && plan_matvec(p, 2, bytes, w.group, sms) ? 2 : 1;
+    if (nt == 1 && !plan_matvec(p, 1, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    const uint32_t rt = mv_tiles((int)nt), smem = p.off_ring + kMvWarps * mv_ahead((int)rt) * rt * bytes;
     const MatvecKernel kernel = nt == 2 ? pick_matvec<2>(w) : pick_matvec<1>(w);
     const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512);
     if (e != cudaSuccess) return e;
-    const uint32_t clusters = sms / p.S < p.tiles ? sms / p.S : p.tiles;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(clusters * p.S, (M + 8 * nt - 1) / (8 * nt), 1);
+    cfg.gridDim = dim3(p.clusters * p.S, (M + 8 * nt - 1) / (8 * nt), 1);
     cfg.blockDim = dim3(kMvThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
