@@ -2,20 +2,26 @@
 // block's gate, its scale and the residual addition; and their gradients.
 // The formulas stand at foil_block_norm_dev in include/foil_c.h.
 //
-// HBM-bound: every tensor is read and written once.  A row lives in the
-// registers of one warp (up to 32 E channels) or one CTA, E channels a thread,
-// and a warp or CTA goes over many rows, the weights in its registers.
-// Channels are moved in vectors of 16 bytes where D, the strides and the
-// pointers allow, else of 4 bytes (even D), else one by one.
+// Bound by HBM, closely followed by instruction issue: every tensor is read
+// and written once, with 10 (forward) to 30 instructions a channel.  A row lives
+// in the registers of one warp, one CTA or a cluster of CTAs (its team), 8 or 16
+// channels a thread; a team goes over many rows, the weights in its registers and
+// the next row on its way while the present one is worked on.  (A ring of three
+// rows in shared memory, tried: 10 to 50 % slower, for the instructions it
+// takes.)  Channels are moved in vectors of 16 bytes where D, the strides and
+// the pointers allow, else of 4 bytes (even D), else one by one.
 #include "block_norm.cuh"
 
 #include <cstring>
 
-#include "common.cuh"
+#include "gemm_ptx.cuh"
 
 namespace foil {
 namespace norm {
 namespace {
+
+using gemm::cluster_sync;
+using gemm::map_to_rank;
 
 // V values of type T (uint16_t: bf16 bits) as loaded.
 template <class T, int V>
@@ -48,144 +54,247 @@ struct Raw {
     }
 };
 
-template <int V>
-__device__ __forceinline__ void put(uint16_t* p, const float* v) {
-    if constexpr (V == 8) {
-        *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]),
-                                                  cvt_bf16x2(v[4], v[5]), cvt_bf16x2(v[6], v[7]));
-    } else if constexpr (V == 2) {
-        *reinterpret_cast<uint32_t*>(p) = cvt_bf16x2(v[0], v[1]);
-    } else {
-        *p = (uint16_t)(cvt_bf16x2(v[0], 0.0f) & 0xffffu);
-    }
+// Two channels at a time: sm_100a multiplies and adds fp32 pairs in one
+// instruction, and these kernels are near the issue limit.
+__device__ __forceinline__ uint64_t bits(float2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ float2 pair_of(uint64_t b) {
+    return make_float2(__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32)));
 }
-template <int V>
-__device__ __forceinline__ void put(float* p, const float* v) {
-    if constexpr (V == 8) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else if constexpr (V == 2) {
-        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
-    } else {
-        *p = v[0];
-    }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair_of(d);
 }
-
-__device__ __forceinline__ float act(float g, uint32_t kind) { return kind ? 1.0f / (1.0f + expf(-g)) : g; }
-
-// The threads that hold one row: a warp, or the whole CTA.
-struct Team {
-    uint32_t size, rank;   // threads, this thread
-    uint32_t index, count; // this team, teams of the grid
-    float* shared;         // 2 x N x 32 floats, CTA teams only
-    uint32_t flip;
-
-    // Sums of N values over the team, the same bits in every thread.
-    template <int N>
-    __device__ __forceinline__ void sum(float (&v)[N]) {
-#pragma unroll
-        for (int o = 16; o; o >>= 1)
-#pragma unroll
-            for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-        if (size == 32u) return;
-        float* part = shared + flip * (N * 32);
-        flip ^= 1u;  // two sets in turn: one barrier a sum
-        if (rank % 32u == 0u)
-#pragma unroll
-            for (int n = 0; n < N; ++n) part[n * 32 + rank / 32u] = v[n];
-        __syncthreads();
-        const uint32_t warps = size / 32u;
-#pragma unroll
-        for (int n = 0; n < N; ++n) {
-            float s = rank % 32u < warps ? part[n * 32 + rank % 32u] : 0.0f;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            v[n] = s;
-        }
-    }
-};
-
-__device__ __forceinline__ Team team_of(uint32_t size, float* shared) {
-    if (size == 32u) {
-        const uint32_t per = blockDim.x / 32u;
-        return Team{32u, threadIdx.x % 32u, blockIdx.x * per + threadIdx.x / 32u, gridDim.x * per, shared, 0u};
-    }
-    return Team{size, threadIdx.x, blockIdx.x, gridDim.x, shared, 0u};
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+    return pair_of(d);
 }
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
+// Channels 2 i and 2 i + 1 of a thread's.
 template <class T, int V, int NV>
-__device__ __forceinline__ void load_row(Raw<T, V> (&r)[NV], const T* p, const Team& t, uint32_t D) {
+__device__ __forceinline__ float2 get2(const Raw<T, V> (&r)[NV], int i) {
+    if constexpr (V == 1) return make_float2(r[2 * i].get(0), r[2 * i + 1].get(0));
+    const Raw<T, V>& v = r[2 * i / V];
+    return make_float2(v.get(2 * i % V), v.get(2 * i % V + 1));
+}
+
+// Channels of vector j, from pairs.
+template <int V>
+__device__ __forceinline__ void put(uint16_t* p, const float2* v, int j) {
+    if constexpr (V == 8) {
+        v += 4 * j;
+        *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(v[0].x, v[0].y), cvt_bf16x2(v[1].x, v[1].y),
+                                                  cvt_bf16x2(v[2].x, v[2].y), cvt_bf16x2(v[3].x, v[3].y));
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<uint32_t*>(p) = cvt_bf16x2(v[j].x, v[j].y);
+    } else {
+        *p = (uint16_t)(cvt_bf16x2(j % 2 ? v[j / 2].y : v[j / 2].x, 0.0f) & 0xffffu);
+    }
+}
+template <int V>
+__device__ __forceinline__ void put(float* p, const float2* v, int j) {
+    if constexpr (V == 8) {
+        v += 4 * j;
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(p) = v[j];
+    } else {
+        *p = j % 2 ? v[j / 2].y : v[j / 2].x;
+    }
+}
+// A row's share of this thread to memory.
+template <int V, int NV, class T, class Team>
+__device__ __forceinline__ void store_row(T* p, const float2 (&v)[V * NV / 2], const Team& t, uint32_t D) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const uint32_t i = (j * t.size + t.rank) * V;
-        if (p && i < D)
-            r[j].load(p + i);
-        else
-            r[j].zero();
+        if (i < D) put<V>(p + i, v, j);
     }
 }
 
-template <class R, int V, int NV, int THREADS>
-__global__ void __launch_bounds__(THREADS) forward_kernel(const Forward p, uint32_t team_size) {
-    __shared__ float shared[64];
-    Team team = team_of(team_size, shared);
-    griddep_wait();  // launched with programmatic stream serialization
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + expf(-g)); }
+__device__ __forceinline__ float2 sigmoid2(float2 g) { return make_float2(sigmoid(g.x), sigmoid(g.y)); }
+
+// The threads that hold one row: a warp, a CTA, or the CTAs of a cluster.
+struct Team {
+    uint32_t size, rank;    // threads, this thread
+    uint32_t ctas;          // CTAs of a team (0: the team is a warp)
+    uint32_t index, count;  // this team, teams of the grid
+    float* shared;          // two sets of kSumFloats floats
+    uint32_t flip;
+
+    // Sums of N (1 to 4) values over the team, the same bits in every thread.
+    // A warp's lanes first halve the values they hold (lanes with bit 16 clear
+    // go on with values 0 and 1, and so on), so four sums take 6 shuffles
+    // instead of 20; then 8 lanes add the warps' sums of one value.
+    template <int N>
+    __device__ __forceinline__ void sum(float (&v)[N]) {
+        constexpr uint32_t kAll = 0xffffffffu;
+        const uint32_t lane = threadIdx.x % 32u;
+        float s;
+        if constexpr (N == 1) {
+            s = v[0];
+#pragma unroll
+            for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+            if (ctas == 0) {
+                v[0] = s;
+                return;
+            }
+        } else {
+            const float v3 = N > 3 ? v[N - 1] : 0.0f, v2 = N > 2 ? v[2] : 0.0f;
+            const bool up = lane & 16u, odd = lane & 8u;
+            const float a = (up ? v2 : v[0]) + __shfl_xor_sync(kAll, up ? v[0] : v2, 16);
+            const float b = (up ? v3 : v[1]) + __shfl_xor_sync(kAll, up ? v[1] : v3, 16);
+            s = (odd ? b : a) + __shfl_xor_sync(kAll, odd ? a : b, 8);
+#pragma unroll
+            for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+        }
+        // s: the warp's sum of value lane / 8 (N > 1).
+        if (ctas) {
+            const uint32_t warps = blockDim.x / 32u, all = warps * ctas;
+            float* part = shared + flip * kSumFloats;  // [value][warp], two sets in turn: one barrier a sum
+            flip ^= 1u;
+            const uint32_t value = N == 1 ? 0u : lane / 8u;
+            if (N == 1 ? lane == 0 : lane % 8u == 0 && value < (uint32_t)N) {
+                float* at = part + value * kMaxTeamWarps + rank / 32u;
+                if (ctas == 1u)
+                    *at = s;
+                else
+                    for (uint32_t c = 0; c < ctas; ++c)
+                        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_rank(at, c)), "f"(s) : "memory");
+            }
+            if (ctas == 1u)
+                __syncthreads();
+            else
+                cluster_sync();
+            s = 0.0f;
+            if (value < (uint32_t)N)
+                for (uint32_t w = lane % 8u; w < all; w += 8u) s += part[value * kMaxTeamWarps + w];
+#pragma unroll
+            for (int o = 4; o; o >>= 1) s += __shfl_xor_sync(kAll, s, o);
+        }
+#pragma unroll
+        for (int n = 0; n < N; ++n) v[n] = __shfl_sync(kAll, s, 8 * n);
+    }
+    static constexpr uint32_t kMaxTeamWarps = 64, kSumFloats = 4 * kMaxTeamWarps;
+};
+
+__device__ __forceinline__ Team team_of(uint32_t ctas, float* shared) {
+    if (ctas == 0) {
+        const uint32_t per = blockDim.x / 32u;
+        return Team{32u, threadIdx.x % 32u, 0u, blockIdx.x * per + threadIdx.x / 32u, gridDim.x * per, shared, 0u};
+    }
+    return Team{ctas * blockDim.x, blockIdx.x % ctas * blockDim.x + threadIdx.x, ctas, blockIdx.x / ctas,
+                gridDim.x / ctas, shared, 0u};
+}
+
+// bf16 weights of the thread's channels; ones where there are none.
+template <int V, int NV>
+__device__ __forceinline__ void load_weights(Raw<uint16_t, V> (&r)[NV], const uint16_t* p, const Team& t, uint32_t D) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t i = (j * t.size + t.rank) * V;
+#pragma unroll
+        for (int k = 0; k < Raw<uint16_t, V>::kWords; ++k) r[j].w[k] = 0x3f803f80u;
+        if (p && i < D) r[j].load(p + i);
+    }
+}
+
+// A thread's channels of row t of a tensor (none: zeros).  Row strides are
+// below 2^32, so the offset is one multiplication.
+template <class T, int V, int NV>
+__device__ __forceinline__ void load_row(Raw<T, V> (&r)[NV], const void* base, uint32_t t, uint64_t ld, const Team& team,
+                                         uint32_t D) {
+    const T* p = static_cast<const T*>(base) + (uint64_t)t * (uint32_t)ld + team.rank * V;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        r[j].zero();
+        if (base && (j * team.size + team.rank) * V < D) r[j].load(p + j * team.size * V);
+    }
+}
+
+template <class R, int V, int NV, int THREADS, int CTAS>
+__global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p, uint32_t team_ctas) {
+    __shared__ float shared[2 * Team::kSumFloats];
+    Team team = team_of(team_ctas, shared);
+    if (team_ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
+    griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
-    Raw<uint16_t, V> w_post[NV], w_pre[NV];
-    load_row(w_post, p.w_post, team, p.D);
-    load_row(w_pre, p.w_pre, team, p.D);
     const float inv_d = 1.0f / (float)p.D;
-    for (uint64_t t = team.index; t < p.T; t += team.count) {
+    for (uint64_t row = team.index; row < p.T; row += team.count) {
+        const uint32_t t = (uint32_t)row;
         Raw<R, V> resid[NV];
         Raw<uint16_t, V> u[NV], gate[NV];
-        load_row(u, p.u ? p.u + t * p.ld_u : nullptr, team, p.D);
-        load_row(resid, static_cast<const R*>(p.resid) + t * p.ld_resid, team, p.D);
-        load_row(gate, p.gate ? p.gate + (uint32_t)t / p.gate_rows * p.ld_gate : nullptr, team, p.D);
+        load_row(u, p.u, t, p.ld_u, team, p.D);
+        load_row(resid, p.resid, t, p.ld_resid, team, p.D);
+        load_row(gate, p.gate, t / p.gate_rows, p.ld_gate, team, p.D);
+        constexpr int kPairs = V * NV / 2;
         float k = p.scale;
         if (p.post) {
-            float s[1] = {0.0f};
+            float2 q = both(0.0f);
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) s[0] = fmaf(u[j].get(i), u[j].get(i), s[0]);
+            for (int i = 0; i < kPairs; ++i) q = fma2(get2(u, i), get2(u, i), q);
+            float s[1] = {sum2(q)};
             team.sum(s);
             const float rp = 1.0f / sqrtf(s[0] * inv_d + p.eps);
             if (p.rstd_post && team.rank == 0) p.rstd_post[t] = rp;
             k *= rp;
         }
-        float h[NV][V], s[1] = {0.0f};
+        // The weights come from the first-level cache for every row: registers
+        // for them would cost a resident CTA.
+        Raw<uint16_t, V> w[NV];
+        load_weights(w, p.w_post, team, p.D);
+        float2 h[kPairs], q = both(0.0f);
+        // Without a branch u is zeros (and k a number), so h = resid.
+        if (!p.gate) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+            for (int i = 0; i < kPairs; ++i)
+                h[i] = fma2(mul2(get2(u, i), get2(w, i)), both(k), get2(resid, i));
+        } else if (p.gate_act == 0) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float b = u[j].get(i) * k;
-                if (p.w_post) b *= w_post[j].get(i);
-                if (p.gate) b *= act(gate[j].get(i), p.gate_act);
-                h[j][i] = p.u ? resid[j].get(i) + b : resid[j].get(i);
-                s[0] = fmaf(h[j][i], h[j][i], s[0]);
-            }
-        if (p.h)
+            for (int i = 0; i < kPairs; ++i)
+                h[i] = fma2(mul2(mul2(get2(u, i), get2(w, i)), get2(gate, i)), both(k), get2(resid, i));
+        } else {
 #pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const uint32_t i = (j * team.size + team.rank) * V;
-                if (i < p.D) put<V>(static_cast<R*>(p.h) + t * p.ld_h + i, h[j]);
-            }
+            for (int i = 0; i < kPairs; ++i)
+                h[i] = fma2(mul2(mul2(get2(u, i), get2(w, i)), sigmoid2(get2(gate, i))), both(k), get2(resid, i));
+        }
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) q = fma2(h[i], h[i], q);
+        if (p.h) store_row<V, NV>(static_cast<R*>(p.h) + (uint64_t)t * (uint32_t)p.ld_h, h, team, p.D);
         if (!p.y) continue;
+        load_weights(w, p.w_pre, team, p.D);
+        float s[1] = {sum2(q)};
         team.sum(s);
         const float r = 1.0f / sqrtf(s[0] * inv_d + p.eps);
         if (p.rstd_pre && team.rank == 0) p.rstd_pre[t] = r;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const uint32_t i = (j * team.size + team.rank) * V;
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                h[j][e] *= r;
-                if (p.w_pre) h[j][e] *= w_pre[j].get(e);
-            }
-            if (i < p.D) put<V>(p.y + t * p.ld_y + i, h[j]);
-        }
+        for (int i = 0; i < kPairs; ++i) h[i] = mul2(mul2(h[i], both(r)), get2(w, i));
+        store_row<V, NV>(p.y + (uint64_t)t * (uint32_t)p.ld_y, h, team, p.D);
     }
 }
+
+// A row's team of E channels a thread in CTAs of at most `most` threads: a warp
+// (4 of them share a CTA), a CTA, or a cluster of CTAs.
+constexpr uint32_t kForwardThreads = 1024, kBackwardThreads = 512;  // of an SM, by registers
+struct Shape {
+    uint32_t threads, ctas, teams;  // threads of a CTA, CTAs of a team (0: a warp), teams of a CTA
+    Shape(uint32_t D, uint32_t E, uint32_t most) {
+        const uint32_t team = (D + 32 * E - 1) / (32 * E) * 32;
+        ctas = team == 32 ? 0 : (team + most - 1) / most;
+        threads = team == 32 ? 128 : ((team + ctas - 1) / ctas + 31) / 32 * 32;
+        teams = ctas ? 1 : 4;
+    }
+    // CTAs (or clusters) that run at once with `per_sm` threads on an SM.
+    uint32_t resident(uint32_t per_sm) const {
+        const uint32_t sms = (uint32_t)foil_sm_count(), n = per_sm / threads ? per_sm / threads : 1;
+        return ctas > 1 ? foil_resident_clusters(ctas) : sms * n;
+    }
+};
 
 // Backward.  A team takes a chunk of consecutive tokens and sums dw_pre,
 // dw_post and, for a gate row that several tokens share, dgate in its
@@ -198,10 +307,11 @@ struct Chunks {
     uint32_t per_gate;        // chunks of a gate row, 0: a chunk holds whole gate rows
     uint32_t gates;           // gate rows
 };
-Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows, uint32_t sms) {
-    // Enough teams to fill the GPU, at least 8 tokens each: a chunk writes and
+Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
+    // As many teams as run at once, at least 8 tokens each: a chunk writes and
     // reads 3 x 4 bytes a channel beside the 12 and more of each token.
-    const uint32_t teams = sms * (D > 256 ? 2 : 16);
+    const Shape sh(D, 8, 512);
+    const uint32_t teams = sh.resident(kBackwardThreads) * sh.teams;
     uint32_t rows = (T + teams - 1) / teams;
     rows = rows < 8 ? 8 : rows;
     Chunks c{};
@@ -219,28 +329,13 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows, uint32_t sms) {
     return c;
 }
 
-template <class R, int V, int NV>
-struct Loaded {
-    Raw<R, V> dh[NV], h[NV];
-    Raw<uint16_t, V> dy[NV], u[NV], gate[NV];
-    float rh, ru;
-    __device__ __forceinline__ void load(const Backward& p, const Team& team, uint64_t t) {
-        load_row(dy, p.dy ? p.dy + t * p.ld_dy : nullptr, team, p.D);
-        load_row(h, p.dy ? static_cast<const R*>(p.h) + t * p.ld_h : nullptr, team, p.D);
-        load_row(u, p.u ? p.u + t * p.ld_u : nullptr, team, p.D);
-        load_row(dh, p.dh ? static_cast<const R*>(p.dh) + t * p.ld_dh : nullptr, team, p.D);
-        load_row(gate, p.gate ? p.gate + (uint32_t)t / p.gate_rows * p.ld_gate : nullptr, team, p.D);
-        rh = p.dy ? p.rstd_pre[t] : 0.0f;
-        ru = p.post && p.u ? p.rstd_post[t] : 1.0f;
-    }
-};
-
-template <class R, int V, int NV, int THREADS>
+template <class R, int V, int NV, int THREADS, bool GATE>
 __global__ void __launch_bounds__(THREADS)
-backward_kernel(const Backward p, const Chunks c, uint32_t team_size) {
-    __shared__ float shared[192];
-    Team team = team_of(team_size, shared);
-    griddep_wait();  // launched with programmatic stream serialization
+backward_kernel(const Backward p, const Chunks c, uint32_t team_ctas) {
+    __shared__ float shared[2 * Team::kSumFloats];
+    Team team = team_of(team_ctas, shared);
+    if (team_ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
+    griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
     if (team.index >= c.count) return;  // whole warps, or nobody
     // Tokens [t0, t1).
@@ -254,67 +349,99 @@ backward_kernel(const Backward p, const Chunks c, uint32_t team_size) {
         t0 = (uint64_t)team.index * c.rows;
         t1 = min((uint64_t)p.T, t0 + c.rows);
     }
+    constexpr int kPairs = V * NV / 2;
     Raw<uint16_t, V> w_post[NV], w_pre[NV];
-    load_row(w_post, p.w_post, team, p.D);
-    load_row(w_pre, p.w_pre, team, p.D);
-    float dw_post[NV][V] = {}, dw_pre[NV][V] = {}, dgate[NV][V] = {};
+    load_weights(w_post, p.w_post, team, p.D);
+    load_weights(w_pre, p.w_pre, team, p.D);
+    float2 dw_post[kPairs], dw_pre[kPairs], dgate[GATE ? kPairs : 1];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+        dw_post[i] = dw_pre[i] = both(0.0f);
+        if constexpr (GATE) dgate[i] = both(0.0f);
+    }
+    // The activation's derivative as a polynomial of its value: g - g^2, or 1.
+    const float2 der2 = both(p.gate_act ? -1.0f : 0.0f), der1 = both(p.gate_act ? 1.0f : 0.0f),
+                 der0 = both(p.gate_act ? 0.0f : 1.0f);
     const float inv_d = 1.0f / (float)p.D;
-    for (uint64_t t = t0; t < t1; ++t) {
-        Loaded<R, V, NV> x;
-        x.load(p, team, t);
+    struct {
+        Raw<R, V> dh[NV], h[NV];
+        Raw<uint16_t, V> dy[NV], u[NV], gate[GATE ? NV : 1];
+        float rh, ru;
+    } x, ahead;
+    uint32_t gate_row = GATE ? (uint32_t)t0 / p.gate_rows : 0u;               // of token t
+    uint32_t gate_left = GATE ? p.gate_rows - (uint32_t)t0 % p.gate_rows : 0u;  // its tokens from t on
+    auto fetch = [&](uint32_t t, bool new_gate) {
+        load_row(ahead.dy, p.dy, t, p.ld_dy, team, p.D);
+        load_row(ahead.h, p.dy ? p.h : nullptr, t, p.ld_h, team, p.D);
+        load_row(ahead.u, p.u, t, p.ld_u, team, p.D);
+        load_row(ahead.dh, p.dh, t, p.ld_dh, team, p.D);
+        if constexpr (GATE)
+            if (new_gate) load_row(ahead.gate, p.gate, gate_row + (t != t0), p.ld_gate, team, p.D);
+        ahead.rh = p.dy ? p.rstd_pre[t] : 0.0f;
+        ahead.ru = p.post && p.u ? p.rstd_post[t] : 1.0f;
+    };
+    if (t0 < t1) fetch((uint32_t)t0, true);
+    for (uint32_t t = (uint32_t)t0; t < t1; ++t) {
+        x = ahead;
+        if (t + 1u < t1) fetch(t + 1u, gate_left == 1u);
         // c1 = mean(a hhat) and c2 = mean(dp pv), dp = k (dh + rh (a - hhat c1))
-        // with k = scale act: one round of sums, c2 = s[1] - c1 s[2].
-        float s[3] = {0.0f, 0.0f, 0.0f};
+        // with k = scale act: one round of sums, c2 = ru (S1 - c1 rh S2).
+        const float ks = p.scale * x.ru;
+        float2 e[kPairs], hh[kPairs], ga[GATE ? kPairs : 1];
+        if constexpr (GATE) {
+            if (p.gate_act) {
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+                for (int i = 0; i < kPairs; ++i) ga[i] = sigmoid2(get2(x.gate, i));
+            } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float hh = x.h[j].get(i) * x.rh;
-                const float a = x.dy[j].get(i) * (p.w_pre ? w_pre[j].get(i) : 1.0f);
-                s[0] = fmaf(a, hh, s[0]);
-                if (p.post) {
-                    float k = p.scale * x.u[j].get(i) * x.ru * (p.w_post ? w_post[j].get(i) : 1.0f);
-                    if (p.gate) k *= act(x.gate[j].get(i), p.gate_act);
-                    s[1] = fmaf(k, fmaf(x.rh, a, x.dh[j].get(i)), s[1]);
-                    s[2] = fmaf(k, x.rh * hh, s[2]);
-                }
+                for (int i = 0; i < kPairs; ++i) ga[i] = get2(x.gate, i);
             }
-        team.sum(s);
-        const float c1 = s[0] * inv_d, c2 = (s[1] - c1 * s[2]) * inv_d;
-        const bool last = p.gate_rows && ((uint32_t)(t + 1) % p.gate_rows == 0 || t + 1 == p.T);
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float dh[V], du[V], dg[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float hh = x.h[j].get(i) * x.rh;
-                const float dy = x.dy[j].get(i), a = dy * (p.w_pre ? w_pre[j].get(i) : 1.0f);
-                dh[i] = fmaf(x.rh, a - hh * c1, x.dh[j].get(i));
-                dw_pre[j][i] = fmaf(dy, hh, dw_pre[j][i]);
-                const float uh = x.u[j].get(i) * x.ru, wp = p.w_post ? w_post[j].get(i) : 1.0f;
-                const float dz = p.scale * dh[i];
-                float dp = dz, der = 1.0f;
-                if (p.gate) {
-                    const float g = act(x.gate[j].get(i), p.gate_act);
-                    dp *= g;
-                    if (p.gate_act) der = g * (1.0f - g);
-                }
-                dw_post[j][i] = fmaf(dp, uh, dw_post[j][i]);
-                du[i] = p.post ? x.ru * (dp * wp - uh * c2) : dp;
-                dgate[j][i] = fmaf(dz * der, uh * wp, dgate[j][i]);
-                dg[i] = dgate[j][i];
-            }
-            const uint32_t i = (j * team.size + team.rank) * V;
-            if (i < p.D) {
-                if (p.dresid) put<V>(static_cast<R*>(p.dresid) + t * p.ld_dresid + i, dh);
-                if (p.du) put<V>(p.du + t * p.ld_du + i, du);
-                if (p.dgate && last && !c.per_gate)
-                    put<V>(p.dgate + (uint32_t)t / p.gate_rows * p.ld_dgate + i, dg);
-            }
-            if (last && !c.per_gate)
-#pragma unroll
-                for (int e = 0; e < V; ++e) dgate[j][e] = 0.0f;
         }
+        float2 s0 = both(0.0f), s1 = both(0.0f), s2 = both(0.0f);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            hh[i] = mul2(get2(x.h, i), both(x.rh));
+            const float2 dy = get2(x.dy, i), a = mul2(dy, get2(w_pre, i));
+            dw_pre[i] = fma2(dy, hh[i], dw_pre[i]);
+            s0 = fma2(a, hh[i], s0);
+            e[i] = fma2(both(x.rh), a, get2(x.dh, i));
+            float2 k = mul2(get2(x.u, i), get2(w_post, i));
+            if constexpr (GATE) k = mul2(k, ga[i]);
+            s1 = fma2(k, e[i], s1);
+            s2 = fma2(k, hh[i], s2);
+        }
+        float s[3] = {sum2(s0), sum2(s1), sum2(s2)};
+        team.sum(s);
+        const float c1 = x.rh * s[0] * inv_d;
+        const float c2 = p.post ? x.ru * x.ru * ks * (s[1] - c1 * s[2]) * inv_d : 0.0f;
+        // hh becomes du, e becomes dh.
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            e[i] = fma2(both(-c1), hh[i], e[i]);
+            const float2 u = get2(x.u, i), wp = get2(w_post, i), dz = mul2(e[i], both(ks));
+            float2 dp = dz;
+            if constexpr (GATE) {
+                dp = mul2(dz, ga[i]);
+                const float2 der = fma2(ga[i], fma2(ga[i], der2, der1), der0);
+                dgate[i] = fma2(mul2(dz, der), mul2(u, wp), dgate[i]);
+            }
+            dw_post[i] = fma2(dp, u, dw_post[i]);
+            hh[i] = fma2(both(-c2), u, mul2(dp, wp));
+        }
+        if (p.dresid)
+            store_row<V, NV>(static_cast<R*>(p.dresid) + (uint64_t)t * (uint32_t)p.ld_dresid, e, team, p.D);
+        if (p.du) store_row<V, NV>(p.du + (uint64_t)t * (uint32_t)p.ld_du, hh, team, p.D);
+        if constexpr (GATE)
+            if (--gate_left == 0 || t + 1u == t1) {
+                if (!c.per_gate) {  // the chunk holds all of the gate row's tokens
+                    if (p.dgate)
+                        store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
+#pragma unroll
+                    for (int i = 0; i < kPairs; ++i) dgate[i] = both(0.0f);
+                }
+                ++gate_row;
+                gate_left = p.gate_rows;
+            }
     }
     const uint64_t plane = (uint64_t)c.count * p.D;
     float* ws = p.ws + (uint64_t)team.index * p.D;
@@ -324,9 +451,11 @@ backward_kernel(const Backward p, const Chunks c, uint32_t team_size) {
         if (i >= p.D) continue;
 #pragma unroll
         for (int e = 0; e < V; ++e) {  // the workspace's rows are not aligned for vectors
-            if (p.dw_pre) ws[i + e] = dw_pre[j][e];
-            if (p.dw_post) ws[plane + i + e] = dw_post[j][e];
-            if (p.dgate && c.per_gate) ws[2 * plane + i + e] = dgate[j][e];
+            const int at = j * V + e;
+            if (p.dw_pre) ws[i + e] = at % 2 ? dw_pre[at / 2].y : dw_pre[at / 2].x;
+            if (p.dw_post) ws[plane + i + e] = at % 2 ? dw_post[at / 2].y : dw_post[at / 2].x;
+            if constexpr (GATE)
+                if (p.dgate && c.per_gate) ws[2 * plane + i + e] = at % 2 ? dgate[at / 2].y : dgate[at / 2].x;
         }
     }
 }
@@ -375,50 +504,50 @@ struct Width {
 };
 
 template <class K, class... Args>
-cudaError_t launch(K kernel, dim3 grid, uint32_t threads, cudaStream_t s, Args... args) {
+cudaError_t launch(K kernel, dim3 grid, uint32_t threads, uint32_t cluster, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
     cfg.gridDim = grid, cfg.blockDim = dim3(threads, 1, 1), cfg.stream = s;
-    cudaLaunchAttribute la[1];
+    cudaLaunchAttribute la[2];
     la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     la[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = la, cfg.numAttrs = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = cluster, la[1].val.clusterDim.y = 1, la[1].val.clusterDim.z = 1;
+    cfg.attrs = la, cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) foil_count_launch();
     return e;
 }
 
-// Threads of a row's team for E channels each, and CTAs' threads: warps that
-// are teams of their own share a CTA of 4.
-uint32_t team_threads(uint32_t D, uint32_t E) { return (D + 32 * E - 1) / (32 * E) * 32; }
+template <class R, int V, int E, int THREADS, int CTAS>
+cudaError_t forward_launch(const Forward& p, const Shape& sh, cudaStream_t s) {
+    const uint32_t resident = sh.resident(kForwardThreads);
+    const uint32_t teams = (p.T + sh.teams - 1) / sh.teams < resident ? (p.T + sh.teams - 1) / sh.teams : resident;
+    return launch(forward_kernel<R, V, E / V, THREADS, CTAS>, dim3(teams * (sh.ctas ? sh.ctas : 1)), sh.threads, sh.ctas, s,
+                  p, sh.ctas);
+}
 
+// 8 channels a thread up to 2048 channels, 16 up to 8192 in a CTA of up to 512
+// threads, then two CTAs.
 template <class R, int V>
 cudaError_t forward_typed(const Forward& p, cudaStream_t s) {
-    const uint32_t sms = (uint32_t)foil_sm_count();
-    const bool wide = p.D > 2048;  // 16 channels a thread
-    const uint32_t team = team_threads(p.D, wide ? 16 : 8), threads = team == 32 ? 128 : team;
-    const uint64_t ctas = team == 32 ? (p.T + 3) / 4 : p.T, most = (uint64_t)sms * (2048 / threads);
-    const dim3 grid((unsigned)(ctas < most ? ctas : most));
-    if (!wide) return launch(forward_kernel<R, V, 8 / V, 256>, grid, threads, s, p, team);
-    return threads <= 512 ? launch(forward_kernel<R, V, 16 / V, 512>, grid, threads, s, p, team)
-                          : launch(forward_kernel<R, V, 16 / V, 1024>, grid, threads, s, p, team);
+    if (p.D <= 2048) return forward_launch<R, V, 8, 256, 4>(p, Shape(p.D, 8, 512), s);
+    return forward_launch<R, V, 16, 512, 2>(p, Shape(p.D, 16, 512), s);
 }
 
 template <class R, int V>
 cudaError_t backward_typed(const Backward& p, const Chunks& c, cudaStream_t s) {
-    const bool wide = p.D > 4096;
-    const uint32_t team = team_threads(p.D, wide ? 16 : 8), threads = team == 32 ? 128 : team;
-    const dim3 grid(team == 32 ? (c.count + 3) / 4 : c.count);
-    if (!wide) return launch(backward_kernel<R, V, 8 / V, 512>, grid, threads, s, p, c, team);
-    return threads <= 512 ? launch(backward_kernel<R, V, 16 / V, 512>, grid, threads, s, p, c, team)
-                          : launch(backward_kernel<R, V, 16 / V, 1024>, grid, threads, s, p, c, team);
+    const Shape sh(p.D, 8, 512);
+    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.ctas ? sh.ctas : 1));
+    return p.gate ? launch(backward_kernel<R, V, 8 / V, 512, true>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas)
+                  : launch(backward_kernel<R, V, 8 / V, 512, false>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas);
 }
 
 }  // namespace
 
 uint64_t backward_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows) {
     if (T == 0 || D == 0) return 0;
-    const Chunks c = plan_chunks(T, D, gate_rows, (uint32_t)foil_sm_count());
+    const Chunks c = plan_chunks(T, D, gate_rows);
     return (uint64_t)c.count * D * 4 * (c.per_gate ? 3 : 2);
 }
 
@@ -443,7 +572,7 @@ cudaError_t backward(const Backward& p, bool fp32, cudaStream_t s) {
             }
         return cudaSuccess;
     }
-    const Chunks c = plan_chunks(p.T, p.D, p.gate_rows, (uint32_t)foil_sm_count());
+    const Chunks c = plan_chunks(p.T, p.D, p.gate_rows);
     Width w(p.D);
     w.use(p.dh, p.ld_dh, fp32 ? 4 : 2), w.use(p.h, p.ld_h, fp32 ? 4 : 2), w.use(p.dresid, p.ld_dresid, fp32 ? 4 : 2);
     w.use(p.dy, p.ld_dy, 2), w.use(p.u, p.ld_u, 2), w.use(p.gate, p.ld_gate, 2), w.use(p.du, p.ld_du, 2);
@@ -460,7 +589,7 @@ cudaError_t backward(const Backward& p, bool fp32, cudaStream_t s) {
     Chunks sums = c;
     if (!shared_gate) sums.gates = 0;
     const uint32_t rows = 2 + sums.gates;
-    return launch(sum_chunks, dim3((p.D + 31) / 32, rows < 32768 ? rows : 32768), 256, s, p, sums);
+    return launch(sum_chunks, dim3((p.D + 31) / 32, rows < 32768 ? rows : 32768), 256, 1, s, p, sums);
 }
 
 }  // namespace norm

@@ -102,6 +102,11 @@ void foil_count_launch();
 cudaError_t foil_smem_optin(const void* kernel, int bytes);
 int foil_sm_count();
 
+// Clusters of S (2 to 8) CTAs, one CTA on an SM, that run at the same time on
+// the current device (74, 33 and 15 of 2, 4 and 8 on 148 SMs: a cluster stays
+// inside a GPC); asked for once for each device.  Defined in layout.cu.
+uint32_t foil_resident_clusters(uint32_t S);
+
 // Wall-time limit (ns) of each bounded device-side wait, passed to every
 // kernel launch; process-wide, set by foil_set_wait_limit_ns (default 2 s).
 uint64_t foil_wait_limit_ns();

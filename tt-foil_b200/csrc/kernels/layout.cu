@@ -8,6 +8,7 @@
 // accesses, and the permutation happens in shared memory.  The shared-memory
 // index is XOR-swizzled so that every 8-lane phase of a 16-byte access hits 8
 // distinct 4-bank groups (conflict-free on both sides).
+#include <atomic>
 #include <cstring>
 
 #include "common.cuh"
@@ -174,6 +175,40 @@ extern "C" int foil_untilize_dev(const uint16_t* tiles, uint16_t* row_major,
     const cudaError_t le = launch_layout(foil::untilize_kernel, (unsigned)grid, (cudaStream_t)stream,
                                          (const uint4*)tiles, (uint4*)row_major, rows, cols);
     return check_launch("foil_untilize_dev", le);
+}
+
+// ---------------------------------------------------- resident clusters ---
+// A kernel that fills an SM with one CTA by its shared memory; only its
+// occupancy is asked for.
+static __global__ void occupancy_probe() {}
+
+uint32_t foil_resident_clusters(uint32_t S) {
+    static std::atomic<uint32_t> known[64][9];
+    const uint32_t sms = (uint32_t)foil_sm_count();
+    int dev = 0;
+    if (S < 2 || S > 8 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return S ? sms / S : sms;
+    std::atomic<uint32_t>& k = known[dev][S];
+    uint32_t n = k.load(std::memory_order_relaxed);
+    if (n) return n;
+    constexpr int kSmem = 160 * 1024;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = dim3(sms / S * S, 1, 1);
+    cfg.blockDim = dim3(512, 1, 1);
+    cfg.dynamicSmemBytes = kSmem;
+    cudaLaunchAttribute la[1];
+    la[0].id = cudaLaunchAttributeClusterDimension;
+    la[0].val.clusterDim.x = S, la[0].val.clusterDim.y = 1, la[0].val.clusterDim.z = 1;
+    cfg.attrs = la;
+    cfg.numAttrs = 1;
+    int got = 0;
+    if (foil_smem_optin((const void*)occupancy_probe, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&got, occupancy_probe, &cfg) != cudaSuccess || got <= 0) {
+        cudaGetLastError();
+        got = (int)(sms / S);
+    }
+    k.store(n = (uint32_t)got, std::memory_order_relaxed);
+    return n;
 }
 
 // ---------------------------------------------------- batched transpose ---

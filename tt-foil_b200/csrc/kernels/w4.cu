@@ -3,8 +3,6 @@
 // foil_w4_pack_dev in include/foil_c.h.
 #include "w4.cuh"
 
-#include <atomic>
-
 #include "gemm_ptx.cuh"
 
 namespace foil {
@@ -471,35 +469,6 @@ cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weigh
     return count(cudaGetLastError());
 }
 
-// Clusters of S CTAs, one CTA on an SM, that run at the same time (74, 33 and
-// 15 of 2, 4 and 8 on 148 SMs: a cluster stays inside a GPC); asked for once
-// for each device.
-static uint32_t resident_clusters(uint32_t S, uint32_t sms) {
-    static std::atomic<uint32_t> known[64][4];
-    int dev = 0;
-    if (S == 1 || cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return sms / S;
-    std::atomic<uint32_t>& k = known[dev][S == 2 ? 1 : S == 4 ? 2 : 3];
-    uint32_t n = k.load(std::memory_order_relaxed);
-    if (n == 0) {
-        const MatvecKernel kernel = matvec_kernel<1, mv_tiles(1), 128, false>;
-        cudaLaunchConfig_t cfg{};
-        cfg.gridDim = dim3(sms / S * S, 1, 1), cfg.blockDim = dim3(kMvThreads, 1, 1);
-        cfg.dynamicSmemBytes = 150000;
-        cudaLaunchAttribute la[1]{};
-        la[0].id = cudaLaunchAttributeClusterDimension;
-        la[0].val.clusterDim.x = S, la[0].val.clusterDim.y = 1, la[0].val.clusterDim.z = 1;
-        cfg.attrs = la, cfg.numAttrs = 1;
-        int got = 0;
-        if (foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512) != cudaSuccess ||
-            cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess || got <= 0) {
-            cudaGetLastError();
-            got = (int)(sms / S);
-        }
-        k.store(n = (uint32_t)got, std::memory_order_relaxed);
-    }
-    return n;
-}
-
 // The split of K over the CTAs of a cluster (S) and the warps of a CTA (WK):
 // the one whose busiest warp reads the fewest storage blocks, among those
 // whose slice of x fits.  A cluster barrier costs about as much as two blocks
@@ -513,7 +482,7 @@ static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, 
         const uint32_t pitch = ks * 256 + 64;  // 64 bytes more: rows of an 8-lane read phase on distinct banks
         const uint32_t off_sum = width * pitch, sums = ks * (128 / group) * width * 4;
         const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
-        const uint32_t fit = resident_clusters(S, sms), clusters = fit < p.tiles ? fit : p.tiles;
+        const uint32_t fit = (S == 1 ? sms : foil_resident_clusters(S)), clusters = fit < p.tiles ? fit : p.tiles;
         const uint32_t tc = ((p.tiles + clusters - 1) / clusters + rt - 1) / rt;  // runs of rt tiles
         for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
             // A run's set-up and join cost about as much as one of its steps.

@@ -51,7 +51,7 @@ Span matrix(const char* what, const void* p, uint64_t& ld, uint64_t rows, uint64
     if (!p) return Span(nullptr, 0);
     if (ld < cols) invalid(what, "a row stride is shorter than a row");
     if ((uintptr_t)p % elem) invalid(what, "misaligned pointer");
-    if (rows && ld > (1ull << 46) / rows) invalid(what, "tensor too large");
+    if (ld >= (1ull << 32) || (rows && ld > (1ull << 46) / rows)) invalid(what, "tensor too large");
     Span s(p, rows ? ((rows - 1) * ld + cols) * elem : 0);
     s.pitch = ld * elem, s.row = cols * elem;
     return s;
