@@ -28,10 +28,6 @@ template <class T, int V>
 struct Raw {
     static constexpr int kWords = (sizeof(T) * V + 3) / 4;
     uint32_t w[kWords];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < kWords; ++i) w[i] = 0;
-    }
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (sizeof(T) * V >= 16) {
 #pragma unroll
@@ -106,22 +102,37 @@ __device__ __forceinline__ void put(float* p, const float2* v, int j) {
         *p = j % 2 ? v[j / 2].y : v[j / 2].x;
     }
 }
-// A row's share of this thread to memory.
+// A row's share of this thread to memory (nowhere if p is null).
 template <int V, int NV, class T, class Team>
 __device__ __forceinline__ void store_row(T* p, const float2 (&v)[V * NV / 2], const Team& t, uint32_t D) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const uint32_t i = (j * t.size + t.rank) * V;
-        if (i < D) put<V>(p + i, v, j);
+        if (p && i < D) put<V>(p + i, v, j);
     }
 }
 
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + expf(-g)); }
+// The same without vectors: the workspace's rows are not aligned for them.
+template <int V, int NV, class Team>
+__device__ __forceinline__ void store_plain(float* p, const float2 (&v)[V * NV / 2], const Team& t, uint32_t D) {
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+        const uint32_t i = (j * t.size + t.rank) * V;
+        if (i >= D) continue;
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[i + e] = (j * V + e) % 2 ? v[(j * V + e) / 2].y : v[(j * V + e) / 2].x;
+    }
+}
+
+// At most 2^-17 relative off, to |g| = 88: __expf is within 2 + 1.173 |g| units
+// in the last place.
+__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
 __device__ __forceinline__ float2 sigmoid2(float2 g) { return make_float2(sigmoid(g.x), sigmoid(g.y)); }
 
 // The threads that hold one row: a warp, a CTA, or the CTAs of a cluster.
 struct Team {
     uint32_t size, rank;    // threads, this thread
+    uint32_t lane;
     uint32_t ctas;          // CTAs of a team (0: the team is a warp)
     uint32_t index, count;  // this team, teams of the grid
     float* shared;          // two sets of kSumFloats floats
@@ -134,7 +145,6 @@ struct Team {
     template <int N>
     __device__ __forceinline__ void sum(float (&v)[N]) {
         constexpr uint32_t kAll = 0xffffffffu;
-        const uint32_t lane = threadIdx.x % 32u;
         float s;
         if constexpr (N == 1) {
             s = v[0];
@@ -186,38 +196,86 @@ struct Team {
 __device__ __forceinline__ Team team_of(uint32_t ctas, float* shared) {
     if (ctas == 0) {
         const uint32_t per = blockDim.x / 32u;
-        return Team{32u, threadIdx.x % 32u, 0u, blockIdx.x * per + threadIdx.x / 32u, gridDim.x * per, shared, 0u};
+        return Team{32u, threadIdx.x % 32u, threadIdx.x % 32u, 0u, blockIdx.x * per + threadIdx.x / 32u, gridDim.x * per, shared, 0u};
     }
-    return Team{ctas * blockDim.x, blockIdx.x % ctas * blockDim.x + threadIdx.x, ctas, blockIdx.x / ctas,
+    return Team{ctas * blockDim.x, blockIdx.x % ctas * blockDim.x + threadIdx.x, threadIdx.x % 32u, ctas, blockIdx.x / ctas,
                 gridDim.x / ctas, shared, 0u};
 }
 
-// bf16 weights of the thread's channels; ones where there are none.
+// Element of vector j of this thread.  Threads past D read the last vector
+// again, so that loads need no branch; what they hold must not enter a sum.
+template <int V>
+__device__ __forceinline__ uint32_t column(int j, const Team& t, uint32_t D) {
+    return min((j * t.size + t.rank) * V, D - V);
+}
+template <int V>
+__device__ __forceinline__ bool inside(int j, const Team& t, uint32_t D) {
+    return (j * t.size + t.rank) * V < D;
+}
+
+// bf16 weights of the thread's channels: ones where there are none, zeros past D.
 template <int V, int NV>
 __device__ __forceinline__ void load_weights(Raw<uint16_t, V> (&r)[NV], const uint16_t* p, const Team& t, uint32_t D) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-        const uint32_t i = (j * t.size + t.rank) * V;
+        const uint32_t none = inside<V>(j, t, D) ? 0x3f803f80u : 0u;
+        if (p && none)
+            r[j].load(p + column<V>(j, t, D));
+        else
 #pragma unroll
-        for (int k = 0; k < Raw<uint16_t, V>::kWords; ++k) r[j].w[k] = 0x3f803f80u;
-        if (p && i < D) r[j].load(p + i);
+            for (int k = 0; k < Raw<uint16_t, V>::kWords; ++k) r[j].w[k] = none;
     }
 }
 
-// A thread's channels of row t of a tensor (none: zeros).  Row strides are
-// below 2^32, so the offset is one multiplication.
+// A row of zeros, read where a tensor is not given; a factor of one.
+__device__ uint4 g_zeros[kMaxD * 4 / 16];
+__device__ float g_one = 1.0f;
+
+// A tensor as a team reads it.  Row strides are below 2^32, so a row's offset
+// is one multiplication.
 template <class T, int V, int NV>
-__device__ __forceinline__ void load_row(Raw<T, V> (&r)[NV], const void* base, uint32_t t, uint64_t ld, const Team& team,
-                                         uint32_t D) {
-    const T* p = static_cast<const T*>(base) + (uint64_t)t * (uint32_t)ld + team.rank * V;
+struct Input {
+    const T* p;
+    uint32_t ld;
+    __device__ __forceinline__ Input(const void* base, uint64_t stride)
+        : p(static_cast<const T*>(base ? base : g_zeros)), ld(base ? (uint32_t)stride : 0u) {}
+    __device__ __forceinline__ void load(Raw<T, V> (&r)[NV], uint32_t row, const Team& team, uint32_t D) const {
+        const T* q = p + (uint64_t)row * ld;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        r[j].zero();
-        if (base && (j * team.size + team.rank) * V < D) r[j].load(p + j * team.size * V);
+        for (int j = 0; j < NV; ++j) r[j].load(q + column<V>(j, team, D));
     }
+};
+
+// This thread's part of a row's sum of squares.
+template <int V, int NV>
+__device__ __forceinline__ float sum_squares(const float2 (&v)[V * NV / 2], const Team& t, uint32_t D) {
+    float s = 0.0f;
+    if constexpr (V == 1) {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const float x = j % 2 ? v[j / 2].y : v[j / 2].x;
+            s += inside<V>(j, t, D) ? x * x : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            float2 q = mul2(v[j * (V / 2)], v[j * (V / 2)]);
+#pragma unroll
+            for (int i = 1; i < V / 2; ++i) q = fma2(v[j * (V / 2) + i], v[j * (V / 2) + i], q);
+            s += inside<V>(j, t, D) ? sum2(q) : 0.0f;
+        }
+    }
+    return s;
 }
 
-template <class R, int V, int NV, int THREADS, int CTAS>
+// Gates: none, as they are, through the logistic function.
+enum { kNoGate = 0, kPlainGate = 1, kSigmoidGate = 2 };
+template <int GATE, int V, int NV>
+__device__ __forceinline__ float2 gate2(const Raw<uint16_t, V> (&r)[NV], int i) {
+    return GATE == kSigmoidGate ? sigmoid2(get2(r, i)) : get2(r, i);
+}
+
+template <class R, int V, int NV, int THREADS, int CTAS, int GATE>
 __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p, uint32_t team_ctas) {
     __shared__ float shared[2 * Team::kSumFloats];
     Team team = team_of(team_ctas, shared);
@@ -225,20 +283,22 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
     griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
     const float inv_d = 1.0f / (float)p.D;
+    const Input<R, V, NV> resid_in(p.resid, p.ld_resid);
+    const Input<uint16_t, V, NV> u_in(p.u, p.ld_u), gate_in(p.gate, p.ld_gate);
     for (uint64_t row = team.index; row < p.T; row += team.count) {
         const uint32_t t = (uint32_t)row;
         Raw<R, V> resid[NV];
         Raw<uint16_t, V> u[NV], gate[NV];
-        load_row(u, p.u, t, p.ld_u, team, p.D);
-        load_row(resid, p.resid, t, p.ld_resid, team, p.D);
-        load_row(gate, p.gate, t / p.gate_rows, p.ld_gate, team, p.D);
+        u_in.load(u, t, team, p.D);
+        resid_in.load(resid, t, team, p.D);
+        if constexpr (GATE) gate_in.load(gate, p.gate_rows == 1 ? t : t / p.gate_rows, team, p.D);
         constexpr int kPairs = V * NV / 2;
         float k = p.scale;
         if (p.post) {
-            float2 q = both(0.0f);
+            float2 v[kPairs];
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i) q = fma2(get2(u, i), get2(u, i), q);
-            float s[1] = {sum2(q)};
+            for (int i = 0; i < kPairs; ++i) v[i] = get2(u, i);
+            float s[1] = {sum_squares<V, NV>(v, team, p.D)};
             team.sum(s);
             const float rp = 1.0f / sqrtf(s[0] * inv_d + p.eps);
             if (p.rstd_post && team.rank == 0) p.rstd_post[t] = rp;
@@ -248,27 +308,18 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
         // for them would cost a resident CTA.
         Raw<uint16_t, V> w[NV];
         load_weights(w, p.w_post, team, p.D);
-        float2 h[kPairs], q = both(0.0f);
+        float2 h[kPairs];
         // Without a branch u is zeros (and k a number), so h = resid.
-        if (!p.gate) {
 #pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-                h[i] = fma2(mul2(get2(u, i), get2(w, i)), both(k), get2(resid, i));
-        } else if (p.gate_act == 0) {
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-                h[i] = fma2(mul2(mul2(get2(u, i), get2(w, i)), get2(gate, i)), both(k), get2(resid, i));
-        } else {
-#pragma unroll
-            for (int i = 0; i < kPairs; ++i)
-                h[i] = fma2(mul2(mul2(get2(u, i), get2(w, i)), sigmoid2(get2(gate, i))), both(k), get2(resid, i));
+        for (int i = 0; i < kPairs; ++i) {
+            float2 b = mul2(get2(u, i), get2(w, i));
+            if constexpr (GATE) b = mul2(b, gate2<GATE>(gate, i));
+            h[i] = fma2(b, both(k), get2(resid, i));
         }
-#pragma unroll
-        for (int i = 0; i < kPairs; ++i) q = fma2(h[i], h[i], q);
         if (p.h) store_row<V, NV>(static_cast<R*>(p.h) + (uint64_t)t * (uint32_t)p.ld_h, h, team, p.D);
         if (!p.y) continue;
         load_weights(w, p.w_pre, team, p.D);
-        float s[1] = {sum2(q)};
+        float s[1] = {sum_squares<V, NV>(h, team, p.D)};
         team.sum(s);
         const float r = 1.0f / sqrtf(s[0] * inv_d + p.eps);
         if (p.rstd_pre && team.rank == 0) p.rstd_pre[t] = r;
@@ -280,7 +331,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
 
 // A row's team of E channels a thread in CTAs of at most `most` threads: a warp
 // (4 of them share a CTA), a CTA, or a cluster of CTAs.
-constexpr uint32_t kForwardThreads = 1024, kBackwardThreads = 512;  // of an SM, by registers
+constexpr uint32_t kBackwardThreads = 512;  // of an SM, by registers
 struct Shape {
     uint32_t threads, ctas, teams;  // threads of a CTA, CTAs of a team (0: a warp), teams of a CTA
     Shape(uint32_t D, uint32_t E, uint32_t most) {
@@ -318,8 +369,10 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
     if (gate_rows > T) gate_rows = T;
     c.gates = gate_rows ? (T + gate_rows - 1) / gate_rows : 0;
     if (gate_rows > rows) {
-        c.per_gate = (gate_rows + rows - 1) / rows;
+        // Not more chunks than teams, if there are fewer gate rows.
+        c.per_gate = c.gates < teams ? teams / c.gates : 1;
         c.rows = (gate_rows + c.per_gate - 1) / c.per_gate;
+        c.rows = c.rows < 8 ? 8 : c.rows;
         c.per_gate = (gate_rows + c.rows - 1) / c.rows;
         c.count = c.per_gate * c.gates;
     } else {
@@ -329,135 +382,181 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
     return c;
 }
 
-template <class R, int V, int NV, int THREADS, bool GATE>
-__global__ void __launch_bounds__(THREADS)
-backward_kernel(const Backward p, const Chunks c, uint32_t team_ctas) {
+// GATE: kNoGate where a gate row serves several tokens or there is none (then
+// the gate's part is taken out of the sums over its tokens: with A = sum dz
+// uhat, dw_post gains act A and dgate is act' w_post A), else a gate row for
+// each token.
+template <class R, int V, int NV, int THREADS, int GATE>
+__global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, uint32_t team_ctas) {
+    constexpr int kPairs = V * NV / 2;
     __shared__ float shared[2 * Team::kSumFloats];
+    __shared__ float2 post_sum[GATE ? 1 : kPairs * THREADS];  // dw_post of the gate rows done, a slot for each thread
     Team team = team_of(team_ctas, shared);
     if (team_ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
     griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
     if (team.index >= c.count) return;  // whole warps, or nobody
     // Tokens [t0, t1).
-    uint64_t t0, t1;
+    uint32_t t0, t1;
     if (c.per_gate) {
         const uint64_t gate0 = (uint64_t)(team.index / c.per_gate) * p.gate_rows;
         const uint64_t end = min((uint64_t)p.T, gate0 + p.gate_rows);
-        t0 = min(end, gate0 + (uint64_t)(team.index % c.per_gate) * c.rows);
-        t1 = min(end, t0 + c.rows);
+        const uint64_t first = min(end, gate0 + (uint64_t)(team.index % c.per_gate) * c.rows);
+        t0 = (uint32_t)first, t1 = (uint32_t)min(end, first + c.rows);
     } else {
-        t0 = (uint64_t)team.index * c.rows;
-        t1 = min((uint64_t)p.T, t0 + c.rows);
+        const uint64_t first = (uint64_t)team.index * c.rows;
+        t0 = (uint32_t)first, t1 = (uint32_t)min((uint64_t)p.T, first + c.rows);
     }
-    constexpr int kPairs = V * NV / 2;
-    Raw<uint16_t, V> w_post[NV], w_pre[NV];
-    load_weights(w_post, p.w_post, team, p.D);
+    Raw<uint16_t, V> w_pre[NV], w_post[GATE ? NV : 1];
     load_weights(w_pre, p.w_pre, team, p.D);
-    float2 dw_post[kPairs], dw_pre[kPairs], dgate[GATE ? kPairs : 1];
+    if constexpr (GATE) load_weights(w_post, p.w_post, team, p.D);
+    float2 dw_pre[kPairs], dw_post[kPairs], gw[GATE ? 1 : kPairs];  // dw_post: A; gw: act(gate) w_post
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
         dw_post[i] = dw_pre[i] = both(0.0f);
-        if constexpr (GATE) dgate[i] = both(0.0f);
+        if constexpr (!GATE) post_sum[i * blockDim.x + threadIdx.x] = both(0.0f);
     }
-    // The activation's derivative as a polynomial of its value: g - g^2, or 1.
-    const float2 der2 = both(p.gate_act ? -1.0f : 0.0f), der1 = both(p.gate_act ? 1.0f : 0.0f),
-                 der0 = both(p.gate_act ? 0.0f : 1.0f);
     const float inv_d = 1.0f / (float)p.D;
-    struct {
+    struct Row {
         Raw<R, V> dh[NV], h[NV];
         Raw<uint16_t, V> dy[NV], u[NV], gate[GATE ? NV : 1];
         float rh, ru;
-    } x, ahead;
-    uint32_t gate_row = GATE ? (uint32_t)t0 / p.gate_rows : 0u;               // of token t
-    uint32_t gate_left = GATE ? p.gate_rows - (uint32_t)t0 % p.gate_rows : 0u;  // its tokens from t on
-    auto fetch = [&](uint32_t t, bool new_gate) {
-        load_row(ahead.dy, p.dy, t, p.ld_dy, team, p.D);
-        load_row(ahead.h, p.dy ? p.h : nullptr, t, p.ld_h, team, p.D);
-        load_row(ahead.u, p.u, t, p.ld_u, team, p.D);
-        load_row(ahead.dh, p.dh, t, p.ld_dh, team, p.D);
-        if constexpr (GATE)
-            if (new_gate) load_row(ahead.gate, p.gate, gate_row + (t != t0), p.ld_gate, team, p.D);
-        ahead.rh = p.dy ? p.rstd_pre[t] : 0.0f;
-        ahead.ru = p.post && p.u ? p.rstd_post[t] : 1.0f;
     };
-    if (t0 < t1) fetch((uint32_t)t0, true);
-    for (uint32_t t = (uint32_t)t0; t < t1; ++t) {
-        x = ahead;
-        if (t + 1u < t1) fetch(t + 1u, gate_left == 1u);
+    const Input<R, V, NV> dh_in(p.dh, p.ld_dh), h_in(p.dy ? p.h : nullptr, p.ld_h);
+    const Input<uint16_t, V, NV> dy_in(p.dy, p.ld_dy), u_in(p.u, p.ld_u), gate_in(p.gate, p.ld_gate);
+    const bool post = p.post && p.u;
+    const float* const rstd_pre = p.dy ? p.rstd_pre : reinterpret_cast<const float*>(g_zeros);
+    const float* const rstd_post = post ? p.rstd_post : &g_one;
+    const uint32_t pre_step = p.dy ? 1u : 0u, post_step = post ? 1u : 0u;
+    auto fetch = [&](Row& x, uint32_t t) {
+        dy_in.load(x.dy, t, team, p.D);
+        h_in.load(x.h, t, team, p.D);
+        u_in.load(x.u, t, team, p.D);
+        dh_in.load(x.dh, t, team, p.D);
+        if constexpr (GATE) gate_in.load(x.gate, t, team, p.D);
+        x.rh = rstd_pre[(uint64_t)t * pre_step];
+        x.ru = rstd_post[(uint64_t)t * post_step];
+    };
+    // A gate row that several tokens share: before and after its tokens here.
+    uint32_t gate_row = 0, gate_left = 0xffffffffu;  // of token t, and its tokens from t on
+    auto start_gate = [&] {
+        Raw<uint16_t, V> g[NV], wp[NV];
+        load_weights(wp, p.w_post, team, p.D);
+        if (p.gate) gate_in.load(g, gate_row, team, p.D);
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            gw[i] = get2(wp, i);
+            if (p.gate) gw[i] = mul2(gw[i], p.gate_act ? sigmoid2(get2(g, i)) : get2(g, i));
+        }
+    };
+    auto end_gate = [&] {
+        Raw<uint16_t, V> g[NV], wp[NV];
+        load_weights(wp, p.w_post, team, p.D);
+        if (p.gate) gate_in.load(g, gate_row, team, p.D);
+        float2 dgate[kPairs];
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            float2 a = dw_post[i];
+            dgate[i] = mul2(get2(wp, i), a);
+            if (p.gate) {
+                float2 ga = get2(g, i);
+                if (p.gate_act) {  // the logistic function's derivative is g - g^2
+                    ga = sigmoid2(ga);
+                    dgate[i] = mul2(dgate[i], fma2(mul2(ga, ga), both(-1.0f), ga));
+                }
+                a = mul2(a, ga);
+            }
+            float2& sum = post_sum[i * blockDim.x + threadIdx.x];
+            sum = fma2(a, both(1.0f), sum);
+            dw_post[i] = both(0.0f);
+        }
+        if (!p.gate || !p.dgate) return;
+        if (c.per_gate)
+            store_plain<V, NV>(p.ws + (2ull * c.count + team.index) * p.D, dgate, team, p.D);
+        else
+            store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
+    };
+    // One token: x is its row, which arrived while the one before was worked
+    // on; the next one goes to `ahead`.
+    auto step = [&](const Row& x, Row& ahead, uint32_t t) {
+        if (t + 1u < t1) fetch(ahead, t + 1u);
         // c1 = mean(a hhat) and c2 = mean(dp pv), dp = k (dh + rh (a - hhat c1))
         // with k = scale act: one round of sums, c2 = ru (S1 - c1 rh S2).
         const float ks = p.scale * x.ru;
+        const float2 rh = both(x.rh);
         float2 e[kPairs], hh[kPairs], ga[GATE ? kPairs : 1];
-        if constexpr (GATE) {
-            if (p.gate_act) {
-#pragma unroll
-                for (int i = 0; i < kPairs; ++i) ga[i] = sigmoid2(get2(x.gate, i));
-            } else {
-#pragma unroll
-                for (int i = 0; i < kPairs; ++i) ga[i] = get2(x.gate, i);
-            }
-        }
         float2 s0 = both(0.0f), s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-            hh[i] = mul2(get2(x.h, i), both(x.rh));
+            hh[i] = mul2(get2(x.h, i), rh);
             const float2 dy = get2(x.dy, i), a = mul2(dy, get2(w_pre, i));
             dw_pre[i] = fma2(dy, hh[i], dw_pre[i]);
             s0 = fma2(a, hh[i], s0);
-            e[i] = fma2(both(x.rh), a, get2(x.dh, i));
-            float2 k = mul2(get2(x.u, i), get2(w_post, i));
-            if constexpr (GATE) k = mul2(k, ga[i]);
+            e[i] = fma2(rh, a, get2(x.dh, i));
+            float2 k;
+            if constexpr (GATE) {
+                ga[i] = gate2<GATE>(x.gate, i);
+                k = mul2(mul2(get2(x.u, i), get2(w_post, i)), ga[i]);
+            } else {
+                k = mul2(get2(x.u, i), gw[i]);
+            }
             s1 = fma2(k, e[i], s1);
             s2 = fma2(k, hh[i], s2);
         }
         float s[3] = {sum2(s0), sum2(s1), sum2(s2)};
         team.sum(s);
         const float c1 = x.rh * s[0] * inv_d;
-        const float c2 = p.post ? x.ru * x.ru * ks * (s[1] - c1 * s[2]) * inv_d : 0.0f;
-        // hh becomes du, e becomes dh.
+        const float c2 = post ? x.ru * x.ru * ks * (s[1] - c1 * s[2]) * inv_d : 0.0f;
+        const float2 m1 = both(-c1), m2 = both(-c2), k2 = both(ks);
+        // e becomes dh, hh becomes du.
+        float2 dgate[GATE ? kPairs : 1];
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
-            e[i] = fma2(both(-c1), hh[i], e[i]);
-            const float2 u = get2(x.u, i), wp = get2(w_post, i), dz = mul2(e[i], both(ks));
-            float2 dp = dz;
+            e[i] = fma2(m1, hh[i], e[i]);
+            const float2 u = get2(x.u, i), dz = mul2(e[i], k2);
             if constexpr (GATE) {
-                dp = mul2(dz, ga[i]);
-                const float2 der = fma2(ga[i], fma2(ga[i], der2, der1), der0);
-                dgate[i] = fma2(mul2(dz, der), mul2(u, wp), dgate[i]);
+                const float2 wp = get2(w_post, i), dp = mul2(dz, ga[i]);
+                dgate[i] = mul2(GATE == kSigmoidGate ? fma2(mul2(dp, ga[i]), both(-1.0f), dp) : dz, mul2(u, wp));
+                dw_post[i] = fma2(dp, u, dw_post[i]);
+                hh[i] = fma2(m2, u, mul2(dp, wp));
+            } else {
+                dw_post[i] = fma2(dz, u, dw_post[i]);
+                hh[i] = fma2(m2, u, mul2(dz, gw[i]));
             }
-            dw_post[i] = fma2(dp, u, dw_post[i]);
-            hh[i] = fma2(both(-c2), u, mul2(dp, wp));
         }
-        if (p.dresid)
-            store_row<V, NV>(static_cast<R*>(p.dresid) + (uint64_t)t * (uint32_t)p.ld_dresid, e, team, p.D);
-        if (p.du) store_row<V, NV>(p.du + (uint64_t)t * (uint32_t)p.ld_du, hh, team, p.D);
-        if constexpr (GATE)
-            if (--gate_left == 0 || t + 1u == t1) {
-                if (!c.per_gate) {  // the chunk holds all of the gate row's tokens
-                    if (p.dgate)
-                        store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
-#pragma unroll
-                    for (int i = 0; i < kPairs; ++i) dgate[i] = both(0.0f);
-                }
-                ++gate_row;
-                gate_left = p.gate_rows;
-            }
-    }
-    const uint64_t plane = (uint64_t)c.count * p.D;
-    float* ws = p.ws + (uint64_t)team.index * p.D;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const uint32_t i = (j * team.size + team.rank) * V;
-        if (i >= p.D) continue;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {  // the workspace's rows are not aligned for vectors
-            const int at = j * V + e;
-            if (p.dw_pre) ws[i + e] = at % 2 ? dw_pre[at / 2].y : dw_pre[at / 2].x;
-            if (p.dw_post) ws[plane + i + e] = at % 2 ? dw_post[at / 2].y : dw_post[at / 2].x;
-            if constexpr (GATE)
-                if (p.dgate && c.per_gate) ws[2 * plane + i + e] = at % 2 ? dgate[at / 2].y : dgate[at / 2].x;
+        store_row<V, NV>(p.dresid ? static_cast<R*>(p.dresid) + (uint64_t)t * (uint32_t)p.ld_dresid : nullptr, e, team,
+                         p.D);
+        store_row<V, NV>(p.du ? p.du + (uint64_t)t * (uint32_t)p.ld_du : nullptr, hh, team, p.D);
+        if constexpr (GATE) {
+            if (p.dgate) store_row<V, NV>(p.dgate + (uint64_t)t * (uint32_t)p.ld_dgate, dgate, team, p.D);
+        } else if (--gate_left == 0u) {
+            end_gate();
+            ++gate_row;
+            gate_left = p.gate_rows;
+            if (t + 1u < t1) start_gate();
         }
+    };
+    if (t0 < t1) {
+        Row a, b;
+        fetch(a, t0);
+        if constexpr (!GATE) {
+            if (p.gate) gate_row = t0 / p.gate_rows, gate_left = p.gate_rows - t0 % p.gate_rows;
+            start_gate();
+        }
+        for (uint32_t t = t0; t < t1; t += 2u) {
+            step(a, b, t);
+            if (t + 1u < t1) step(b, a, t + 1u);
+        }
+        if constexpr (!GATE)
+            if (!p.gate || gate_left != p.gate_rows) end_gate();  // the last row's tokens go on in another chunk, or end
+    } else if (!GATE && c.per_gate && p.dgate) {
+        store_plain<V, NV>(p.ws + (2ull * c.count + team.index) * p.D, dw_post, team, p.D);  // no tokens: zeros
     }
+    if constexpr (!GATE)
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) dw_post[i] = post_sum[i * blockDim.x + threadIdx.x];
+    if (p.dw_pre) store_plain<V, NV>(p.ws + (uint64_t)team.index * p.D, dw_pre, team, p.D);
+    if (p.dw_post) store_plain<V, NV>(p.ws + ((uint64_t)c.count + team.index) * p.D, dw_post, team, p.D);
 }
 
 // Adds the chunks' sums: blockIdx.y 0 and 1 dw_pre and dw_post, 2 + g gate row
@@ -519,28 +618,42 @@ cudaError_t launch(K kernel, dim3 grid, uint32_t threads, uint32_t cluster, cuda
     return e;
 }
 
-template <class R, int V, int E, int THREADS, int CTAS>
+template <class R, int V, int E, int THREADS, int CTAS, int GATE>
 cudaError_t forward_launch(const Forward& p, const Shape& sh, cudaStream_t s) {
-    const uint32_t resident = sh.resident(kForwardThreads);
+    const uint32_t resident = sh.resident(THREADS * CTAS);
     const uint32_t teams = (p.T + sh.teams - 1) / sh.teams < resident ? (p.T + sh.teams - 1) / sh.teams : resident;
-    return launch(forward_kernel<R, V, E / V, THREADS, CTAS>, dim3(teams * (sh.ctas ? sh.ctas : 1)), sh.threads, sh.ctas, s,
+    return launch(forward_kernel<R, V, E / V, THREADS, CTAS, GATE>, dim3(teams * (sh.ctas ? sh.ctas : 1)), sh.threads, sh.ctas, s,
                   p, sh.ctas);
 }
 
 // 8 channels a thread up to 2048 channels, 16 up to 8192 in a CTA of up to 512
-// threads, then two CTAs.
+// threads, then two CTAs.  As many CTAs on an SM as about 85 registers a thread
+// allow (with 64 they spill, with more too few rows are on their way).
+template <class R, int V, int GATE>
+cudaError_t forward_gated(const Forward& p, cudaStream_t s) {
+    if (p.D <= 2048) return forward_launch<R, V, 8, 256, 4, GATE>(p, Shape(p.D, 8, 512), s);
+    if (p.D <= 4096) return forward_launch<R, V, 16, 256, 3, GATE>(p, Shape(p.D, 16, 512), s);
+    if (p.D <= 6144) return forward_launch<R, V, 16, 384, 2, GATE>(p, Shape(p.D, 16, 512), s);
+    return forward_launch<R, V, 16, 512, 1, GATE>(p, Shape(p.D, 16, 512), s);
+}
+
 template <class R, int V>
 cudaError_t forward_typed(const Forward& p, cudaStream_t s) {
-    if (p.D <= 2048) return forward_launch<R, V, 8, 256, 4>(p, Shape(p.D, 8, 512), s);
-    return forward_launch<R, V, 16, 512, 2>(p, Shape(p.D, 16, 512), s);
+    if (!p.gate) return forward_gated<R, V, kNoGate>(p, s);
+    return p.gate_act ? forward_gated<R, V, kSigmoidGate>(p, s) : forward_gated<R, V, kPlainGate>(p, s);
+}
+
+template <class R, int V, int GATE>
+cudaError_t backward_launch(const Backward& p, const Chunks& c, cudaStream_t s) {
+    const Shape sh(p.D, 8, 512);
+    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.ctas ? sh.ctas : 1));
+    return launch(backward_kernel<R, V, 8 / V, 512, GATE>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas);
 }
 
 template <class R, int V>
 cudaError_t backward_typed(const Backward& p, const Chunks& c, cudaStream_t s) {
-    const Shape sh(p.D, 8, 512);
-    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.ctas ? sh.ctas : 1));
-    return p.gate ? launch(backward_kernel<R, V, 8 / V, 512, true>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas)
-                  : launch(backward_kernel<R, V, 8 / V, 512, false>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas);
+    if (!p.gate || p.gate_rows > 1) return backward_launch<R, V, kNoGate>(p, c, s);
+    return p.gate_act ? backward_launch<R, V, kSigmoidGate>(p, c, s) : backward_launch<R, V, kPlainGate>(p, c, s);
 }
 
 }  // namespace
