@@ -1,88 +1,450 @@
-// Embedding rows: scaled lookup and the table's gradient.
+// Embedding rows: scaled lookup, and the table's gradient by sorted tokens.
+//
+// Lookup: bound by HBM, a gather of whole rows: a few threads of one CTA a row,
+// four vectors of 8 channels each on their way.
+//
+// Gradient, three launches:
+//  1. sort_tokens: a stable radix sort of (id, token) in one cluster (one CTA
+//     for few tokens), the digits' counts exchanged through distributed shared
+//     memory; it also marks the rows that are named in a bit map.
+//  2. sum_runs: CTAs take kRun consecutive sorted tokens, add the rows of one
+//     id in registers in that order and write an id's sum to the table where
+//     all of its tokens are in the run; the sums of the first and the last id,
+//     where they go on beyond it, go to the workspace.  Further CTAs write the
+//     zeros of the rows that no token names, so the table is written once.
+//  3. join_runs: adds the parts of the ids that several runs share, in order.
+// Bound by HBM (the table's rows written, the tokens' rows read).  The order of
+// every sum is fixed by the ids alone; there are no floating-point atomics.
 #include "embed_rows.cuh"
 
-#include "common.cuh"
+#include <cstring>
+
+#include "gemm_ptx.cuh"
 
 namespace foil {
 namespace embed {
 namespace {
 
-constexpr int kThreads = 256;
+using gemm::cluster_sync;
+using gemm::map_to_rank;
 
 __device__ __forceinline__ int64_t load_id(const void* ids, int32_t id_bytes, uint64_t t) {
     return id_bytes == 8 ? static_cast<const int64_t*>(ids)[t] : (int64_t)static_cast<const int32_t*>(ids)[t];
 }
-__device__ __forceinline__ float load(const uint16_t* p, uint64_t i) { return bf16_bits_to_f32(p[i]); }
-__device__ __forceinline__ float load(const float* p, uint64_t i) { return p[i]; }
-__device__ __forceinline__ void store(uint16_t* p, uint64_t i, float v) { p[i] = (uint16_t)(cvt_bf16x2(v, 0.0f) & 0xffffu); }
-__device__ __forceinline__ void store(float* p, uint64_t i, float v) { p[i] = v; }
 
-// One CTA for each token.
-template <class O>
-__global__ void __launch_bounds__(kThreads) lookup_kernel(Lookup p) {
-    const uint64_t t = blockIdx.x;
-    const int64_t id = load_id(p.ids, p.id_bytes, t);
-    const bool ok = id != p.pad_id && id >= 0 && id < (int64_t)p.V;
-    if (!ok && id != p.pad_id && threadIdx.x == 0) atomicOr(p.err, kErrBadIndex);
-    O* out = static_cast<O*>(p.out) + t * p.ld_out;
-    for (uint32_t i = threadIdx.x; i < p.D; i += kThreads)
-        store(out, i, ok ? p.scale * load(p.table, (uint64_t)id * p.ld_table + i) : 0.0f);
-}
-
-// One CTA for each table row: looks through all ids.
-template <class I>
-__global__ void __launch_bounds__(kThreads) gradient_kernel(Gradient p) {
-    const uint64_t v = blockIdx.x;
-    float* row = p.dtable + v * p.ld_dtable;
-    __shared__ uint32_t hit;
-    for (uint32_t i0 = 0; i0 < p.D; i0 += kThreads) {
-        const uint32_t i = i0 + threadIdx.x;
-        float s = 0.0f;
-        bool any = false;
-        for (uint32_t t0 = 0; t0 < p.T; t0 += kThreads) {
-            const uint32_t t = t0 + threadIdx.x;
-            const int64_t id = t < p.T ? load_id(p.ids, p.id_bytes, t) : -1;
-            const bool bad = t < p.T && id != p.pad_id && (id < 0 || id >= (int64_t)p.V);
-            if (bad && v == 0) atomicOr(p.err, kErrBadIndex);
-            if (!__syncthreads_or(t < p.T && id == (int64_t)v && id != p.pad_id)) continue;
-            for (uint32_t j = 0; j < kThreads && t0 + j < p.T; ++j) {
-                if (threadIdx.x == j) hit = id == (int64_t)v && id != p.pad_id;
-                __syncthreads();
-                if (hit && i < p.D) s += load(static_cast<const I*>(p.dout) + (uint64_t)(t0 + j) * p.ld_dout, i);
-                any |= hit != 0;
-                __syncthreads();
-            }
+// V values of type T (uint16_t: bf16 bits) to fp32 and back.
+template <int V>
+__device__ __forceinline__ void load(const uint16_t* p, float (&v)[V]) {
+    if constexpr (V == 8) {
+        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = bf16_bits_to_f32(a[i] & 0xffffu);
+            v[2 * i + 1] = __uint_as_float(a[i] & 0xffff0000u);
         }
-        if (i < p.D && (any || !p.accumulate)) row[i] = (p.accumulate ? row[i] : 0.0f) + p.scale * s;
+    } else if constexpr (V == 2) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+        v[0] = bf16_bits_to_f32(w & 0xffffu), v[1] = __uint_as_float(w & 0xffff0000u);
+    } else {
+        v[0] = bf16_bits_to_f32(*p);
+    }
+}
+template <int V>
+__device__ __forceinline__ void load(const float* p, float (&v)[V]) {
+    if constexpr (V == 8) {
+        const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else if constexpr (V == 2) {
+        const float2 a = *reinterpret_cast<const float2*>(p);
+        v[0] = a.x, v[1] = a.y;
+    } else {
+        v[0] = *p;
+    }
+}
+template <int V>
+__device__ __forceinline__ void store(uint16_t* p, const float (&v)[V]) {
+    if constexpr (V == 8)
+        *reinterpret_cast<uint4*>(p) = make_uint4(cvt_bf16x2(v[0], v[1]), cvt_bf16x2(v[2], v[3]),
+                                                  cvt_bf16x2(v[4], v[5]), cvt_bf16x2(v[6], v[7]));
+    else if constexpr (V == 2)
+        *reinterpret_cast<uint32_t*>(p) = cvt_bf16x2(v[0], v[1]);
+    else
+        *p = (uint16_t)(cvt_bf16x2(v[0], 0.0f) & 0xffffu);
+}
+template <int V>
+__device__ __forceinline__ void store(float* p, const float (&v)[V]) {
+    if constexpr (V == 8) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    } else {
+        *p = v[0];
     }
 }
 
-cudaError_t count(cudaError_t e) {
+// Widest vector (8, 2 or 1 channels) for rows of D that every tensor allows.
+struct Width {
+    int v = 8;
+    explicit Width(uint32_t D) {
+        while (v > 1 && D % v) v = v == 8 ? 2 : 1;
+    }
+    void use(const void* p, uint64_t ld, uint64_t elem) {
+        while (v > 1 && ((uintptr_t)p % (v * elem < 16 ? v * elem : 16) || ld % v)) v = v == 8 ? 2 : 1;
+    }
+};
+
+template <class K, class... Args>
+cudaError_t launch(K kernel, dim3 grid, uint32_t threads, uint32_t cluster, cudaStream_t s, Args... args) {
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof cfg);
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads, 1, 1), cfg.stream = s;
+    cudaLaunchAttribute la[2];
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    la[1].id = cudaLaunchAttributeClusterDimension;
+    la[1].val.clusterDim.x = cluster, la[1].val.clusterDim.y = 1, la[1].val.clusterDim.z = 1;
+    cfg.attrs = la, cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e == cudaSuccess) foil_count_launch();
     return e;
+}
+
+// ------------------------------------------------------------------ lookup ---
+constexpr uint32_t kThreads = 256;
+
+// A CTA holds kThreads / team rows at a time, `team` threads each.
+template <class O, int V>
+__global__ void __launch_bounds__(kThreads) lookup_kernel(const Lookup p, uint32_t team) {
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    const uint32_t lane = threadIdx.x % team, per = kThreads / team;
+    for (uint64_t t = (uint64_t)blockIdx.x * per + threadIdx.x / team; t < p.T; t += (uint64_t)gridDim.x * per) {
+        const int64_t id = load_id(p.ids, p.id_bytes, t);
+        const bool ok = id != p.pad_id && id >= 0 && id < (int64_t)p.V;
+        if (!ok && id != p.pad_id && lane == 0) atomicOr(p.err, kErrBadIndex);
+        const uint16_t* row = p.table + (ok ? (uint64_t)id * p.ld_table : 0u);
+        O* out = static_cast<O*>(p.out) + t * p.ld_out;
+        for (uint32_t i0 = lane * V; i0 < p.D; i0 += 4u * team * V) {
+            float v[4][V];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t i = i0 + j * team * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[j][e] = 0.0f;
+                if (ok && i < p.D) load<V>(row + i, v[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t i = i0 + j * team * V;
+                if (i >= p.D) continue;
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[j][e] *= p.scale;
+                store<V>(out + i, v[j]);
+            }
+        }
+    }
+}
+
+template <class O, int V>
+cudaError_t lookup_launch(const Lookup& p, cudaStream_t s) {
+    uint32_t team = 1;
+    while (team < kThreads && (uint64_t)team * 4 * V < p.D) team *= 2;
+    const uint64_t ctas = ((uint64_t)p.T + kThreads / team - 1) / (kThreads / team);
+    const uint64_t most = (uint64_t)foil_sm_count() * 8;
+    return launch(lookup_kernel<O, V>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 1, s, p, team);
+}
+
+// -------------------------------------------------------------------- sort ---
+constexpr uint32_t kRun = 32;         // sorted tokens of a run
+constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxRadix = 256, kSortCtas = 8;
+
+struct Plan {
+    uint32_t runs, slabs, ctas;        // runs of tokens, column slabs of a run, CTAs of the sort
+    uint32_t passes, bits;             // passes of `bits` bits
+    uint32_t *key0, *token0, *key1, *token1;  // buffers of the sort, in turn
+    uint32_t *key, *token;             // those that hold the result
+    uint32_t* marks;                   // a bit for each row that is named
+    float *head, *tail;                // [run][D]: sums that begin before, or end after, the run
+};
+uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
+
+Plan make_plan(const Gradient& p, uint64_t* bytes) {
+    Plan q{};
+    q.runs = (p.T + kRun - 1) / kRun;
+    q.ctas = p.T > 4096 ? kSortCtas : 1;  // below, one CTA is as fast
+    uint32_t bits = 1;
+    while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
+    q.passes = (bits + 7) / 8;
+    q.bits = (bits + q.passes - 1) / q.passes;
+    char* at = static_cast<char*>(p.ws);
+    uint64_t off = 0;
+    auto take = [&](uint64_t n) {
+        char* r = at ? at + off : nullptr;
+        off += align16(n);
+        return r;
+    };
+    q.key0 = (uint32_t*)take(4ull * p.T), q.token0 = (uint32_t*)take(4ull * p.T);
+    q.key1 = (uint32_t*)take(4ull * p.T), q.token1 = (uint32_t*)take(4ull * p.T);
+    q.key = q.passes % 2 ? q.key1 : q.key0, q.token = q.passes % 2 ? q.token1 : q.token0;
+    q.marks = (uint32_t*)take(4ull * ((p.V + 31) / 32));
+    if (q.runs > 1) q.head = (float*)take(4ull * q.runs * p.D), q.tail = (float*)take(4ull * q.runs * p.D);
+    if (bytes) *bytes = off;
+    return q;
+}
+
+__global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p, const Plan q) {
+    __shared__ uint32_t count[kSortWarps][kMaxRadix];     // of a warp's digits, then their next places
+    __shared__ uint32_t total[kSortCtas][kMaxRadix];      // of every CTA's digits
+    __shared__ uint32_t scan[kMaxRadix / 32];
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = blockIdx.x, ctas = q.ctas;
+    const uint32_t radix = 1u << q.bits, tid = threadIdx.x;
+    auto sync_all = [&] {
+        if (ctas > 1)
+            cluster_sync();
+        else
+            __syncthreads();
+    };
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    for (uint32_t i = rank * kSortThreads + tid; i < (p.V + 31u) / 32u; i += ctas * kSortThreads) q.marks[i] = 0u;
+    // This warp's tokens, in order.
+    const uint32_t part = rank * kSortWarps + warp, parts = ctas * kSortWarps;
+    const uint32_t first = (uint32_t)((uint64_t)p.T * part / parts), last = (uint32_t)((uint64_t)p.T * (part + 1) / parts);
+    if (ctas > 1) cluster_sync();  // every CTA runs before its memory is written
+    for (uint32_t pass = 0; pass < q.passes; ++pass) {
+        const uint32_t *key_in = pass % 2 ? q.key1 : q.key0, *token_in = pass % 2 ? q.token1 : q.token0;
+        uint32_t *key_out = pass % 2 ? q.key0 : q.key1, *token_out = pass % 2 ? q.token0 : q.token1;
+        const uint32_t shift = pass * q.bits;
+        auto key_of = [&](uint32_t i) {
+            if (pass) return __ldcg(key_in + i);
+            const int64_t id = load_id(p.ids, p.id_bytes, i);
+            if (id == p.pad_id) return p.V;
+            if (id >= 0 && id < (int64_t)p.V) return (uint32_t)id;
+            atomicOr(p.err, kErrBadIndex);
+            return p.V;
+        };
+        for (uint32_t d = lane; d < radix; d += 32u) count[warp][d] = 0u;
+        __syncwarp();
+        for (uint32_t i0 = first; i0 < last; i0 += 32u) {
+            const uint32_t i = i0 + lane;
+            const uint32_t d = i < last ? key_of(i) >> shift & (radix - 1u) : ~0u;
+            const uint32_t peers = __match_any_sync(0xffffffffu, d);
+            if (i < last && (peers & ((1u << lane) - 1u)) == 0u) count[warp][d] += __popc(peers);
+            __syncwarp();
+        }
+        __syncthreads();
+        // Digit tid: the tokens of the warps before each warp, and of the CTA.
+        if (tid < radix) {
+            uint32_t sum = 0;
+            for (uint32_t w = 0; w < kSortWarps; ++w) {
+                const uint32_t n = count[w][tid];
+                count[w][tid] = sum;
+                sum += n;
+            }
+            if (ctas == 1)
+                total[0][tid] = sum;
+            else
+                for (uint32_t c = 0; c < ctas; ++c)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(&total[rank][tid], c)), "r"(sum)
+                                 : "memory");
+        }
+        sync_all();
+        // The places of digit tid: after all smaller digits, after the CTAs before.
+        uint32_t all = 0, before = 0, incl = 0;
+        if (tid < kMaxRadix) {
+            if (tid < radix)
+                for (uint32_t c = 0; c < ctas; ++c) {
+                    const uint32_t n = total[c][tid];
+                    all += n;
+                    before += c < rank ? n : 0u;
+                }
+            incl = all;
+            for (uint32_t o = 1; o < 32u; o <<= 1) {
+                const uint32_t n = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += n;
+            }
+            if (lane == 31u) scan[warp] = incl;
+        }
+        __syncthreads();
+        if (tid < radix) {
+            uint32_t base = incl - all + before;
+            for (uint32_t w = 0; w < warp; ++w) base += scan[w];
+            for (uint32_t w = 0; w < kSortWarps; ++w) count[w][tid] += base;
+        }
+        __syncthreads();
+        const bool done = pass + 1 == q.passes;
+        for (uint32_t i0 = first; i0 < last; i0 += 32u) {
+            const uint32_t i = i0 + lane;
+            const uint32_t key = i < last ? key_of(i) : ~0u, d = i < last ? key >> shift & (radix - 1u) : ~0u;
+            const uint32_t peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1u);
+            uint32_t at = 0;
+            if (i < last) at = count[warp][d] + __popc(lower);
+            __syncwarp();
+            if (i < last) {
+                if (lower == 0u) count[warp][d] += __popc(peers);
+                key_out[at] = key;
+                token_out[at] = pass ? __ldcg(token_in + i) : i;
+                if (done && key < p.V) atomicOr(q.marks + key / 32u, 1u << key % 32u);
+            }
+            __syncwarp();
+        }
+        sync_all();
+    }
+}
+
+// -------------------------------------------------------------------- sums ---
+constexpr uint32_t kAhead = 8;  // rows of tokens on their way
+
+template <class I, int V>
+__global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Plan q) {
+    __shared__ uint32_t key[kRun + 2], token[kRun];
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    const uint64_t sums = (uint64_t)q.runs * q.slabs;
+    if (blockIdx.x >= sums) {
+        // 32 rows of the table: zeros where no token names them, a warp a row.
+        const uint32_t word = (uint32_t)(blockIdx.x - sums), marks = __ldcg(q.marks + word);
+        for (uint32_t r = threadIdx.x / 32u; r < 32u; r += kThreads / 32u) {
+            const uint64_t v = (uint64_t)word * 32u + r;
+            if (v >= p.V || marks >> r & 1u) continue;
+            float* row = p.dtable + v * p.ld_dtable;
+            const float zero[V] = {};
+            for (uint32_t i = threadIdx.x % 32u * V; i < p.D; i += 32u * V) store<V>(row + i, zero);
+        }
+        return;
+    }
+    const uint32_t run = (uint32_t)(blockIdx.x / q.slabs), first = run * kRun, n = min(kRun, p.T - first);
+    const uint32_t *keys = q.key, *tokens = q.token;
+    if (threadIdx.x < kRun + 2u) {  // the keys before and after the run too
+        const uint32_t i = first + threadIdx.x - 1u;
+        key[threadIdx.x] = first + threadIdx.x >= 1u && i < p.T ? __ldcg(keys + i) : ~0u;
+        if (threadIdx.x >= 1u && threadIdx.x <= kRun && i < p.T) token[threadIdx.x - 1u] = __ldcg(tokens + i);
+    }
+    __syncthreads();
+    const uint32_t col = (blockIdx.x % q.slabs * kThreads + threadIdx.x) * V;
+    if (col >= p.D) return;
+    const I* dout = static_cast<const I*>(p.dout) + col;
+    float acc[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+    bool before = key[0] == key[1];  // the id began before the run
+    for (uint32_t r0 = 0; r0 < n; r0 += kAhead) {
+        float x[kAhead][V];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t r = min(r0 + j, n - 1u);  // past the end: read again, not used
+            load<V>(dout + (uint64_t)token[r] * p.ld_dout, x[j]);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t r = r0 + j;
+            if (r >= n || key[r + 1] >= p.V) return;  // padding and bad ids come last
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] += x[j][e];
+            const bool ends = key[r + 2] != key[r + 1];
+            if (!ends && r + 1u < n) continue;
+            if (ends && !before) {
+                float* row = p.dtable + (uint64_t)key[r + 1] * p.ld_dtable + col;
+                float v[V];
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = 0.0f;
+                if (p.accumulate) load<V>(row, v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[e] = fmaf(p.scale, acc[e], v[e]);
+                store<V>(row, v);
+            } else {
+                float* part = (before ? q.head : q.tail) + (uint64_t)run * p.D + col;
+#pragma unroll
+                for (int e = 0; e < V; ++e) part[e] = acc[e];
+            }
+            before = false;
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[e] = 0.0f;
+        }
+    }
+}
+
+// blockIdx.x: a run whose last id begins there and goes on; blockIdx.y: 128
+// columns.  8 warps take every eighth part, their sums are added in order.
+__global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Plan q) {
+    __shared__ float part[kThreads / 32][128];
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    const uint32_t *keys = q.key, run = blockIdx.x, first = run * kRun, end = first + kRun;
+    if (end >= p.T) return;
+    const uint32_t id = __ldcg(keys + end - 1u);
+    if (id >= p.V || __ldcg(keys + end) != id) return;
+    if (first && __ldcg(keys + first) == id && __ldcg(keys + first - 1u) == id) return;  // began earlier
+    // Runs after this one that begin with the id: binary search.
+    uint32_t lo = run + 1u, hi = q.runs;  // lo begins with it, hi does not
+    while (hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        (__ldcg(keys + mid * kRun) == id ? lo : hi) = mid;
+    }
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, col = blockIdx.y * 128u + lane;
+    float s[4] = {};
+    for (uint32_t r = run + warp; r < hi; r += kThreads / 32u) {
+        const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col + 32u * j < p.D) s[j] += row[32 * j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) part[warp][lane + 32 * j] = s[j];
+    __syncthreads();
+    const uint32_t i = blockIdx.y * 128u + threadIdx.x;
+    if (threadIdx.x >= 128u || i >= p.D) return;
+    float sum = 0.0f;
+    for (uint32_t w = 0; w < kThreads / 32u; ++w) sum += part[w][threadIdx.x];
+    float* at = p.dtable + (uint64_t)id * p.ld_dtable + i;
+    *at = fmaf(p.scale, sum, p.accumulate ? *at : 0.0f);
+}
+
+template <class I>
+cudaError_t sum_launch(const Gradient& p, Plan q, int v, cudaStream_t s) {
+    q.slabs = (p.D + kThreads * v - 1) / (kThreads * v);
+    const uint64_t grid = (uint64_t)q.runs * q.slabs + (p.accumulate ? 0 : (p.V + 31) / 32);
+    if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
+    const dim3 g((unsigned)grid);
+    if (v == 8) return launch(sum_runs<I, 8>, g, kThreads, 1, s, p, q);
+    return v == 2 ? launch(sum_runs<I, 2>, g, kThreads, 1, s, p, q) : launch(sum_runs<I, 1>, g, kThreads, 1, s, p, q);
 }
 
 }  // namespace
 
 uint64_t gradient_ws_bytes(uint32_t T, uint32_t V, uint32_t D) {
-    (void)T, (void)V, (void)D;
-    return 0;
+    if (T == 0 || V == 0 || D == 0) return 0;
+    Gradient p{};
+    p.T = T, p.V = V, p.D = D;
+    uint64_t bytes = 0;
+    make_plan(p, &bytes);
+    return bytes;
 }
 
 cudaError_t lookup(const Lookup& p, bool fp32, cudaStream_t s) {
+    Width w(p.D);
+    w.use(p.table, p.ld_table, 2), w.use(p.out, p.ld_out, fp32 ? 4 : 2);
     if (fp32)
-        lookup_kernel<float><<<p.T, kThreads, 0, s>>>(p);
-    else
-        lookup_kernel<uint16_t><<<p.T, kThreads, 0, s>>>(p);
-    return count(cudaGetLastError());
+        return w.v == 8 ? lookup_launch<float, 8>(p, s)
+                        : w.v == 2 ? lookup_launch<float, 2>(p, s) : lookup_launch<float, 1>(p, s);
+    return w.v == 8 ? lookup_launch<uint16_t, 8>(p, s)
+                    : w.v == 2 ? lookup_launch<uint16_t, 2>(p, s) : lookup_launch<uint16_t, 1>(p, s);
 }
 
 cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
-    if (fp32)
-        gradient_kernel<float><<<p.V, kThreads, 0, s>>>(p);
-    else
-        gradient_kernel<uint16_t><<<p.V, kThreads, 0, s>>>(p);
-    return count(cudaGetLastError());
+    if (p.T == 0)
+        return p.accumulate ? cudaSuccess
+                            : cudaMemset2DAsync(p.dtable, p.ld_dtable * 4, 0, (size_t)p.D * 4, p.V, s);
+    const Plan q = make_plan(p, nullptr);
+    cudaError_t e = launch(sort_tokens, dim3(q.ctas), kSortThreads, q.ctas, s, p, q);
+    if (e != cudaSuccess) return e;
+    Width w(p.D);
+    w.use(p.dout, p.ld_dout, fp32 ? 4 : 2), w.use(p.dtable, p.ld_dtable, 4);
+    e = fp32 ? sum_launch<float>(p, q, w.v, s) : sum_launch<uint16_t>(p, q, w.v, s);
+    if (e != cudaSuccess || q.runs < 2) return e;
+    return launch(join_runs, dim3(q.runs, (p.D + 127) / 128), kThreads, 1, s, p, q);
 }
 
 }  // namespace embed
