@@ -94,8 +94,15 @@ template <int V>
 __device__ __forceinline__ void put(float* p, const float2* v, int j) {
     if constexpr (V == 8) {
         v += 4 * j;
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        if (((uintptr_t)p & 31u) == 0) {  // one store of whole sectors
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(i % 2 ? v[i / 2].y : v[i / 2].x);
+            gemm::st_global_v8(p, w);
+        } else {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        }
     } else if constexpr (V == 2) {
         *reinterpret_cast<float2*>(p) = v[j];
     } else {

@@ -6,12 +6,13 @@
 // Gradient, three launches:
 //  1. sort_tokens: a stable radix sort of (id, token) in one cluster (one CTA
 //     for few tokens), the digits' counts exchanged through distributed shared
-//     memory; it also marks the rows that are named in a bit map.
+//     memory.  Meanwhile the other SMs write the zeros of the table's rows that
+//     no token names (each CTA looks through the ids for its rows), so the
+//     table is written once.
 //  2. sum_runs: CTAs take kRun consecutive sorted tokens, add the rows of one
 //     id in registers in that order and write an id's sum to the table where
 //     all of its tokens are in the run; the sums of the first and the last id,
-//     where they go on beyond it, go to the workspace.  Further CTAs write the
-//     zeros of the rows that no token names, so the table is written once.
+//     where they go on beyond it, go to the workspace.
 //  3. join_runs: adds the parts of the ids that several runs share, in order.
 // Bound by HBM (the table's rows written, the tokens' rows read).  The order of
 // every sum is fixed by the ids alone; there are no floating-point atomics.
@@ -75,8 +76,17 @@ __device__ __forceinline__ void store(uint16_t* p, const float (&v)[V]) {
 template <int V>
 __device__ __forceinline__ void store(float* p, const float (&v)[V]) {
     if constexpr (V == 8) {
-        reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        // One store of whole sectors where the address allows (two of half
+        // sectors each reached two thirds of the bandwidth).
+        uint32_t w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(v[i]);
+        if (((uintptr_t)p & 31u) == 0) {
+            gemm::st_global_v8(p, w);
+        } else {
+            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        }
     } else if constexpr (V == 2) {
         *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
     } else {
@@ -96,10 +106,11 @@ struct Width {
 };
 
 template <class K, class... Args>
-cudaError_t launch(K kernel, dim3 grid, uint32_t threads, uint32_t cluster, cudaStream_t s, Args... args) {
+cudaError_t launch(K kernel, dim3 grid, uint32_t threads, uint32_t smem, uint32_t cluster, cudaStream_t s,
+                   Args... args) {
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof cfg);
-    cfg.gridDim = grid, cfg.blockDim = dim3(threads, 1, 1), cfg.stream = s;
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads, 1, 1), cfg.dynamicSmemBytes = smem, cfg.stream = s;
     cudaLaunchAttribute la[2];
     la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     la[0].val.programmaticStreamSerializationAllowed = 1;
@@ -153,19 +164,24 @@ cudaError_t lookup_launch(const Lookup& p, cudaStream_t s) {
     while (team < kThreads && (uint64_t)team * 4 * V < p.D) team *= 2;
     const uint64_t ctas = ((uint64_t)p.T + kThreads / team - 1) / (kThreads / team);
     const uint64_t most = (uint64_t)foil_sm_count() * 8;
-    return launch(lookup_kernel<O, V>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 1, s, p, team);
+    return launch(lookup_kernel<O, V>, dim3((unsigned)(ctas < most ? ctas : most)), kThreads, 0, 1, s, p, team);
 }
 
 // -------------------------------------------------------------------- sort ---
 constexpr uint32_t kRun = 32;         // sorted tokens of a run
-constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kMaxRadix = 256, kSortCtas = 8;
+constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
+constexpr uint32_t kMaxBits = 9, kMaxRadix = 1u << kMaxBits;
+// A warp's counts of each digit, every CTA's, and the scan's; or the marks of
+// a clearing CTA's rows.
+constexpr uint32_t kSortSmem = (kSortWarps * kMaxRadix + kSortCtas * kMaxRadix + 32) * 4;
+constexpr uint32_t kMarkRows = kSortSmem * 8 / 32 * 32;  // rows that one CTA can clear
 
 struct Plan {
-    uint32_t runs, slabs, ctas;        // runs of tokens, column slabs of a run, CTAs of the sort
+    uint32_t runs, slabs;              // runs of tokens, column slabs of a run
+    uint32_t ctas, clear;              // CTAs of the sort, CTAs that clear rows
     uint32_t passes, bits;             // passes of `bits` bits
     uint32_t *key0, *token0, *key1, *token1;  // buffers of the sort, in turn
     uint32_t *key, *token;             // those that hold the result
-    uint32_t* marks;                   // a bit for each row that is named
     float *head, *tail;                // [run][D]: sums that begin before, or end after, the run
 };
 uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
@@ -176,7 +192,7 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     q.ctas = p.T > 4096 ? kSortCtas : 1;  // below, one CTA is as fast
     uint32_t bits = 1;
     while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
-    q.passes = (bits + 7) / 8;
+    q.passes = (bits + kMaxBits - 1) / kMaxBits;
     q.bits = (bits + q.passes - 1) / q.passes;
     char* at = static_cast<char*>(p.ws);
     uint64_t off = 0;
@@ -188,16 +204,38 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     q.key0 = (uint32_t*)take(4ull * p.T), q.token0 = (uint32_t*)take(4ull * p.T);
     q.key1 = (uint32_t*)take(4ull * p.T), q.token1 = (uint32_t*)take(4ull * p.T);
     q.key = q.passes % 2 ? q.key1 : q.key0, q.token = q.passes % 2 ? q.token1 : q.token0;
-    q.marks = (uint32_t*)take(4ull * ((p.V + 31) / 32));
     if (q.runs > 1) q.head = (float*)take(4ull * q.runs * p.D), q.tail = (float*)take(4ull * q.runs * p.D);
     if (bytes) *bytes = off;
     return q;
 }
 
+// Zeros to the rows [v0, v1) that no token names.
+template <int V>
+__device__ __forceinline__ void clear_rows(const Gradient& p, uint32_t* marks, uint32_t v0, uint32_t v1) {
+    const uint32_t tid = threadIdx.x, warp = tid / 32u, lane = tid % 32u;
+    for (uint32_t i = tid; i < (v1 - v0 + 31u) / 32u; i += kSortThreads) marks[i] = 0u;
+    __syncthreads();
+#pragma unroll 4
+    for (uint32_t t = tid; t < p.T; t += kSortThreads) {
+        const int64_t id = load_id(p.ids, p.id_bytes, t);
+        if (id >= (int64_t)v0 && id < (int64_t)v1 && id != p.pad_id)
+            atomicOr(&marks[((uint32_t)id - v0) / 32u], 1u << ((uint32_t)id - v0) % 32u);
+    }
+    __syncthreads();
+    const float zero[V] = {};
+    for (uint32_t r = warp; r < v1 - v0; r += kSortWarps) {
+        if (marks[r / 32u] >> r % 32u & 1u) continue;
+        float* row = p.dtable + (uint64_t)(v0 + r) * p.ld_dtable;
+        for (uint32_t i = lane * V; i < p.D; i += 32u * V) store<V>(row + i, zero);
+    }
+}
+
+template <int V>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p, const Plan q) {
-    __shared__ uint32_t count[kSortWarps][kMaxRadix];     // of a warp's digits, then their next places
-    __shared__ uint32_t total[kSortCtas][kMaxRadix];      // of every CTA's digits
-    __shared__ uint32_t scan[kMaxRadix / 32];
+    extern __shared__ __align__(16) uint32_t smem[];
+    __shared__ uint32_t warp_sum[kMaxRadix / 32];
+    uint32_t* const count = smem;                                // [warp][digit]: counts, then next places
+    uint32_t* const total = smem + kSortWarps * kMaxRadix;       // [CTA][digit]
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, rank = blockIdx.x, ctas = q.ctas;
     const uint32_t radix = 1u << q.bits, tid = threadIdx.x;
     auto sync_all = [&] {
@@ -208,10 +246,15 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p,
     };
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
-    for (uint32_t i = rank * kSortThreads + tid; i < (p.V + 31u) / 32u; i += ctas * kSortThreads) q.marks[i] = 0u;
+    if (rank >= ctas) {
+        const uint64_t c = rank - ctas;
+        clear_rows<V>(p, smem, (uint32_t)(p.V * c / q.clear), (uint32_t)(p.V * (c + 1) / q.clear));
+        return;
+    }
     // This warp's tokens, in order.
     const uint32_t part = rank * kSortWarps + warp, parts = ctas * kSortWarps;
     const uint32_t first = (uint32_t)((uint64_t)p.T * part / parts), last = (uint32_t)((uint64_t)p.T * (part + 1) / parts);
+    uint32_t* const mine = count + warp * kMaxRadix;
     if (ctas > 1) cluster_sync();  // every CTA runs before its memory is written
     for (uint32_t pass = 0; pass < q.passes; ++pass) {
         const uint32_t *key_in = pass % 2 ? q.key1 : q.key0, *token_in = pass % 2 ? q.token1 : q.token0;
@@ -225,29 +268,34 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p,
             atomicOr(p.err, kErrBadIndex);
             return p.V;
         };
-        for (uint32_t d = lane; d < radix; d += 32u) count[warp][d] = 0u;
+        for (uint32_t d = lane; d < radix; d += 32u) mine[d] = 0u;
         __syncwarp();
         for (uint32_t i0 = first; i0 < last; i0 += 32u) {
             const uint32_t i = i0 + lane;
             const uint32_t d = i < last ? key_of(i) >> shift & (radix - 1u) : ~0u;
             const uint32_t peers = __match_any_sync(0xffffffffu, d);
-            if (i < last && (peers & ((1u << lane) - 1u)) == 0u) count[warp][d] += __popc(peers);
+            if (i < last && (peers & ((1u << lane) - 1u)) == 0u) mine[d] += __popc(peers);
             __syncwarp();
         }
         __syncthreads();
         // Digit tid: the tokens of the warps before each warp, and of the CTA.
+        uint32_t n[kSortWarps];
         if (tid < radix) {
             uint32_t sum = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < kSortWarps; ++w) n[w] = count[w * kMaxRadix + tid];
+#pragma unroll
             for (uint32_t w = 0; w < kSortWarps; ++w) {
-                const uint32_t n = count[w][tid];
-                count[w][tid] = sum;
-                sum += n;
+                const uint32_t k = n[w];
+                n[w] = sum;
+                sum += k;
             }
             if (ctas == 1)
-                total[0][tid] = sum;
+                total[tid] = sum;
             else
                 for (uint32_t c = 0; c < ctas; ++c)
-                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(&total[rank][tid], c)), "r"(sum)
+                    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(map_to_rank(total + rank * kMaxRadix + tid, c)),
+                                 "r"(sum)
                                  : "memory");
         }
         sync_all();
@@ -256,37 +304,37 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p,
         if (tid < kMaxRadix) {
             if (tid < radix)
                 for (uint32_t c = 0; c < ctas; ++c) {
-                    const uint32_t n = total[c][tid];
-                    all += n;
-                    before += c < rank ? n : 0u;
+                    const uint32_t k = total[c * kMaxRadix + tid];
+                    all += k;
+                    before += c < rank ? k : 0u;
                 }
             incl = all;
             for (uint32_t o = 1; o < 32u; o <<= 1) {
-                const uint32_t n = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= o) incl += n;
+                const uint32_t k = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += k;
             }
-            if (lane == 31u) scan[warp] = incl;
+            if (lane == 31u) warp_sum[warp] = incl;
         }
         __syncthreads();
         if (tid < radix) {
             uint32_t base = incl - all + before;
-            for (uint32_t w = 0; w < warp; ++w) base += scan[w];
-            for (uint32_t w = 0; w < kSortWarps; ++w) count[w][tid] += base;
+            for (uint32_t w = 0; w < warp; ++w) base += warp_sum[w];
+#pragma unroll
+            for (uint32_t w = 0; w < kSortWarps; ++w) count[w * kMaxRadix + tid] = n[w] + base;
         }
         __syncthreads();
-        const bool done = pass + 1 == q.passes;
         for (uint32_t i0 = first; i0 < last; i0 += 32u) {
             const uint32_t i = i0 + lane;
             const uint32_t key = i < last ? key_of(i) : ~0u, d = i < last ? key >> shift & (radix - 1u) : ~0u;
+            const uint32_t token = i >= last ? 0u : pass ? __ldcg(token_in + i) : i;
             const uint32_t peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1u);
             uint32_t at = 0;
-            if (i < last) at = count[warp][d] + __popc(lower);
+            if (i < last) at = mine[d] + __popc(lower);
             __syncwarp();
             if (i < last) {
-                if (lower == 0u) count[warp][d] += __popc(peers);
+                if (lower == 0u) mine[d] += __popc(peers);
                 key_out[at] = key;
-                token_out[at] = pass ? __ldcg(token_in + i) : i;
-                if (done && key < p.V) atomicOr(q.marks + key / 32u, 1u << key % 32u);
+                token_out[at] = token;
             }
             __syncwarp();
         }
@@ -302,19 +350,6 @@ __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Pla
     __shared__ uint32_t key[kRun + 2], token[kRun];
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
-    const uint64_t sums = (uint64_t)q.runs * q.slabs;
-    if (blockIdx.x >= sums) {
-        // 32 rows of the table: zeros where no token names them, a warp a row.
-        const uint32_t word = (uint32_t)(blockIdx.x - sums), marks = __ldcg(q.marks + word);
-        for (uint32_t r = threadIdx.x / 32u; r < 32u; r += kThreads / 32u) {
-            const uint64_t v = (uint64_t)word * 32u + r;
-            if (v >= p.V || marks >> r & 1u) continue;
-            float* row = p.dtable + v * p.ld_dtable;
-            const float zero[V] = {};
-            for (uint32_t i = threadIdx.x % 32u * V; i < p.D; i += 32u * V) store<V>(row + i, zero);
-        }
-        return;
-    }
     const uint32_t run = (uint32_t)(blockIdx.x / q.slabs), first = run * kRun, n = min(kRun, p.T - first);
     const uint32_t *keys = q.key, *tokens = q.token;
     if (threadIdx.x < kRun + 2u) {  // the keys before and after the run too
@@ -366,50 +401,74 @@ __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Pla
     }
 }
 
-// blockIdx.x: a run whose last id begins there and goes on; blockIdx.y: 128
+// blockIdx.x: a run whose last id begins there and goes on; blockIdx.y: 256
 // columns.  8 warps take every eighth part, their sums are added in order.
+constexpr uint32_t kJoinColumns = 256;
+
 __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Plan q) {
-    __shared__ float part[kThreads / 32][128];
+    __shared__ float part[kThreads / 32][kJoinColumns];
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
     const uint32_t *keys = q.key, run = blockIdx.x, first = run * kRun, end = first + kRun;
     if (end >= p.T) return;
-    const uint32_t id = __ldcg(keys + end - 1u);
-    if (id >= p.V || __ldcg(keys + end) != id) return;
-    if (first && __ldcg(keys + first) == id && __ldcg(keys + first - 1u) == id) return;  // began earlier
-    // Runs after this one that begin with the id: binary search.
-    uint32_t lo = run + 1u, hi = q.runs;  // lo begins with it, hi does not
+    const uint32_t id = __ldcg(keys + end - 1u), next = __ldcg(keys + end), begin = __ldcg(keys + first);
+    const uint32_t previous = first ? __ldcg(keys + first - 1u) : ~0u;
+    if (id >= p.V || next != id) return;
+    if (begin == id && previous == id) return;  // began earlier
+    // Runs after this one that begin with the id: lo begins with it, hi does
+    // not; 32 places between them at a time.
+    uint32_t lo = run + 1u, hi = q.runs;
     while (hi - lo > 1u) {
-        const uint32_t mid = lo + (hi - lo) / 2u;
-        (__ldcg(keys + mid * kRun) == id ? lo : hi) = mid;
+        const uint32_t step = (hi - lo + 32u) / 33u, at = lo + (threadIdx.x % 32u + 1u) * step;
+        const uint32_t in = __popc(__ballot_sync(0xffffffffu, at < hi && __ldcg(keys + (uint64_t)at * kRun) == id));
+        hi = min(hi, lo + (in + 1u) * step);
+        lo += in * step;
     }
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, col = blockIdx.y * 128u + lane;
-    float s[4] = {};
+    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, col = blockIdx.y * kJoinColumns + lane;
+    constexpr int kEach = kJoinColumns / 32;
+    float s[kEach] = {};
     for (uint32_t r = run + warp; r < hi; r += kThreads / 32u) {
         const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < kEach; ++j)
             if (col + 32u * j < p.D) s[j] += row[32 * j];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) part[warp][lane + 32 * j] = s[j];
+    for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = s[j];
     __syncthreads();
-    const uint32_t i = blockIdx.y * 128u + threadIdx.x;
-    if (threadIdx.x >= 128u || i >= p.D) return;
-    float sum = 0.0f;
-    for (uint32_t w = 0; w < kThreads / 32u; ++w) sum += part[w][threadIdx.x];
-    float* at = p.dtable + (uint64_t)id * p.ld_dtable + i;
-    *at = fmaf(p.scale, sum, p.accumulate ? *at : 0.0f);
+    for (uint32_t k = threadIdx.x; k < kJoinColumns; k += kThreads) {
+        const uint32_t i = blockIdx.y * kJoinColumns + k;
+        if (i >= p.D) return;
+        float sum = 0.0f;
+        for (uint32_t w = 0; w < kThreads / 32u; ++w) sum += part[w][k];
+        float* at = p.dtable + (uint64_t)id * p.ld_dtable + i;
+        *at = fmaf(p.scale, sum, p.accumulate ? *at : 0.0f);
+    }
+}
+
+template <int V>
+cudaError_t sort_launch(const Gradient& p, Plan& q, cudaStream_t s) {
+    // The other SMs clear rows, as many CTAs as run beside the sort.
+    const uint32_t sms = (uint32_t)foil_sm_count(), fit = q.ctas > 1 ? foil_resident_clusters(q.ctas) * q.ctas : sms;
+    q.clear = 0;
+    if (!p.accumulate) {
+        q.clear = fit > q.ctas ? fit - q.ctas : q.ctas;
+        while ((uint64_t)q.clear * kMarkRows < p.V + q.clear) q.clear += q.ctas;
+    }
+    const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(sort_tokens<V>), (int)kSortSmem);
+    if (e != cudaSuccess) return e;
+    return launch(sort_tokens<V>, dim3(q.ctas + q.clear), kSortThreads, kSortSmem, q.ctas, s, p, q);
 }
 
 template <class I>
 cudaError_t sum_launch(const Gradient& p, Plan q, int v, cudaStream_t s) {
     q.slabs = (p.D + kThreads * v - 1) / (kThreads * v);
-    const uint64_t grid = (uint64_t)q.runs * q.slabs + (p.accumulate ? 0 : (p.V + 31) / 32);
+    const uint64_t grid = (uint64_t)q.runs * q.slabs;
     if (grid > 0x7fffffffull) return cudaErrorInvalidConfiguration;
     const dim3 g((unsigned)grid);
-    if (v == 8) return launch(sum_runs<I, 8>, g, kThreads, 1, s, p, q);
-    return v == 2 ? launch(sum_runs<I, 2>, g, kThreads, 1, s, p, q) : launch(sum_runs<I, 1>, g, kThreads, 1, s, p, q);
+    if (v == 8) return launch(sum_runs<I, 8>, g, kThreads, 0, 1, s, p, q);
+    return v == 2 ? launch(sum_runs<I, 2>, g, kThreads, 0, 1, s, p, q)
+                  : launch(sum_runs<I, 1>, g, kThreads, 0, 1, s, p, q);
 }
 
 }  // namespace
@@ -437,14 +496,15 @@ cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
     if (p.T == 0)
         return p.accumulate ? cudaSuccess
                             : cudaMemset2DAsync(p.dtable, p.ld_dtable * 4, 0, (size_t)p.D * 4, p.V, s);
-    const Plan q = make_plan(p, nullptr);
-    cudaError_t e = launch(sort_tokens, dim3(q.ctas), kSortThreads, q.ctas, s, p, q);
-    if (e != cudaSuccess) return e;
+    Plan q = make_plan(p, nullptr);
     Width w(p.D);
-    w.use(p.dout, p.ld_dout, fp32 ? 4 : 2), w.use(p.dtable, p.ld_dtable, 4);
+    w.use(p.dtable, p.ld_dtable, 4);
+    cudaError_t e = w.v == 8 ? sort_launch<8>(p, q, s) : w.v == 2 ? sort_launch<2>(p, q, s) : sort_launch<1>(p, q, s);
+    if (e != cudaSuccess) return e;
+    w.use(p.dout, p.ld_dout, fp32 ? 4 : 2);
     e = fp32 ? sum_launch<float>(p, q, w.v, s) : sum_launch<uint16_t>(p, q, w.v, s);
     if (e != cudaSuccess || q.runs < 2) return e;
-    return launch(join_runs, dim3(q.runs, (p.D + 127) / 128), kThreads, 1, s, p, q);
+    return launch(join_runs, dim3(q.runs, (p.D + kJoinColumns - 1) / kJoinColumns), kThreads, 0, 1, s, p, q);
 }
 
 }  // namespace embed
