@@ -189,7 +189,9 @@ uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
 Plan make_plan(const Gradient& p, uint64_t* bytes) {
     Plan q{};
     q.runs = (p.T + kRun - 1) / kRun;
-    q.ctas = p.T > 4096 ? kSortCtas : 1;  // below, one CTA is as fast
+    // One CTA sorts few tokens as fast.  Clusters of 4 leave 128 SMs to the
+    // zeros, of 8 only 112 (a cluster stays inside a GPC).
+    q.ctas = p.T <= 4096 ? 1 : p.accumulate ? kSortCtas : kSortCtas / 2;
     uint32_t bits = 1;
     while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
     q.passes = (bits + kMaxBits - 1) / kMaxBits;

@@ -14,12 +14,6 @@ using gemm::cp_async16;
 using gemm::map_to_rank;
 using gemm::smem_u32;
 
-// Element index of (row r, column c) in a tile stream of ct tile columns.
-__device__ __forceinline__ uint64_t tile_index(uint32_t r, uint32_t c, uint32_t ct) {
-    return ((uint64_t)(r / 32u) * ct + c / 32u) * 1024u + ((r % 32u / 16u) * 2u + c % 32u / 16u) * 256u +
-           (r % 16u) * 16u + c % 16u;
-}
-
 // Byte offset of the 32-bit word of codes that holds (n, k..k+7), k % 8 == 0.
 __device__ __forceinline__ uint64_t word_offset(uint32_t n, uint32_t k, uint32_t kb, uint32_t bytes) {
     return ((uint64_t)(n / kBlockN) * kb + k / kBlockK) * bytes +
@@ -58,67 +52,260 @@ __global__ void pack_kernel(const uint8_t* __restrict__ codes, const uint16_t* _
     }
 }
 
-// One thread for each (column, group).
-__global__ void quantize_kernel(const uint16_t* __restrict__ tiles, uint8_t* __restrict__ packed, Weights w,
-                                uint32_t kb, uint64_t groups) {
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= groups) return;
-    const uint32_t np = (w.N + 15u) / 16u * 16u;
-    const uint32_t n = (uint32_t)(i % np), k0 = (uint32_t)(i / np) * w.group;
-    const uint32_t bytes = block_bytes(w.group, w.zeros), ct = w.N / 32u;
-    float lo = 0.0f, hi = 0.0f;
-    bool bad = false;
-    for (uint32_t k = k0; k < k0 + w.group && k < w.K && n < w.N; ++k) {
-        const float v = bf16_bits_to_f32(tiles[tile_index(k, n, ct)]);
-        bad |= !isfinite(v);
-        lo = fminf(lo, v);
-        hi = fmaxf(hi, v);
+// ---------------------------------------------------- tile stream <-> codes ---
+// One warp a storage block: 16 columns n by 128 k are the same face column of
+// four tiles, eight faces of 512 contiguous bytes.  Lane l of a face holds its
+// row k = l / 2, columns 8 (l % 2) + 0..7; in the storage a lane holds words
+// of one column and 8 k.  Between the two lies an 8 x 8 transpose of codes
+// over the 8 lanes of equal l % 2 and l / 16, three exchanges of half a word.
+// Bound by HBM; no shared memory, 16-byte accesses in whole sectors.
+
+// Codes in word position i + 4 j stand for element 2 i + j (column or k), so
+// that bits i and i + 16 are a bf16 pair's.  With e the element's bits: position
+// bit 2 is e0, bit 1 is e2, bit 0 is e1; the lane's bits 1, 2, 3 are e0, e1, e2.
+__device__ __forceinline__ uint32_t swap_codes(uint32_t w, uint32_t lane, uint32_t lane_bit, uint32_t shift,
+                                               uint32_t low) {
+    const uint32_t o = __shfl_xor_sync(0xffffffffu, w, lane_bit);
+    return lane & lane_bit ? (w & ~low) | (o >> shift & low) : (w & low) | (o & low) << shift;
+}
+__device__ __forceinline__ uint32_t transpose_codes(uint32_t w, uint32_t lane) {
+    w = swap_codes(w, lane, 2, 16, 0x0000ffffu);
+    w = swap_codes(w, lane, 8, 8, 0x00ff00ffu);
+    return swap_codes(w, lane, 4, 4, 0x0f0f0f0fu);
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+__device__ __forceinline__ void word_set(uint4& v, int i, uint32_t w) {
+    if (i == 0) v.x = w;
+    if (i == 1) v.y = w;
+    if (i == 2) v.z = w;
+    if (i == 3) v.w = w;
+}
+
+// Face (k face f of block kb, column tile n16) in a stream of ct tile columns.
+__device__ __forceinline__ uint64_t face_offset(uint32_t kb, uint32_t f, uint32_t n16, uint32_t ct) {
+    const uint32_t kt = kb * 4u + f / 2u;
+    return ((uint64_t)kt * ct + n16 / 2u) * 1024u + ((f % 2u) * 2u + n16 % 2u) * 256u;
+}
+
+// w / s: the product with the reciprocal, corrected once by its residual
+// (Newton's iteration for a quotient).  Where the quotient is k + 1/2, which
+// decides the rounding, it is representable and comes out exact; anywhere else
+// two bf16 values' quotient is at least 2^-12 away from k + 1/2.
+__device__ __forceinline__ float quotient(float w, float s, float inv) {
+    const float t = w * inv;
+    return fmaf(fmaf(-t, s, w), inv, t);
+}
+
+// A column's scale (its bits), the scale's reciprocal and the zero point from
+// the largest value and the largest magnitude below zero (bf16 bits).
+struct Column {
+    uint32_t s_bits, zero;
+    float s, inv;
+};
+template <bool ZEROS>
+__device__ __forceinline__ Column column_of(uint32_t hi, uint32_t lo) {
+    Column c;
+    const bool bad = max(hi, lo) >= 0x7f80u;  // an infinity or NaN among them
+    const float fh = bf16_bits_to_f32(hi), fl = bf16_bits_to_f32(lo);
+    c.s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(ZEROS ? (fh + fl) / 15.0f : fmaxf(fh, fl) / 7.0f);
+    c.s = bf16_bits_to_f32(c.s_bits);
+    c.zero = 8;
+    if (!(c.s > 0.0f) || !isfinite(c.s)) {
+        c.s = 0.0f, c.inv = 0.0f;  // every code is the zero point
+        return c;
     }
-    float s = w.zeros ? (hi - lo) / 15.0f : fmaxf(hi, -lo) / 7.0f;
-    const uint32_t s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(s);
-    s = bf16_bits_to_f32(s_bits);
-    const bool ok = s > 0.0f && isfinite(s);
-    const float z = !w.zeros || !ok ? 8.0f : fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f);
-    for (uint32_t k = k0; k < k0 + w.group; k += 8) {
-        uint32_t word = 0;
-        for (uint32_t j = 0; j < 8; ++j) {
-            float q = z;
-            if (ok && k + j < w.K && n < w.N) {
-                q = rintf(bf16_bits_to_f32(tiles[tile_index(k + j, n, ct)]) / s) + z;
-                q = fminf(fmaxf(q, 0.0f), 15.0f);
-            }
-            word |= (uint32_t)q << nibble_shift(j);
+    c.inv = 1.0f / c.s;
+    if (ZEROS) c.zero = (uint32_t)fminf(fmaxf(rintf(fl / c.s), 0.0f), 15.0f);
+    return c;
+}
+
+template <int GROUP, bool ZEROS>
+__global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restrict__ tiles, uint8_t* __restrict__ packed,
+                                                       Weights w, uint32_t kb_count, uint64_t blocks) {
+    constexpr int kGroups = 128 / GROUP, kFaces = GROUP / 16;  // of a block, of a group
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    const uint32_t lane = threadIdx.x % 32u, nt = (w.N + 15u) / 16u, ct = w.N / 32u;
+    const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 32u);
+    for (uint64_t b = (uint64_t)blockIdx.x * (blockDim.x / 32u) + threadIdx.x / 32u; b < blocks; b += step) {
+        const uint32_t kb = (uint32_t)(b / nt), n16 = (uint32_t)(b % nt);
+        uint4 x[8];
+#pragma unroll
+        for (int f = 0; f < 8; ++f) {
+            x[f] = make_uint4(0, 0, 0, 0);
+            if (kb * 128u + f * 16u < w.K)
+                x[f] = __ldcs(reinterpret_cast<const uint4*>(tiles + face_offset(kb, f, n16, ct)) + lane);
         }
-        *reinterpret_cast<uint32_t*>(packed + word_offset(n, k, kb, bytes)) = word;
+        uint8_t* const block = packed + ((uint64_t)n16 * kb_count + kb) * block_bytes(GROUP, ZEROS);
+        uint4 out[2];  // words of k = 32 i + 8 (lane / 16), and 16 more
+#pragma unroll
+        for (int gi = 0; gi < kGroups; ++gi) {
+            // Largest value (or magnitude) of each column, two columns a word:
+            // magnitudes' bits order like integers.
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                hi[i] = lo[i] = 0;
+#pragma unroll
+                for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) {
+                    const uint32_t v = word_of(x[f], i), mag = v & 0x7fff7fffu;
+                    if constexpr (ZEROS) {
+                        const uint32_t neg = (v >> 15 & 0x00010001u) * 0xffffu;  // halves that are negative
+                        hi[i] = __vmaxu2(hi[i], mag & ~neg);
+                        lo[i] = __vmaxu2(lo[i], mag & neg);
+                    } else {
+                        hi[i] = __vmaxu2(hi[i], mag);
+                    }
+                }
+#pragma unroll
+                for (int o = 2; o < 32; o <<= 1) {
+                    hi[i] = __vmaxu2(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+                    if constexpr (ZEROS) lo[i] = __vmaxu2(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+                }
+            }
+            // Lane l makes column 8 (l % 2) + l / 2 % 8, then all lanes ask for theirs.
+            const uint32_t e = lane / 2u % 8u;
+            const uint32_t eh = e < 4u ? (e < 2u ? hi[0] : hi[1]) : (e < 6u ? hi[2] : hi[3]);
+            const uint32_t el = e < 4u ? (e < 2u ? lo[0] : lo[1]) : (e < 6u ? lo[2] : lo[3]);
+            const Column c = column_of<ZEROS>(e % 2u ? eh >> 16 : eh & 0xffffu, e % 2u ? el >> 16 : el & 0xffffu);
+            if (lane < 16u) {
+                const uint32_t n = lane % 2u * 8u + e;
+                reinterpret_cast<uint16_t*>(block + kCodeBytes)[gi * 16 + n] = (uint16_t)c.s_bits;
+                if constexpr (ZEROS) block[kCodeBytes + 32 * kGroups + gi * 16 + n] = (uint8_t)c.zero;
+            }
+            float s[8], inv[8];
+            uint32_t zero[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int from = (int)(lane % 2u) + 2 * j;
+                s[j] = __shfl_sync(0xffffffffu, c.s, from);
+                inv[j] = __shfl_sync(0xffffffffu, c.inv, from);
+                zero[j] = ZEROS ? __shfl_sync(0xffffffffu, c.zero, from) : 8u;
+            }
+            const bool tiny = __any_sync(0xffffffffu, !isfinite(c.inv));  // a reciprocal overflows: divide
+#pragma unroll
+            for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t v = word_of(x[f], j / 2);
+                    const float wf = j % 2 ? __uint_as_float(v & 0xffff0000u) : bf16_bits_to_f32(v & 0xffffu);
+                    float t = quotient(wf, s[j], inv[j]);
+                    if (tiny) t = s[j] > 0.0f ? wf / s[j] : 0.0f;
+                    if (inv[j] == 0.0f) t = 0.0f;
+                    // To an integer, ties to even: 1.5 * 2^23 leaves no fraction bits.
+                    uint32_t code;
+                    if constexpr (ZEROS) {
+                        const int q = (int)(__float_as_uint(t + 12582912.0f) & 0x3fu) << 26 >> 26;
+                        code = (uint32_t)min(max(q + (int)zero[j], 0), 15);
+                    } else {
+                        code = __float_as_uint(t + 12582920.0f) & 15u;  // |t| < 7.04: no need to clamp
+                    }
+                    word |= code << (4 * (j / 2 + 4 * (j % 2)));
+                }
+                word_set(out[f % 2], f / 2, transpose_codes(word, lane));
+            }
+        }
+        // Lane l holds column 8 (l % 2) + l / 2 % 8.
+        uint4* const dst = reinterpret_cast<uint4*>(block) + (lane % 2u * 8u + lane / 2u % 8u) * 4u + lane / 16u;
+        dst[0] = out[0];
+        dst[2] = out[1];
     }
-    *reinterpret_cast<uint16_t*>(packed + scale_offset(n, k0, kb, bytes, w.group)) = (uint16_t)s_bits;
-    if (w.zeros) packed[zero_offset(n, k0, kb, bytes, w.group)] = (uint8_t)z;
 }
 
-__device__ __forceinline__ float weight(const uint8_t* packed, uint32_t n, uint32_t k, const Weights& w, uint32_t kb,
-                                        uint32_t bytes) {
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(packed + word_offset(n, k / 8u * 8u, kb, bytes));
-    const int q = (int)((word >> nibble_shift(k % 8u)) & 15u);
-    const int z = w.zeros ? packed[zero_offset(n, k, kb, bytes, w.group)] : 8;
-    return bf16_bits_to_f32(*reinterpret_cast<const uint16_t*>(packed + scale_offset(n, k, kb, bytes, w.group))) *
-           (float)(q - z);
+// Two weights of a word of codes: (q - z) s in bf16, (16 + q) - (16 + z) exact
+// and the product rounded once.
+template <int I>
+__device__ __forceinline__ uint32_t weights2(uint32_t w, uint32_t z16, uint32_t s) {
+    const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
+    uint32_t r;
+    asm("{\n\t.reg .b32 t;\n\t"
+        "lop3.b32 t, %1, 0x00780078, %2, 0xea;\n\t"
+        "sub.rn.bf16x2 t, t, %3;\n\t"
+        "mul.rn.bf16x2 %0, t, %4;\n\t}"
+        : "=r"(r)
+        : "r"(v), "r"(0x41804180u), "r"(z16), "r"(s));
+    return r;
+}
+// 16 + z in bf16 for both halves' zero points.
+__device__ __forceinline__ uint32_t sixteen(uint32_t z0, uint32_t z1) {
+    return 0x41804180u | (z0 & 15u) << 3 | (z1 & 15u) << 19;
 }
 
-// One thread for each element of the tile stream.
-__global__ void dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* __restrict__ tiles, Weights w,
-                                  uint32_t kb, uint32_t transpose, uint64_t total) {
-    const uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= total) return;
-    const uint32_t ct = ((transpose ? w.K : w.N) + 31u) / 32u;
-    const uint64_t tile = i / 1024u;
-    const uint32_t e = (uint32_t)(i % 1024u), face = e / 256u;
-    const uint32_t r = (uint32_t)(tile / ct) * 32u + face / 2u * 16u + e % 256u / 16u;
-    const uint32_t c = (uint32_t)(tile % ct) * 32u + face % 2u * 16u + e % 16u;
-    const uint32_t k = transpose ? c : r, n = transpose ? r : c;
-    uint32_t bits = 0;
-    if (k < w.K && n < w.N)
-        bits = cvt_bf16x2(weight(packed, n, k, w, kb, block_bytes(w.group, w.zeros)), 0.0f) & 0xffffu;
-    tiles[i] = (uint16_t)bits;
+template <int GROUP, bool ZEROS, bool TRANSPOSE>
+__global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restrict__ packed, uint16_t* __restrict__ tiles,
+                                                         Weights w, uint32_t kb_count, uint64_t blocks) {
+    constexpr int kGroups = 128 / GROUP, kFaces = GROUP / 16;
+    griddep_wait();  // launched with programmatic stream serialization
+    griddep_launch_dependents();
+    const uint32_t lane = threadIdx.x % 32u;
+    // Tile columns of the output; 16-column blocks up to whole tiles (the one
+    // past N, if any, is zeros).
+    const uint32_t nt = (w.N + 31u) / 32u * 2u, stored = (w.N + 15u) / 16u;
+    const uint32_t kt = (w.K + 31u) / 32u, ct = TRANSPOSE ? kt : nt / 2u;
+    const uint64_t step = (uint64_t)gridDim.x * (blockDim.x / 32u);
+    for (uint64_t b = (uint64_t)blockIdx.x * (blockDim.x / 32u) + threadIdx.x / 32u; b < blocks; b += step) {
+        const uint32_t kb = (uint32_t)(TRANSPOSE ? b % kb_count : b / nt), n16 = (uint32_t)(TRANSPOSE ? b / kb_count : b % nt);
+        const uint8_t* const block = packed + ((uint64_t)n16 * kb_count + kb) * block_bytes(GROUP, ZEROS);
+        // The column whose words this lane reads, and those it writes.
+        const uint32_t row = TRANSPOSE ? lane / 2u : lane % 2u * 8u + lane / 2u % 8u;
+        const uint32_t half = TRANSPOSE ? lane % 2u : lane / 16u;
+        uint4 in[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        const bool there = n16 < stored;
+        if (there) {
+            const uint4* src = reinterpret_cast<const uint4*>(block) + row * 4u + half;
+            in[0] = __ldcs(src), in[1] = __ldcs(src + 2);
+        }
+#pragma unroll
+        for (int gi = 0; gi < kGroups; ++gi) {
+            uint32_t s[4] = {0, 0, 0, 0}, z[4] = {0x41c041c0u, 0x41c041c0u, 0x41c041c0u, 0x41c041c0u};
+            if (there) {
+                const uint8_t* scales = block + kCodeBytes + gi * 32;
+                const uint8_t* zeros = block + kCodeBytes + 32 * kGroups + gi * 16;
+                if constexpr (TRANSPOSE) {
+                    const uint32_t one = reinterpret_cast<const uint16_t*>(scales)[row];
+                    s[0] = s[1] = s[2] = s[3] = one * 0x00010001u;
+                    if constexpr (ZEROS) z[0] = z[1] = z[2] = z[3] = sixteen(zeros[row], zeros[row]);
+                } else {
+                    const uint4 v = reinterpret_cast<const uint4*>(scales)[lane % 2u];
+                    s[0] = v.x, s[1] = v.y, s[2] = v.z, s[3] = v.w;
+                    if constexpr (ZEROS) {
+                        const uint2 q = reinterpret_cast<const uint2*>(zeros)[lane % 2u];
+                        z[0] = sixteen(q.x, q.x >> 8), z[1] = sixteen(q.x >> 16, q.x >> 24);
+                        z[2] = sixteen(q.y, q.y >> 8), z[3] = sixteen(q.y >> 16, q.y >> 24);
+                    }
+                }
+            }
+#pragma unroll
+            for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) {
+                uint32_t word = word_of(in[f % 2], f / 2);
+                if constexpr (!TRANSPOSE) word = transpose_codes(word, lane);
+                uint4 v = make_uint4(weights2<0>(word, z[0], s[0]), weights2<1>(word, z[1], s[1]),
+                                     weights2<2>(word, z[2], s[2]), weights2<3>(word, z[3], s[3]));
+                const uint32_t k0 = kb * 128u + f * 16u;
+                if (k0 / 32u >= kt) continue;
+                // Zeros past K and N.
+                const uint32_t r = TRANSPOSE ? n16 * 16u + lane / 2u : k0 + lane / 2u;
+                const uint32_t c = (TRANSPOSE ? k0 : n16 * 16u) + lane % 2u * 8u;
+                const uint32_t rows = TRANSPOSE ? w.N : w.K, cols = TRANSPOSE ? w.K : w.N;
+                if (r >= rows || c >= cols) {
+                    v = make_uint4(0, 0, 0, 0);
+                } else if (c + 8u > cols) {
+                    const uint32_t n = cols - c;  // values of this lane that count, 1 to 7
+                    v.x = n > 1u ? v.x : v.x & 0xffffu;
+                    v.y = n > 3u ? v.y : n > 2u ? v.y & 0xffffu : 0u;
+                    v.z = n > 5u ? v.z : n > 4u ? v.z & 0xffffu : 0u;
+                    v.w = n > 6u ? v.w & 0xffffu : 0u;
+                }
+                const uint64_t face = TRANSPOSE ? ((uint64_t)(n16 / 2u) * ct + k0 / 32u) * 1024u +
+                                                      ((n16 % 2u) * 2u + k0 / 16u % 2u) * 256u
+                                                : face_offset(kb, f, n16, ct);
+                __stcs(reinterpret_cast<uint4*>(tiles + face) + lane, v);
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------ matvec ---
@@ -178,9 +365,6 @@ __device__ __forceinline__ uint32_t codes16(uint32_t w) {
     uint32_t r;  // (v & mask) | magic in one instruction
     asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(0x00780078u), "r"(0x41804180u));
     return r;
-}
-__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
-    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
@@ -456,17 +640,51 @@ cudaError_t pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* ze
     return count(cudaGetLastError());
 }
 
-cudaError_t quantize_tiles(const uint16_t* tiles, uint8_t* packed, const Weights& w, cudaStream_t s) {
-    const uint64_t groups = (uint64_t)padded_n(w) * blocks_k(w) * (128u / w.group);
-    quantize_kernel<<<ctas(groups), 256, 0, s>>>(tiles, packed, w, blocks_k(w), groups);
-    return count(cudaGetLastError());
+// One warp a block, 8 a CTA, at most `most` CTAs an SM.
+template <class K, class... Args>
+static cudaError_t launch_blocks(K kernel, uint64_t blocks, cudaStream_t s, Args... args) {
+    const uint64_t ctas = (blocks + 7) / 8, most = (uint64_t)foil_sm_count() * 8;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(ctas < most ? ctas : most), 1, 1), cfg.blockDim = dim3(256, 1, 1), cfg.stream = s;
+    cudaLaunchAttribute la[1]{};
+    la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    la[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = la, cfg.numAttrs = 1;
+    return count(cudaLaunchKernelEx(&cfg, kernel, args..., blocks));
 }
 
-cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weights& w, bool transpose,
-                             cudaStream_t s) {
-    const uint64_t total = (uint64_t)((w.K + 31) / 32) * ((w.N + 31) / 32) * 1024u;
-    dequantize_kernel<<<ctas(total), 256, 0, s>>>(packed, tiles, w, blocks_k(w), transpose ? 1u : 0u, total);
-    return count(cudaGetLastError());
+template <int GROUP, bool ZEROS>
+static cudaError_t quantize_typed(const uint16_t* tiles, uint8_t* packed, const Weights& w, cudaStream_t s) {
+    const uint64_t blocks = (uint64_t)padded_n(w) / 16 * blocks_k(w);
+    return launch_blocks(quantize_kernel<GROUP, ZEROS>, blocks, s, tiles, packed, w, blocks_k(w));
+}
+
+cudaError_t quantize_tiles(const uint16_t* tiles, uint8_t* packed, const Weights& w, cudaStream_t s) {
+    if (w.group == 32)
+        return w.zeros ? quantize_typed<32, true>(tiles, packed, w, s) : quantize_typed<32, false>(tiles, packed, w, s);
+    if (w.group == 64)
+        return w.zeros ? quantize_typed<64, true>(tiles, packed, w, s) : quantize_typed<64, false>(tiles, packed, w, s);
+    return w.zeros ? quantize_typed<128, true>(tiles, packed, w, s) : quantize_typed<128, false>(tiles, packed, w, s);
+}
+
+template <int GROUP, bool ZEROS>
+static cudaError_t dequantize_typed(const uint8_t* packed, uint16_t* tiles, const Weights& w, bool transpose,
+                                    cudaStream_t s) {
+    const uint64_t blocks = (uint64_t)((w.N + 31) / 32) * 2 * blocks_k(w);
+    return transpose
+               ? launch_blocks(dequantize_kernel<GROUP, ZEROS, true>, blocks, s, packed, tiles, w, blocks_k(w))
+               : launch_blocks(dequantize_kernel<GROUP, ZEROS, false>, blocks, s, packed, tiles, w, blocks_k(w));
+}
+
+cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weights& w, bool transpose, cudaStream_t s) {
+    if (w.group == 32)
+        return w.zeros ? dequantize_typed<32, true>(packed, tiles, w, transpose, s)
+                       : dequantize_typed<32, false>(packed, tiles, w, transpose, s);
+    if (w.group == 64)
+        return w.zeros ? dequantize_typed<64, true>(packed, tiles, w, transpose, s)
+                       : dequantize_typed<64, false>(packed, tiles, w, transpose, s);
+    return w.zeros ? dequantize_typed<128, true>(packed, tiles, w, transpose, s)
+                   : dequantize_typed<128, false>(packed, tiles, w, transpose, s);
 }
 
 // The split of K over the CTAs of a cluster (S) and the warps of a CTA (WK):
