@@ -50,23 +50,6 @@ struct Raw {
     }
 };
 
-// Two channels at a time: sm_100a multiplies and adds fp32 pairs in one
-// instruction, and these kernels are near the issue limit.
-__device__ __forceinline__ uint64_t bits(float2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
-__device__ __forceinline__ float2 pair_of(uint64_t b) {
-    return make_float2(__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32)));
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    uint64_t d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
-    return pair_of(d);
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    uint64_t d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
-    return pair_of(d);
-}
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float sum2(float2 v) { return v.x + v.y; }
 
 // Channels 2 i and 2 i + 1 of a thread's.

@@ -55,6 +55,29 @@ __device__ __forceinline__ uint32_t pack_bf16x2(uint32_t lo, uint32_t hi) {
     return (lo & 0xffffu) | (hi << 16);
 }
 
+// Two fp32 values at a time: sm_100a multiplies and adds pairs in one
+// instruction, for kernels near the issue limit.
+__device__ __forceinline__ uint64_t bits(float2 v) { return (uint64_t)__float_as_uint(v.y) << 32 | __float_as_uint(v.x); }
+__device__ __forceinline__ float2 pair_of(uint64_t b) {
+    return make_float2(__uint_as_float((uint32_t)b), __uint_as_float((uint32_t)(b >> 32)));
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)), "l"(bits(c)));
+    return pair_of(d);
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+    return pair_of(d);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(bits(a)), "l"(bits(b)));
+    return pair_of(d);
+}
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
 // Device-side error codes written to the error word.
 enum : uint32_t {
     kErrWaitTimeout = 1u,  // a bounded mbarrier wait gave up

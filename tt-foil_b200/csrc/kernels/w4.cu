@@ -3,6 +3,8 @@
 // foil_w4_pack_dev in include/foil_c.h.
 #include "w4.cuh"
 
+#include <type_traits>
+
 #include "gemm_ptx.cuh"
 
 namespace foil {
@@ -93,9 +95,9 @@ __device__ __forceinline__ uint64_t face_offset(uint32_t kb, uint32_t f, uint32_
 // (Newton's iteration for a quotient).  Where the quotient is k + 1/2, which
 // decides the rounding, it is representable and comes out exact; anywhere else
 // two bf16 values' quotient is at least 2^-12 away from k + 1/2.
-__device__ __forceinline__ float quotient(float w, float s, float inv) {
-    const float t = w * inv;
-    return fmaf(fmaf(-t, s, w), inv, t);
+__device__ __forceinline__ float2 quotient(float2 w, float2 s, float2 inv) {
+    const float2 t = mul2(w, inv);
+    return fma2(fma2(make_float2(-t.x, -t.y), s, w), inv, t);
 }
 
 // A column's scale (its bits), the scale's reciprocal and the zero point from
@@ -175,37 +177,45 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
                 reinterpret_cast<uint16_t*>(block + kCodeBytes)[gi * 16 + n] = (uint16_t)c.s_bits;
                 if constexpr (ZEROS) block[kCodeBytes + 32 * kGroups + gi * 16 + n] = (uint8_t)c.zero;
             }
-            float s[8], inv[8];
-            uint32_t zero[8];
+            float2 s[4], inv[4], zero[ZEROS ? 4 : 1];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int from = (int)(lane % 2u) + 2 * j;
-                s[j] = __shfl_sync(0xffffffffu, c.s, from);
-                inv[j] = __shfl_sync(0xffffffffu, c.inv, from);
-                zero[j] = ZEROS ? __shfl_sync(0xffffffffu, c.zero, from) : 8u;
+            for (int j = 0; j < 4; ++j) {
+                const int from = (int)(lane % 2u) + 4 * j;
+                s[j] = make_float2(__shfl_sync(0xffffffffu, c.s, from), __shfl_sync(0xffffffffu, c.s, from + 2));
+                inv[j] = make_float2(__shfl_sync(0xffffffffu, c.inv, from), __shfl_sync(0xffffffffu, c.inv, from + 2));
+                if constexpr (ZEROS)
+                    zero[j] = make_float2((float)__shfl_sync(0xffffffffu, c.zero, from),
+                                          (float)__shfl_sync(0xffffffffu, c.zero, from + 2));
             }
-            const bool tiny = __any_sync(0xffffffffu, !isfinite(c.inv));  // a reciprocal overflows: divide
-#pragma unroll
-            for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) {
+            auto face_codes = [&](int f, auto divide) {
                 uint32_t word = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t v = word_of(x[f], j / 2);
-                    const float wf = j % 2 ? __uint_as_float(v & 0xffff0000u) : bf16_bits_to_f32(v & 0xffffu);
-                    float t = quotient(wf, s[j], inv[j]);
-                    if (tiny) t = s[j] > 0.0f ? wf / s[j] : 0.0f;
-                    if (inv[j] == 0.0f) t = 0.0f;
-                    // To an integer, ties to even: 1.5 * 2^23 leaves no fraction bits.
-                    uint32_t code;
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t v = word_of(x[f], j);
+                    const float2 wf = make_float2(bf16_bits_to_f32(v & 0xffffu), __uint_as_float(v & 0xffff0000u));
+                    float2 t = quotient(wf, s[j], inv[j]);
+                    if constexpr (decltype(divide)::value)
+                        t = make_float2(s[j].x > 0.0f ? wf.x / s[j].x : 0.0f, s[j].y > 0.0f ? wf.y / s[j].y : 0.0f);
+                    // To integers, ties to even: 1.5 * 2^23 leaves no fraction bits.
+                    const float2 kRound = both(12582912.0f);
                     if constexpr (ZEROS) {
-                        const int q = (int)(__float_as_uint(t + 12582912.0f) & 0x3fu) << 26 >> 26;
-                        code = (uint32_t)min(max(q + (int)zero[j], 0), 15);
+                        t = add2(add2(add2(t, kRound), both(-12582912.0f)), zero[j]);
+                        t = make_float2(fminf(fmaxf(t.x, 0.0f), 15.0f), fminf(fmaxf(t.y, 0.0f), 15.0f));
+                        t = add2(t, kRound);
                     } else {
-                        code = __float_as_uint(t + 12582920.0f) & 15u;  // |t| < 7.04: no need to clamp
+                        t = add2(t, both(12582920.0f));  // + 8; |t| < 7.04, no need to clamp
                     }
-                    word |= code << (4 * (j / 2 + 4 * (j % 2)));
+                    const uint32_t codes = __byte_perm(__float_as_uint(t.x), __float_as_uint(t.y), 0x5410);
+                    word |= (codes & 0x000f000fu) << (4 * j);
                 }
                 word_set(out[f % 2], f / 2, transpose_codes(word, lane));
+            };
+            if (__any_sync(0xffffffffu, !isfinite(c.inv))) {  // a reciprocal overflows: divide
+#pragma unroll
+                for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) face_codes(f, std::true_type());
+            } else {
+#pragma unroll
+                for (int f = gi * kFaces; f < (gi + 1) * kFaces; ++f) face_codes(f, std::false_type());
             }
         }
         // Lane l holds column 8 (l % 2) + l / 2 % 8.
