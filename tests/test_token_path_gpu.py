@@ -174,6 +174,30 @@ def test_matvec_non_finite_rows_stay_apart():
     assert torch.isnan(y1[1]).all() and not torch.isfinite(y1[3]).any()
 
 
+@pytest.mark.parametrize("M,K,group,zeros", [(8, 300, 64, True), (13, 4200, 128, False), (16, 20000, 32, True)])
+def test_matvec_rows_of_very_different_size(M, K, group, zeros):
+    """Rows scaled by powers of two from 2^-118 to 2^100: each within its own bound,
+    and the ordinary rows' bits do not depend on their neighbours."""
+    g = gen(K)
+    N = 70
+    codes, scales, zp = make_weights(g, K, N, group, zeros)
+    w = real_weights(codes, scales, zp, group)
+    x = randn(g, M, K)
+    packed = pack(codes, scales, zp, group)
+    plain = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(x.cuda(), packed, plain, M, K, N, group, zeros=zeros)
+    powers = [0, 40, -80, 100, -118, 0, 23, -66] * 2
+    scale = torch.tensor([2.0 ** p for p in powers[:M]], dtype=F64)[:, None]
+    xs = (x.to(F64) * scale).to(BF)
+    xs[5] = 0
+    y = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(xs.cuda(), packed, y, M, K, N, group, zeros=zeros)
+    # a power of two changes nothing but exponents: the rows' errors scale with them
+    close((y.cpu().to(F64) / scale), (xs.to(F64) / scale) @ w.t(),
+          matvec_slack(xs.to(F64) / scale, codes, scales, zp, group, w), BF)
+    assert torch.equal(y[0].view(torch.int16), plain[0].view(torch.int16)) and (y[5] == 0).all()
+
+
 def test_matvec_repeats_bit_for_bit_and_rows_do_not_depend_on_their_company():
     g = gen(7)
     K, N, group = 4100, 1030, 32

@@ -328,14 +328,20 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 //    6 blocks (1056 to 1216 bytes each: codes, scales, zero points) ahead, no
 //    other warp involved.  (Bulk copies of one block each, measured: 80 to 140 ns of an SM's copy
 //    engine apiece, 1.2 to 2 TB/s in all.)
-//  * mma.m16n8k16 with the weights as the 16-row operand: 16 + q is made in
-//    bf16 by one shift and one logical operation for two codes (0x4180 is 16,
-//    a code at bits 3..6 of its mantissa adds q, exact), laid out in storage
-//    so that a lane's 16-byte words are its operand registers.  x is the other
-//    operand, one 16-byte shared-memory read for two MMAs.
-//  * The group's scale and zero point come after the MMAs in fp32:
-//    s * (sum (16 + q) x - (16 + z) sum x), sum x of each group made once when
-//    x is staged.  Nothing is rounded to fewer than 32 bits before the output.
+//  * mma.m16n8k16 with the weights as the 16-row operand.  bf16 bits 0 to 255
+//    (subnormal numbers and the first binade) stand for 0 to 255 times 2^-133,
+//    so a code needs no conversion: five integer operations make the operands
+//    of a word's eight codes, four masks and one shift, every second pair 16
+//    times too large.  x is the other operand, one 16-byte shared-memory read
+//    for two MMAs, in bf16 times 2^100, and 2^96 against the pairs that are too
+//    large: exact, and the products, q x 2^-33, are ordinary fp32 numbers.
+//    Rows of x whose largest value is not between 2^-69 and 2^21 get a power of
+//    two of their own.  (With 16 + q made in bf16 by a shift and a logical
+//    operation for two codes, eight operations a word, the integer pipe was the
+//    limit: 11.5 us for 16384 x 4096, one row.)
+//  * The accumulators start from minus z sum(x), made once for each group when
+//    x is staged, and end as sum((q - z) x); the group's scale follows in fp32.
+//    Nothing is rounded to fewer than 32 bits before the output.
 //  * K is split over the CTAs of a cluster (S) where x would not fit one SM's
 //    shared memory, and over the warps of a CTA (WK) where there are few
 //    columns; the parts are added in a fixed order through (distributed)
@@ -363,29 +369,44 @@ struct Matvec {
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// Codes number I and I + 4 of a word as 16 + q in bf16.
+// Codes number I and I + 4 of a word in place: q (even I) or 16 q (odd I).
 template <int I>
-__device__ __forceinline__ uint32_t codes16(uint32_t w) {
-    const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
-    uint32_t r;  // (v & mask) | magic in one instruction
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(v), "r"(0x00780078u), "r"(0x41804180u));
-    return r;
+__device__ __forceinline__ uint32_t codes(uint32_t w) {
+    return (I < 2 ? w : w >> 8) & (I % 2 ? 0x00f000f0u : 0x000f000fu);
 }
 __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
                  : "memory");
 }
 
+// A row's powers of two: x is multiplied by up1 up2, its sums by down1 down2
+// (2^133 over the former); two factors each, as their product may not be a
+// number.
+struct RowScale {
+    float up1, up2, down1, down2;
+};
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// For a row whose largest exponent field is `field`: the largest value to 2^120.
+__device__ __forceinline__ RowScale row_scale(uint32_t field) {
+    const int up = 120 - max((int)field - 127, -126), down = 133 - up;  // -8 .. 246, -113 .. 141
+    const int u = min(up, 120), d = min(down, 120);
+    return RowScale{power(u), power(up - u), power(d), power(down - d)};
+}
+constexpr int kScale = 100;                                          // of ordinary rows
+constexpr uint32_t kTopLow = 127 - 69, kTopHigh = 127 + 20;          // exponent fields of their largest values
+
 // The x rows of this CTA's blocks into shared memory (zeros past M and K) and
-// the sum of each group of each row, times -24 (codes stand as 16 + q, and q - 8 is
-// wanted) where there are no zero points.
-template <int NT, int GROUP, bool ZEROS>
-__device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb) {
+// the sum of each group of each row, times -8 where there are no zero points,
+// in the units of the products.  OWN: scaled by each row's own powers, else by
+// 2^kScale, and the largest exponent field of each row is noted in `top`.
+template <int NT, int GROUP, bool ZEROS, bool OWN>
+__device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb,
+                                        uint32_t* top, const RowScale* own) {
     float* sums = reinterpret_cast<float*>(smem + p.off_sum);
     const uint32_t rows = min(p.M - m0, 8u * NT);
     const uint32_t per_row = nkb * 16u, total = rows * per_row;  // 16-byte pieces
@@ -407,17 +428,31 @@ __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t
                                pack_bf16x2(e[6], e[7]));
             }
         }
-        float s = 0.0f;
+        float up1 = power(kScale), up2 = 1.0f, s = 0.0f;
+        if (OWN && i < total) up1 = own[row].up1, up2 = own[row].up2;
+        uint32_t h[4], most = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const uint32_t w = word_of(v, j);
-            s += bf16_bits_to_f32(w & 0xffffu) + bf16_bits_to_f32(w >> 16);
+            float lo = bf16_bits_to_f32(w & 0xffffu) * up1, hi = __uint_as_float(w & 0xffff0000u) * up1;
+            if (OWN) lo *= up2, hi *= up2;
+            s += lo + hi;
+            if (j % 2) lo *= 0.0625f, hi *= 0.0625f;
+            h[j] = cvt_bf16x2(lo, hi);
+            if (!OWN) most = max(most, max(w & 0x7f800000u, w << 16 & 0x7f800000u));
         }
+        s *= power(-100);  // 2^-133 in two steps, with what follows
 #pragma unroll
         for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+        if (!OWN) {
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            if (i < total && c % 16u == 0u) atomicMax(&top[row], most >> 23);
+        }
         if (i < total) {
-            *reinterpret_cast<uint4*>(smem + row * p.x_pitch + c * 16u) = v;
-            if (c % (GROUP / 8) == 0) sums[c / (GROUP / 8) * (8u * NT) + row] = ZEROS ? s : -24.0f * s;
+            *reinterpret_cast<uint4*>(smem + row * p.x_pitch + c * 16u) = make_uint4(h[0], h[1], h[2], h[3]);
+            if (c % (GROUP / 8) == 0)
+                sums[c / (GROUP / 8) * (8u * NT) + row] = (ZEROS ? power(-33) : -8.0f * power(-33)) * s;
         }
     }
 }
@@ -436,9 +471,8 @@ __device__ __forceinline__ void put(const Matvec& p, uint32_t m0, uint32_t tile,
     }
 }
 
-// -(16 + z) for a zero point z, in the bits of a float: 16 + z is 16 with z at
-// bits 19..22 of the mantissa.
-__device__ __forceinline__ float minus16(uint32_t z) { return __uint_as_float(0xc1800000u | (z & 15u) << 19); }
+// -z for a zero point z.
+__device__ __forceinline__ float minus(uint32_t z) { return 8388608.0f - __uint_as_float(0x4b000000u | (z & 15u)); }
 
 template <int NT, int RT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_constant__ Matvec p) {
@@ -447,6 +481,8 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
     constexpr int kAhead = mv_ahead(RT);
     constexpr uint32_t kSlot = RT * kBytes, kPlace = 512 * RT * NT;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint32_t top[8 * NT];
+    __shared__ RowScale own[8 * NT];
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, g = lane / 4u, t = lane % 4u;
     const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = p.clusters;
     const uint32_t m0 = blockIdx.y * 8u * NT;
@@ -469,34 +505,45 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 
     // The warp's blocks in order, one commit group for a block of each tile of
     // the run (empty past the end).
-    uint32_t is_run = wn, is_block = 0;
-    const uint8_t* src = p.packed + (uint64_t)(t0 + RT * wn) * tile_bytes + (uint64_t)(kb0 + b0) * kBytes + lane * 16u;
+    const uint32_t my_runs = nb && wn < runs ? (runs - wn + WN - 1) / WN : 0u;
+    uint32_t left = my_runs * nb, in_run = nb, is_tile = t0 + RT * wn;
+    const uint8_t* src = p.packed + (uint64_t)is_tile * tile_bytes + (uint64_t)(kb0 + b0) * kBytes + lane * 16u;
     auto issue = [&](uint8_t* slot) {
-        if (is_run < runs && nb) {
+        if (left) {
             const uint32_t dst = smem_u32(slot) + lane * 16u;
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
-                if (r && t0 + RT * is_run + r >= t1) break;
-                const uint8_t* s = src + r * tile_bytes;
+                // Past the cluster's last tile: the one before once more, not used.
+                const uint8_t* s = r && is_tile + r < t1 ? src + r * tile_bytes : src;
                 cp_async16(dst + r * kBytes, s, 16);
                 cp_async16(dst + r * kBytes + 512u, s + 512, 16);
                 if (lane < (kBytes - kCodeBytes) / 16u)
                     cp_async16(dst + r * kBytes + kCodeBytes, s + kCodeBytes, 16);
             }
             src += kBytes;
-            if (++is_block == nb) is_block = 0, is_run += WN, src += RT * WN * tile_bytes - (uint64_t)nb * kBytes;
+            --left;
+            if (--in_run == 0) in_run = nb, is_tile += RT * WN, src += RT * WN * tile_bytes - (uint64_t)nb * kBytes;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) issue(ring + i * kSlot);
 
-    stage_x<NT, GROUP, ZEROS>(p, smem, m0, kb0, nkb);
-    if (p.S > 1)
-        cluster_sync();  // also: every CTA of the cluster runs before its memory is written
-    else
+    if (threadIdx.x < 8u * NT) top[threadIdx.x] = 0u;
+    __syncthreads();
+    stage_x<NT, GROUP, ZEROS, false>(p, smem, m0, kb0, nkb, top, own);
+    __syncthreads();
+    const uint32_t most = lane < 8u * NT ? top[lane] : 0u;
+    const bool unusual = __any_sync(0xffffffffu, most > kTopHigh || (most != 0u && most < kTopLow));
+    if (unusual) {
+        if (threadIdx.x < 8u * NT) own[threadIdx.x] = row_scale(top[threadIdx.x]);
         __syncthreads();
+        stage_x<NT, GROUP, ZEROS, true>(p, smem, m0, kb0, nkb, top, own);
+        __syncthreads();
+    }
+    if (p.S > 1) cluster_sync();  // every CTA of the cluster runs before its memory is written
 
+    const uint32_t x_rows = 8u * p.x_pitch;
     const uint8_t* const xrow = smem + g * p.x_pitch + t * 16u + b0 * 256u;
     const float* const sums =
         reinterpret_cast<const float*>(smem + p.off_sum) + b0 * kGroups * (8u * NT) + 2u * t;
@@ -526,11 +573,11 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                     float part[RT][NT][4];
 #pragma unroll
                     for (int r = 0; r < RT; ++r) {
-                        // Start from minus (16 + z) times the group's sum of x.
+                        // Start from minus z times the group's sum of x.
                         float z0 = 1.0f, z1 = 1.0f;
                         if constexpr (ZEROS) {
                             const uint8_t* zp = slot + r * kBytes + kCodeBytes + 32 * kGroups + gi * 16;
-                            z0 = minus16(zp[g]), z1 = minus16(zp[g + 8]);
+                            z0 = minus(zp[g]), z1 = minus(zp[g + 8]);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
@@ -544,15 +591,12 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                         uint4 xv[NT];
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            xv[n] = *reinterpret_cast<const uint4*>(xb + n * 8u * p.x_pitch + q * 64u);
+                            xv[n] = *reinterpret_cast<const uint4*>(xb + n * x_rows + q * 64u);
 #pragma unroll
                         for (int r = 0; r < RT; ++r) {
-                            if (r && r >= (int)n_tiles) break;
                             const uint32_t a = word_of(wa[r], q), c = word_of(wb[r], q);
-                            const uint32_t a0 = codes16<0>(a), a1 = codes16<1>(a), a2 = codes16<2>(a),
-                                           a3 = codes16<3>(a);
-                            const uint32_t c0 = codes16<0>(c), c1 = codes16<1>(c), c2 = codes16<2>(c),
-                                           c3 = codes16<3>(c);
+                            const uint32_t a0 = codes<0>(a), a1 = codes<1>(a), a2 = codes<2>(a), a3 = codes<3>(a);
+                            const uint32_t c0 = codes<0>(c), c1 = codes<1>(c), c2 = codes<2>(c), c3 = codes<3>(c);
 #pragma unroll
                             for (int n = 0; n < NT; ++n) {
                                 mma_bf16(part[r][n], a0, c0, a1, c1, xv[n].x, xv[n].y);
@@ -577,6 +621,21 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
                 issue(slot);
                 slot += kSlot;
                 if (slot == ring_end) slot = ring;
+            }
+            // Out of the products' units.
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                RowScale d0{0.0f, 0.0f, power(133 - kScale), 1.0f}, d1 = d0;
+                if (unusual) d0 = own[8 * n + 2 * t], d1 = own[8 * n + 2 * t + 1];
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    acc[r][n][0] *= d0.down1, acc[r][n][2] *= d0.down1;
+                    acc[r][n][1] *= d1.down1, acc[r][n][3] *= d1.down1;
+                    if (unusual) {
+                        acc[r][n][0] *= d0.down2, acc[r][n][2] *= d0.down2;
+                        acc[r][n][1] *= d1.down2, acc[r][n][3] *= d1.down2;
+                    }
+                }
             }
             if (!joined) {
 #pragma unroll
