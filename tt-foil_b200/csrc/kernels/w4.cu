@@ -364,7 +364,7 @@ struct Matvec {
     uint32_t M, K, N, kb, tiles;
     uint32_t S, WK, clusters, pass_runs;           // split (host)
     uint32_t x_pitch, off_sum, off_red, off_ring;  // shared-memory plan (host)
-    uint32_t relu, x_vec;
+    uint32_t relu, x_vec, x_log;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -408,51 +408,71 @@ template <int NT, int GROUP, bool ZEROS, bool OWN>
 __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb,
                                         uint32_t* top, const RowScale* own) {
     float* sums = reinterpret_cast<float*>(smem + p.off_sum);
-    const uint32_t rows = min(p.M - m0, 8u * NT);
-    const uint32_t per_row = nkb * 16u, total = rows * per_row;  // 16-byte pieces
+    const uint32_t rows = min(p.M - m0, 8u * NT), per_row = nkb * 16u;  // 16-byte pieces
     for (uint32_t i = rows * p.x_pitch + threadIdx.x * 16u; i < 8u * NT * p.x_pitch; i += kMvThreads * 16u)
         *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
-    for (uint32_t i0 = 0; i0 < total; i0 += kMvThreads) {
-        const uint32_t i = i0 + threadIdx.x, row = i / per_row, c = i - row * per_row;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        const uint32_t k = kb0 * kBlockK + c * 8u;
-        if (i < total && k < p.K) {
-            const uint16_t* src = p.x + (m0 + row) * p.ld_x + k;
-            if (p.x_vec && k + 8u <= p.K) {
-                v = *reinterpret_cast<const uint4*>(src);
-            } else {
-                uint32_t e[8];
+    // 2^x_log threads (16 and more) side by side on a row, kMvThreads / 2^x_log
+    // rows at a time; four pieces of a thread on their way.
+    const uint32_t side = 1u << p.x_log, c0 = threadIdx.x & (side - 1u), r0 = threadIdx.x >> p.x_log;
+    const uint32_t row_step = kMvThreads >> p.x_log, along = (per_row + side - 1u) >> p.x_log;
+    const uint32_t steps = (rows + row_step - 1u) / row_step * along;
+    constexpr uint32_t kBatch = 4;
+    uint32_t row = r0, c = c0;
+    for (uint32_t i0 = 0; i0 < steps; i0 += kBatch) {
+        uint4 v[kBatch];
+        uint32_t rows_of[kBatch], cs[kBatch];
 #pragma unroll
-                for (uint32_t j = 0; j < 8; ++j) e[j] = k + j < p.K ? src[j] : 0u;
-                v = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
-                               pack_bf16x2(e[6], e[7]));
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            v[b] = make_uint4(0, 0, 0, 0);
+            const bool in = i0 + b < steps && row < rows && c < per_row;
+            rows_of[b] = in ? row : ~0u, cs[b] = c;
+            const uint32_t k = kb0 * kBlockK + c * 8u;
+            if (in && k < p.K) {
+                const uint16_t* src = p.x + (m0 + row) * p.ld_x + k;
+                if (p.x_vec && k + 8u <= p.K) {
+                    v[b] = *reinterpret_cast<const uint4*>(src);
+                } else {
+                    uint32_t e[8];
+#pragma unroll
+                    for (uint32_t j = 0; j < 8; ++j) e[j] = k + j < p.K ? src[j] : 0u;
+                    v[b] = make_uint4(pack_bf16x2(e[0], e[1]), pack_bf16x2(e[2], e[3]), pack_bf16x2(e[4], e[5]),
+                                      pack_bf16x2(e[6], e[7]));
+                }
             }
+            c += side;
+            if (c >= along << p.x_log) c = c0, row += row_step;
         }
-        float up1 = power(kScale), up2 = 1.0f, s = 0.0f;
-        if (OWN && i < total) up1 = own[row].up1, up2 = own[row].up2;
-        uint32_t h[4], most = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t w = word_of(v, j);
-            float lo = bf16_bits_to_f32(w & 0xffffu) * up1, hi = __uint_as_float(w & 0xffff0000u) * up1;
-            if (OWN) lo *= up2, hi *= up2;
-            s += lo + hi;
-            if (j % 2) lo *= 0.0625f, hi *= 0.0625f;
-            h[j] = cvt_bf16x2(lo, hi);
-            if (!OWN) most = max(most, max(w & 0x7f800000u, w << 16 & 0x7f800000u));
-        }
-        s *= power(-100);  // 2^-133 in two steps, with what follows
+        for (uint32_t b = 0; b < kBatch; ++b) {
+            if (i0 + b >= steps) break;  // every thread
+            const bool in = rows_of[b] != ~0u;
+            float up1 = power(kScale), up2 = 1.0f, s = 0.0f;
+            if (OWN && in) up1 = own[rows_of[b]].up1, up2 = own[rows_of[b]].up2;
+            uint32_t h[4], most = 0;
 #pragma unroll
-        for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        if (!OWN) {
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = word_of(v[b], j);
+                float lo = bf16_bits_to_f32(w & 0xffffu) * up1, hi = __uint_as_float(w & 0xffff0000u) * up1;
+                if (OWN) lo *= up2, hi *= up2;
+                s += lo + hi;
+                if (j % 2) lo *= 0.0625f, hi *= 0.0625f;
+                h[j] = cvt_bf16x2(lo, hi);
+                if (!OWN) most = max(most, max(w & 0x7f800000u, w << 16 & 0x7f800000u));
+            }
+            s *= power(-100);  // 2^-133 in two steps, with what follows
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-            if (i < total && c % 16u == 0u) atomicMax(&top[row], most >> 23);
-        }
-        if (i < total) {
-            *reinterpret_cast<uint4*>(smem + row * p.x_pitch + c * 16u) = make_uint4(h[0], h[1], h[2], h[3]);
-            if (c % (GROUP / 8) == 0)
-                sums[c / (GROUP / 8) * (8u * NT) + row] = (ZEROS ? power(-33) : -8.0f * power(-33)) * s;
+            for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+            if (!OWN) {
+#pragma unroll
+                for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+                if (in && cs[b] % 16u == 0u) atomicMax(&top[rows_of[b]], most >> 23);
+            }
+            if (in) {
+                *reinterpret_cast<uint4*>(smem + rows_of[b] * p.x_pitch + cs[b] * 16u) =
+                    make_uint4(h[0], h[1], h[2], h[3]);
+                if (cs[b] % (GROUP / 8) == 0)
+                    sums[cs[b] / (GROUP / 8) * (8u * NT) + rows_of[b]] = (ZEROS ? power(-33) : -8.0f * power(-33)) * s;
+            }
         }
     }
 }
@@ -500,6 +520,8 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 
     uint8_t* const ring = smem + p.off_ring + warp * (kAhead * kSlot);
     uint8_t* const ring_end = ring + kAhead * kSlot;
+    if (threadIdx.x < 8u * NT) top[threadIdx.x] = 0u;
+    __syncthreads();
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
 
@@ -529,8 +551,6 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) issue(ring + i * kSlot);
 
-    if (threadIdx.x < 8u * NT) top[threadIdx.x] = 0u;
-    __syncthreads();
     stage_x<NT, GROUP, ZEROS, false>(p, smem, m0, kb0, nkb, top, own);
     __syncthreads();
     const uint32_t most = lane < 8u * NT ? top[lane] : 0u;
@@ -808,6 +828,8 @@ cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, cons
     // 16 rows at a time where there are more than 8 and their x fits, else 8.
     const uint32_t nt = M > 8 && plan_matvec(p, 2, bytes, w.group, sms) ? 2 : 1;
     if (nt == 1 && !plan_matvec(p, 1, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    for (p.x_log = 4; p.x_log < 9 && (1u << p.x_log) < (p.kb + p.S - 1) / p.S * 16; ++p.x_log) {
+    }
     const uint32_t rt = mv_tiles((int)nt), smem = p.off_ring + kMvWarps * mv_ahead((int)rt) * rt * bytes;
     const MatvecKernel kernel = nt == 2 ? pick_matvec<2>(w) : pick_matvec<1>(w);
     const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512);
