@@ -349,9 +349,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 //    grid is one CTA per SM, whatever N is.
 constexpr int kMvWarps = 16;
 constexpr int kMvThreads = 32 * kMvWarps;
-// Tiles of a warp at a time: two for up to 8 rows of x, one for up to 16 (the
-// accumulators of two would not fit the registers); and the slots in flight.
-__host__ __device__ constexpr int mv_tiles(int nt) { return nt == 1 ? 2 : 1; }
+// Blocks of each of a warp's tiles that are on their way.
 __host__ __device__ constexpr int mv_ahead(int rt) { return rt == 2 ? 3 : 4; }
 constexpr uint32_t kMaxSmem = 232448;
 
@@ -362,6 +360,7 @@ struct Matvec {
     uint16_t* y;
     uint64_t ld_x, ld_y;
     uint32_t M, K, N, kb, tiles;
+    uint32_t nt, rt;                               // rows of x / 8 and tiles that a warp takes at a time
     uint32_t S, WK, clusters, pass_runs;           // split (host)
     uint32_t x_pitch, off_sum, off_red, off_ring;  // shared-memory plan (host)
     uint32_t relu, x_vec, x_log;
@@ -382,6 +381,22 @@ __device__ __forceinline__ uint32_t codes(uint32_t w) {
 __device__ __forceinline__ void st_cluster_f4(uint32_t addr, float a, float b, float c, float d) {
     asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
                  : "memory");
+}
+
+// 16 bytes at an address that is a multiple of 2, out of the two aligned vectors
+// that hold them.  Up to 14 bytes before and after them are read too.
+__device__ __forceinline__ uint4 load_any(const uint16_t* p) {
+    const uint32_t off = (uint32_t)((uintptr_t)p & 15u);
+    const uint4* at = reinterpret_cast<const uint4*>((uintptr_t)p - off);
+    const uint4 a = at[0], b = off ? at[1] : make_uint4(0, 0, 0, 0);
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = off & 8u ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = off & 4u ? w[i + 1] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], off & 2u ? 16u : 0u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // A row's powers of two: x is multiplied by up1 up2, its sums by down1 down2
@@ -431,6 +446,8 @@ __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t
                 const uint16_t* src = p.x + (m0 + row) * p.ld_x + k;
                 if (p.x_vec && k + 8u <= p.K) {
                     v[b] = *reinterpret_cast<const uint4*>(src);
+                } else if (!p.x_vec && k >= 8u && k + 16u <= p.K) {
+                    v[b] = load_any(src);
                 } else {
                     uint32_t e[8];
 #pragma unroll
@@ -703,9 +720,8 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 }
 
 using MatvecKernel = void (*)(const Matvec);
-template <int NT>
+template <int NT, int RT>
 MatvecKernel pick_matvec(const Weights& w) {
-    constexpr int RT = mv_tiles(NT);
     if (w.group == 32) return w.zeros ? matvec_kernel<NT, RT, 32, true> : matvec_kernel<NT, RT, 32, false>;
     if (w.group == 64) return w.zeros ? matvec_kernel<NT, RT, 64, true> : matvec_kernel<NT, RT, 64, false>;
     return w.zeros ? matvec_kernel<NT, RT, 128, true> : matvec_kernel<NT, RT, 128, false>;
@@ -776,43 +792,52 @@ cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weigh
                    : dequantize_typed<128, false>(packed, tiles, w, transpose, s);
 }
 
-// The split of K over the CTAs of a cluster (S) and the warps of a CTA (WK):
-// the one whose busiest warp reads the fewest storage blocks, among those
-// whose slice of x fits.  A cluster barrier costs about as much as two blocks
-// a warp, the join of a CTA's warps about half a block.
-static bool plan_matvec(Matvec& p, uint32_t nt, uint32_t bytes, uint32_t group, uint32_t sms) {
-    const uint32_t width = 8 * nt, rt = mv_tiles((int)nt), ring = kMvWarps * mv_ahead((int)rt) * rt * bytes;
+// The rows of x (8 nt) and the tiles (rt) that a warp takes at a time, the
+// split of K over the CTAs of a cluster (S) and the warps of a CTA (WK): those
+// whose busiest warp has the least to do, where the slice of x fits.  The unit
+// is one block of a tile at the rate of two tiles and 8 rows; one tile at a
+// time costs 1.15 a block and 16 rows 1.3 (measured at 4096 x 65536).
+static bool plan_matvec(Matvec& p, uint32_t bytes, uint32_t group, uint32_t sms) {
     float best = 0.0f;
-    for (uint32_t S = 1; S <= 8; S *= 2) {
-        const uint32_t ks = (p.kb + S - 1) / S;
-        if (S > 1 && S > p.kb) break;
-        const uint32_t pitch = ks * 256 + 64;  // 64 bytes more: rows of an 8-lane read phase on distinct banks
-        const uint32_t off_sum = width * pitch, sums = ks * (128 / group) * width * 4;
-        const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
-        const uint32_t fit = (S == 1 ? sms : foil_resident_clusters(S)), clusters = fit < p.tiles ? fit : p.tiles;
-        const uint32_t tc = ((p.tiles + clusters - 1) / clusters + rt - 1) / rt;  // runs of rt tiles
-        for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
-            // A run's set-up and join cost about as much as one of its steps.
-            const uint32_t wn = kMvWarps / wk, units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk + 1);
-            const uint32_t place = S * wk * 512 * rt * nt;  // one run's parts
-            const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * place : 0;
-            if (off_red + min_red + ring > kMaxSmem - 1024) continue;
-            // What the ring leaves joins tiles.
-            uint32_t red = kMaxSmem - 1024 - off_red - ring, pass = tc;
-            if (S * wk > 1) {
-                const uint32_t cap = red / place * S;
-                if (cap < tc) pass = cap / wn * wn;
-                red = (pass + S - 1) / S * place;
-            } else {
-                red = 0;
+    for (uint32_t kind = 0; kind < 4; ++kind) {
+        const uint32_t nt = 1 + kind / 2, rt = 1 + kind % 2, width = 8 * nt;
+        if (nt == 2 && p.M <= 8) break;
+        const float step = (rt == 2 ? 2.0f : 1.15f) * (nt == 2 ? 1.3f : 1.0f);
+        const uint32_t ring = kMvWarps * mv_ahead((int)rt) * rt * bytes;
+        for (uint32_t S = 1; S <= 8 && S <= p.kb; S *= 2) {
+            const uint32_t ks = (p.kb + S - 1) / S;
+            const uint32_t pitch = ks * 256 + 64;  // 64 bytes more: rows of an 8-lane read phase on distinct banks
+            const uint32_t off_sum = width * pitch, sums = ks * (128 / group) * width * 4;
+            const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
+            const uint32_t fit = S == 1 ? sms : foil_resident_clusters(S), clusters = fit < p.tiles ? fit : p.tiles;
+            const uint32_t tc = ((p.tiles + clusters - 1) / clusters + rt - 1) / rt;  // runs of rt tiles
+            for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
+                // A run's set-up costs about as much as a block, its join as much
+                // again and a tenth for each part.
+                const uint32_t wn = kMvWarps / wk;
+                const float once = S * wk > 1 ? 2.0f + 0.1f * S * wk : 1.0f;
+                const float units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk * step + once);
+                const uint32_t place = S * wk * 512 * rt * nt;  // one run's parts
+                const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * place : 0;
+                if (off_red + min_red + ring > kMaxSmem - 1024) continue;
+                // What the ring leaves joins tiles.
+                uint32_t red = kMaxSmem - 1024 - off_red - ring, pass = tc;
+                if (S * wk > 1) {
+                    const uint32_t cap = red / place * S;
+                    if (cap < tc) pass = cap / wn * wn;
+                    red = (pass + S - 1) / S * place;
+                } else {
+                    red = 0;
+                }
+                const uint32_t passes = (tc + pass - 1) / pass;
+                const float cost = (units + passes * (S > 1 ? 4.0f : wk > 1 ? 1.0f : 0.0f)) * ((p.M + width - 1) / width);
+                if (best > 0.0f && cost >= best) continue;
+                best = cost;
+                p.nt = nt, p.rt = rt, p.S = S, p.WK = wk, p.clusters = clusters;
+                p.x_pitch = pitch, p.off_sum = off_sum, p.off_red = off_red;
+                p.off_ring = (off_red + red + 127) / 128 * 128;
+                p.pass_runs = pass < tc ? pass : (tc + wn - 1) / wn * wn;
             }
-            const uint32_t passes = (tc + pass - 1) / pass;
-            const float cost = units + passes * (S > 1 ? 2.0f : wk > 1 ? 0.5f : 0.0f);
-            if (best > 0.0f && cost >= best) continue;
-            best = cost;
-            p.S = S, p.WK = wk, p.clusters = clusters, p.x_pitch = pitch, p.off_sum = off_sum, p.off_red = off_red;
-            p.off_ring = (off_red + red + 127) / 128 * 128;
-            p.pass_runs = pass < tc ? pass : (tc + wn - 1) / wn * wn;
         }
     }
     return best > 0.0f;
@@ -825,17 +850,16 @@ cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, cons
     p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0;
     p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0;
     const uint32_t bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
-    // 16 rows at a time where there are more than 8 and their x fits, else 8.
-    const uint32_t nt = M > 8 && plan_matvec(p, 2, bytes, w.group, sms) ? 2 : 1;
-    if (nt == 1 && !plan_matvec(p, 1, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    if (!plan_matvec(p, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
     for (p.x_log = 4; p.x_log < 9 && (1u << p.x_log) < (p.kb + p.S - 1) / p.S * 16; ++p.x_log) {
     }
-    const uint32_t rt = mv_tiles((int)nt), smem = p.off_ring + kMvWarps * mv_ahead((int)rt) * rt * bytes;
-    const MatvecKernel kernel = nt == 2 ? pick_matvec<2>(w) : pick_matvec<1>(w);
+    const uint32_t smem = p.off_ring + kMvWarps * mv_ahead((int)p.rt) * p.rt * bytes;
+    const MatvecKernel kernel = p.nt == 2 ? (p.rt == 2 ? pick_matvec<2, 2>(w) : pick_matvec<2, 1>(w))
+                                          : (p.rt == 2 ? pick_matvec<1, 2>(w) : pick_matvec<1, 1>(w));
     const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)kMaxSmem - 512);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(p.clusters * p.S, (M + 8 * nt - 1) / (8 * nt), 1);
+    cfg.gridDim = dim3(p.clusters * p.S, (M + 8 * p.nt - 1) / (8 * p.nt), 1);
     cfg.blockDim = dim3(kMvThreads, 1, 1);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
