@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(256) dequantize_kernel(const uint8_t* __restri
 //    columns; the parts are added in a fixed order through (distributed)
 //    shared memory.  Clusters take contiguous, near-equal runs of tiles: the
 //    grid is one CTA per SM, whatever N is.
-constexpr int kMvWarps = 16;
+constexpr int kMvWarps = 16, kMvLog = 4;
 constexpr int kMvThreads = 32 * kMvWarps;
 // Blocks of each of a warp's tiles that are on their way.
 __host__ __device__ constexpr int mv_ahead(int rt) { return rt == 2 ? 3 : 4; }
@@ -362,6 +362,8 @@ struct Matvec {
     uint32_t M, K, N, kb, tiles;
     uint32_t nt, rt;                               // rows of x / 8 and tiles that a warp takes at a time
     uint32_t S, WK, clusters, pass_runs;           // split (host)
+    uint32_t S_log, WK_log;                        // both are powers of two
+    uint32_t kb_each, kb_more, tiles_each, tiles_more;  // shares of a CTA / cluster, and how many have one more
     uint32_t x_pitch, off_sum, off_red, off_ring;  // shared-memory plan (host)
     uint32_t relu, x_vec, x_log;
 };
@@ -417,7 +419,7 @@ constexpr uint32_t kTopLow = 127 - 69, kTopHigh = 127 + 20;          // exponent
 
 // The x rows of this CTA's blocks into shared memory (zeros past M and K) and
 // the sum of each group of each row, times -8 where there are no zero points,
-// in the units of the products.  OWN: scaled by each row's own powers, else by
+// in the units of the products (2^100 x 2^-133 = 2^-33).  OWN: scaled by each row's own powers, else by
 // 2^kScale, and the largest exponent field of each row is noted in `top`.
 template <int NT, int GROUP, bool ZEROS, bool OWN>
 __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t m0, uint32_t kb0, uint32_t nkb,
@@ -427,11 +429,11 @@ __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t
     for (uint32_t i = rows * p.x_pitch + threadIdx.x * 16u; i < 8u * NT * p.x_pitch; i += kMvThreads * 16u)
         *reinterpret_cast<uint4*>(smem + i) = make_uint4(0, 0, 0, 0);
     // 2^x_log threads (16 and more) side by side on a row, kMvThreads / 2^x_log
-    // rows at a time; four pieces of a thread on their way.
+    // rows at a time; eight pieces of a thread on their way.
     const uint32_t side = 1u << p.x_log, c0 = threadIdx.x & (side - 1u), r0 = threadIdx.x >> p.x_log;
     const uint32_t row_step = kMvThreads >> p.x_log, along = (per_row + side - 1u) >> p.x_log;
     const uint32_t steps = (rows + row_step - 1u) / row_step * along;
-    constexpr uint32_t kBatch = 4;
+    constexpr uint32_t kBatch = 8;
     uint32_t row = r0, c = c0;
     for (uint32_t i0 = 0; i0 < steps; i0 += kBatch) {
         uint4 v[kBatch];
@@ -463,27 +465,42 @@ __device__ __forceinline__ void stage_x(const Matvec& p, uint8_t* smem, uint32_t
         for (uint32_t b = 0; b < kBatch; ++b) {
             if (i0 + b >= steps) break;  // every thread
             const bool in = rows_of[b] != ~0u;
-            float up1 = power(kScale), up2 = 1.0f, s = 0.0f;
-            if (OWN && in) up1 = own[rows_of[b]].up1, up2 = own[rows_of[b]].up2;
-            uint32_t h[4], most = 0;
+            float s = 0.0f;
+            uint32_t h[4];
+            if constexpr (OWN) {
+                const float up1 = in ? own[rows_of[b]].up1 : 1.0f, up2 = in ? own[rows_of[b]].up2 : 1.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = word_of(v[b], j);
-                float lo = bf16_bits_to_f32(w & 0xffffu) * up1, hi = __uint_as_float(w & 0xffff0000u) * up1;
-                if (OWN) lo *= up2, hi *= up2;
-                s += lo + hi;
-                if (j % 2) lo *= 0.0625f, hi *= 0.0625f;
-                h[j] = cvt_bf16x2(lo, hi);
-                if (!OWN) most = max(most, max(w & 0x7f800000u, w << 16 & 0x7f800000u));
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = word_of(v[b], j);
+                    float lo = bf16_bits_to_f32(w & 0xffffu) * up1 * up2;
+                    float hi = __uint_as_float(w & 0xffff0000u) * up1 * up2;
+                    s += lo + hi;
+                    if (j % 2) lo *= 0.0625f, hi *= 0.0625f;
+                    h[j] = cvt_bf16x2(lo, hi);
+                }
+                s *= power(-100);  // 2^-133 in two steps, with what follows
+            } else {
+                uint32_t most = 0;
+                float2 sum = both(0.0f);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t w = word_of(v[b], j);
+                    // 2^100 or 2^96 times the pair, exact.
+                    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(h[j]) : "r"(w), "r"(j % 2 ? 0x6f806f80u : 0x71807180u));
+                    sum = add2(sum, make_float2(bf16_bits_to_f32(w & 0xffffu), __uint_as_float(w & 0xffff0000u)));
+                    most = __vmaxu2(most, w & 0x7f807f80u);
+                }
+                s = sum.x + sum.y;
+                most = max(most & 0xffffu, most >> 16);
+                if (p.x_log >= 5u) {  // a warp on one row
+                    most = __reduce_max_sync(0xffffffffu, most);
+                    if ((threadIdx.x & 31u) == 0u && in) atomicMax(&top[rows_of[b]], most >> 7);
+                } else {
+                    if (in) atomicMax(&top[rows_of[b]], most >> 7);
+                }
             }
-            s *= power(-100);  // 2^-133 in two steps, with what follows
 #pragma unroll
             for (int o = 1; o < GROUP / 8; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-            if (!OWN) {
-#pragma unroll
-                for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-                if (in && cs[b] % 16u == 0u) atomicMax(&top[rows_of[b]], most >> 23);
-            }
             if (in) {
                 *reinterpret_cast<uint4*>(smem + rows_of[b] * p.x_pitch + cs[b] * 16u) =
                     make_uint4(h[0], h[1], h[2], h[3]);
@@ -521,17 +538,16 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
     __shared__ uint32_t top[8 * NT];
     __shared__ RowScale own[8 * NT];
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, g = lane / 4u, t = lane % 4u;
-    const uint32_t rank = blockIdx.x % p.S, cluster = blockIdx.x / p.S, clusters = p.clusters;
+    const uint32_t rank = blockIdx.x & (p.S - 1u), cluster = blockIdx.x >> p.S_log;
     const uint32_t m0 = blockIdx.y * 8u * NT;
     // This CTA's blocks of k and its cluster's tiles, in runs of RT.
-    const uint32_t kb0 = (uint32_t)((uint64_t)p.kb * rank / p.S);
-    const uint32_t nkb = (uint32_t)((uint64_t)p.kb * (rank + 1) / p.S) - kb0;
-    const uint32_t t0 = (uint32_t)((uint64_t)p.tiles * cluster / clusters);
-    const uint32_t t1 = (uint32_t)((uint64_t)p.tiles * (cluster + 1) / clusters);
+    const uint32_t kb0 = rank * p.kb_each + min(rank, p.kb_more), nkb = p.kb_each + (rank < p.kb_more ? 1u : 0u);
+    const uint32_t t0 = cluster * p.tiles_each + min(cluster, p.tiles_more);
+    const uint32_t t1 = t0 + p.tiles_each + (cluster < p.tiles_more ? 1u : 0u);
     const uint32_t runs = (t1 - t0 + RT - 1) / RT;
     // This warp's share: runs wn, wn + WN, ... and blocks [b0, b0 + nb) of kb0 ...
-    const uint32_t WN = kMvWarps / p.WK, wn = warp / p.WK, wk = warp % p.WK;
-    const uint32_t b0 = nkb * wk / p.WK, nb = nkb * (wk + 1) / p.WK - b0;
+    const uint32_t WN = kMvWarps >> p.WK_log, wn = warp >> p.WK_log, wk = warp & (p.WK - 1u);
+    const uint32_t b0 = nkb * wk >> p.WK_log, nb = (nkb * (wk + 1) >> p.WK_log) - b0;
     const bool joined = p.S * p.WK > 1;
     const uint64_t tile_bytes = (uint64_t)p.kb * kBytes;
 
@@ -544,7 +560,7 @@ __global__ void __launch_bounds__(kMvThreads, 1) matvec_kernel(const __grid_cons
 
     // The warp's blocks in order, one commit group for a block of each tile of
     // the run (empty past the end).
-    const uint32_t my_runs = nb && wn < runs ? (runs - wn + WN - 1) / WN : 0u;
+    const uint32_t my_runs = nb && wn < runs ? (runs - wn + WN - 1) >> (kMvLog - p.WK_log) : 0u;
     uint32_t left = my_runs * nb, in_run = nb, is_tile = t0 + RT * wn;
     const uint8_t* src = p.packed + (uint64_t)is_tile * tile_bytes + (uint64_t)(kb0 + b0) * kBytes + lane * 16u;
     auto issue = [&](uint8_t* slot) {
@@ -851,6 +867,10 @@ cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, cons
     p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0;
     const uint32_t bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
     if (!plan_matvec(p, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    while (1u << p.S_log < p.S) ++p.S_log;
+    while (1u << p.WK_log < p.WK) ++p.WK_log;
+    p.kb_each = p.kb / p.S, p.kb_more = p.kb % p.S;
+    p.tiles_each = p.tiles / p.clusters, p.tiles_more = p.tiles % p.clusters;
     for (p.x_log = 4; p.x_log < 9 && (1u << p.x_log) < (p.kb + p.S - 1) / p.S * 16; ++p.x_log) {
     }
     const uint32_t smem = p.off_ring + kMvWarps * mv_ahead((int)p.rt) * p.rt * bytes;
