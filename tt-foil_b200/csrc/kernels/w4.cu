@@ -809,16 +809,24 @@ cudaError_t dequantize_tiles(const uint8_t* packed, uint16_t* tiles, const Weigh
 }
 
 // The rows of x (8 nt) and the tiles (rt) that a warp takes at a time, the
-// split of K over the CTAs of a cluster (S) and the warps of a CTA (WK): those
-// whose busiest warp has the least to do, where the slice of x fits.  The unit
-// is one block of a tile at the rate of two tiles and 8 rows; one tile at a
-// time costs 1.15 a block and 16 rows 1.3 (measured at 4096 x 65536).
+// split of K over the CTAs of a cluster (S) and the warps of a CTA (WK): the
+// plan of least estimated time, where the slice of x fits.  The terms, in ns,
+// are fitted to what 1 to 16 rows measured over all plans at 2048 x 2048 to
+// 65536 x 4096 (the plan taken is within 5 % of the best there):
+//  staging: 10 a row and block of k (30 if rows are not aligned), so that more
+//  rows want a larger S;
+//  the warps' steps: 25 to 37 a block for each warp at work, 160 at least;
+//  250 for each run of tiles of a warp, 400 for a join in a CTA, 1000 in a
+//  cluster and 6 for each part;
+//  HBM: 43 bytes an SM, with fewer SMs at work for larger clusters, and less
+//  with fewer than 48,000 bytes on their way to an SM.
 static bool plan_matvec(Matvec& p, uint32_t bytes, uint32_t group, uint32_t sms) {
     float best = 0.0f;
     for (uint32_t kind = 0; kind < 4; ++kind) {
         const uint32_t nt = 1 + kind / 2, rt = 1 + kind % 2, width = 8 * nt;
-        if (nt == 2 && p.M <= 8) break;
-        const float step = (rt == 2 ? 2.0f : 1.15f) * (nt == 2 ? 1.3f : 1.0f);
+        if ((nt == 2) != (p.M > 8) && best > 0.0f) continue;  // 8 rows at a time only where 16 do not fit
+        const uint32_t rows = p.M < width ? p.M : width, groups_of_rows = (p.M + width - 1) / width;
+        const float block = (nt == 2 ? (rt == 2 ? 33.0f : 37.0f) : (rt == 2 ? 25.0f : 26.0f)) * (group == 32 ? 1.3f : 1.0f);
         const uint32_t ring = kMvWarps * mv_ahead((int)rt) * rt * bytes;
         for (uint32_t S = 1; S <= 8 && S <= p.kb; S *= 2) {
             const uint32_t ks = (p.kb + S - 1) / S;
@@ -827,12 +835,10 @@ static bool plan_matvec(Matvec& p, uint32_t bytes, uint32_t group, uint32_t sms)
             const uint32_t off_red = (off_sum + sums + 127) / 128 * 128;
             const uint32_t fit = S == 1 ? sms : foil_resident_clusters(S), clusters = fit < p.tiles ? fit : p.tiles;
             const uint32_t tc = ((p.tiles + clusters - 1) / clusters + rt - 1) / rt;  // runs of rt tiles
+            const float staging = 300.0f + (float)(rows * ks) * (p.x_vec ? 10.0f : 30.0f);
+            const float hbm = (float)p.tiles * p.kb * bytes / (43.0f * clusters * S);
             for (uint32_t wk = 1; wk <= kMvWarps && wk <= ks; wk *= 2) {
-                // A run's set-up costs about as much as a block, its join as much
-                // again and a tenth for each part.
-                const uint32_t wn = kMvWarps / wk;
-                const float once = S * wk > 1 ? 2.0f + 0.1f * S * wk : 1.0f;
-                const float units = (tc + wn - 1) / wn * ((ks + wk - 1) / wk * step + once);
+                const uint32_t wn = kMvWarps / wk, rounds = (tc + wn - 1) / wn, rest = tc % wn * wk;
                 const uint32_t place = S * wk * 512 * rt * nt;  // one run's parts
                 const uint32_t min_red = S * wk > 1 ? (wn + S - 1) / S * place : 0;
                 if (off_red + min_red + ring > kMaxSmem - 1024) continue;
@@ -846,8 +852,14 @@ static bool plan_matvec(Matvec& p, uint32_t bytes, uint32_t group, uint32_t sms)
                     red = 0;
                 }
                 const uint32_t passes = (tc + pass - 1) / pass;
-                const float cost = (units + passes * (S > 1 ? 4.0f : wk > 1 ? 1.0f : 0.0f)) * ((p.M + width - 1) / width);
-                if (best > 0.0f && cost >= best) continue;
+                const float last = rest == 0 ? 0.0f : block * rest > 160.0f ? block * rest : 160.0f;
+                const float steps = (float)((ks + wk - 1) / wk * rt) * (tc / wn * block * kMvWarps + last);
+                const float join = (float)passes * (S > 1 ? 1000.0f : wk > 1 ? 400.0f : 0.0f) + 6.0f * tc * wk * rt * nt;
+                const uint32_t busy = tc < wn ? tc * wk : kMvWarps;
+                const float ahead = (float)busy * mv_ahead((int)rt) * rt * bytes;
+                const float read = ahead < 48000.0f ? hbm * (48000.0f / ahead) : hbm;
+                const float cost = (staging + (steps > read ? steps : read) + 250.0f * rounds + join) * groups_of_rows;
+                if (best > 0.0f && cost >= best && p.nt == nt) continue;
                 best = cost;
                 p.nt = nt, p.rt = rt, p.S = S, p.WK = wk, p.clusters = clusters;
                 p.x_pitch = pitch, p.off_sum = off_sum, p.off_red = off_red;
