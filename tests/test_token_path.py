@@ -197,13 +197,17 @@ def test_binding_refuses_tensors_it_cannot_describe():
     host = torch.zeros(4, 64, dtype=torch.int16)
     with pytest.raises(Exception):  # no CUDA device here, or not a CUDA tensor
         ttfoil.embed_rows(torch.zeros(4, dtype=torch.int32), host, host, 4, 4, 64)
+    for bad in (host.t(), host[0].expand(4, 64), host[:, :48].unsqueeze(0)):
+        with pytest.raises(ttfoil.FoilError):
+            ttfoil._mat(bad, 0, -1)
     with pytest.raises(ttfoil.FoilError):
-        ttfoil._ld(host.t(), 0)
+        ttfoil._mat(host, 0, 0)  # on another device
     with pytest.raises(ttfoil.FoilError):
-        ttfoil._ld(host[0].expand(4, 64), 0)
+        ttfoil._vec(host, 0)
     with pytest.raises(ttfoil.FoilError):
-        ttfoil._dense(host[:, :3])
-    assert ttfoil._ld(host[:, :48], 0) == 64 and ttfoil._ld(host.view(-1), 0) == 0
+        ttfoil._vec(host[:, :3], -1)
+    assert ttfoil._mat(host[:, :48], 0, -1)[1] == 64 and ttfoil._mat(host.view(-1), 0, -1)[1] == 0
+    assert ttfoil._mat(host[:1, :48], 0, -1)[1] == 0 and ttfoil._mat(None, 5, -1) == (None, 5)
     with pytest.raises(ttfoil.FoilError):
         ttfoil._is_fp32(None, host, torch.zeros(1))
     with pytest.raises(ttfoil.FoilError):

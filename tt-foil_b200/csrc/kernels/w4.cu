@@ -3,6 +3,7 @@
 // foil_w4_pack_dev in include/foil_c.h.
 #include "w4.cuh"
 
+#include <cstring>
 #include <type_traits>
 
 #include "gemm_ptx.cuh"
@@ -878,7 +879,23 @@ cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, cons
     p.kb = blocks_k(w), p.tiles = (w.N + 15) / 16, p.relu = relu ? 1 : 0;
     p.x_vec = (uintptr_t)x % 16 == 0 && ld_x % 8 == 0;
     const uint32_t bytes = block_bytes(w.group, w.zeros), sms = (uint32_t)foil_sm_count();
-    if (!plan_matvec(p, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+    // The plan depends on the sizes alone; each thread keeps its latest ones
+    // (making one takes as long as a launch).
+    struct Known {
+        uint32_t key[7];
+        Matvec plan;
+    };
+    static thread_local Known known[16];
+    const uint32_t key[7] = {M, w.K, w.N, w.group, w.zeros + 2 * p.x_vec, sms, 1};
+    Known& k = known[(M + w.K / 32 + w.N / 16 * 5 + w.group / 32) % 16];
+    if (memcmp(k.key, key, sizeof key) != 0) {
+        k.key[6] = 0;
+        k.plan = p;
+        if (!plan_matvec(k.plan, bytes, w.group, sms)) return cudaErrorInvalidConfiguration;
+        memcpy(k.key, key, sizeof key);
+    }
+    p = k.plan;
+    p.x = x, p.packed = packed, p.bias = bias, p.y = y, p.ld_x = ld_x, p.ld_y = ld_y, p.relu = relu ? 1 : 0;
     while (1u << p.S_log < p.S) ++p.S_log;
     while (1u << p.WK_log < p.WK) ++p.WK_log;
     p.kb_each = p.kb / p.S, p.kb_more = p.kb % p.S;
