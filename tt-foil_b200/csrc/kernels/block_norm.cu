@@ -333,7 +333,7 @@ struct Shape {
     // CTAs (or clusters) that run at once with `per_sm` threads on an SM.
     uint32_t resident(uint32_t per_sm) const {
         const uint32_t sms = (uint32_t)foil_sm_count(), n = per_sm / threads ? per_sm / threads : 1;
-        return ctas > 1 ? foil_resident_clusters(ctas) : sms * n;
+        return ctas > 1 ? foil_resident_clusters(ctas) * n : sms * n;
     }
 };
 
@@ -349,12 +349,11 @@ struct Chunks {
     uint32_t gates;           // gate rows
 };
 Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
-    // As many teams as run at once, at least 8 tokens each: a chunk writes and
-    // reads 3 x 4 bytes a channel beside the 12 and more of each token.
+    // As many teams as run at once: a chunk writes and reads 3 x 4 bytes a
+    // channel beside the 12 and more of each token.
     const Shape sh(D, 8, 512);
     const uint32_t teams = sh.resident(kBackwardThreads) * sh.teams;
     uint32_t rows = (T + teams - 1) / teams;
-    rows = rows < 8 ? 8 : rows;
     Chunks c{};
     if (gate_rows > T) gate_rows = T;
     c.gates = gate_rows ? (T + gate_rows - 1) / gate_rows : 0;
@@ -362,7 +361,6 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
         // Not more chunks than teams, if there are fewer gate rows.
         c.per_gate = c.gates < teams ? teams / c.gates : 1;
         c.rows = (gate_rows + c.per_gate - 1) / c.per_gate;
-        c.rows = c.rows < 8 ? 8 : c.rows;
         c.per_gate = (gate_rows + c.rows - 1) / c.rows;
         c.count = c.per_gate * c.gates;
     } else {
@@ -550,10 +548,11 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
 }
 
 // Adds the chunks' sums: blockIdx.y 0 and 1 dw_pre and dw_post, 2 + g gate row
-// g.  32 columns a CTA, 8 warps that take every eighth chunk; the warps' sums
+// g.  32 columns a CTA, 32 warps that take every 32nd chunk; the warps' sums
 // are added in order.
-__global__ void __launch_bounds__(256) sum_chunks(const Backward p, const Chunks c) {
-    __shared__ float part[8][32];
+constexpr uint32_t kSumWarps = 32;
+__global__ void __launch_bounds__(32 * kSumWarps) sum_chunks(const Backward p, const Chunks c) {
+    __shared__ float part[kSumWarps][32];
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, i = blockIdx.x * 32u + lane;
@@ -563,13 +562,14 @@ __global__ void __launch_bounds__(256) sum_chunks(const Backward p, const Chunks
         const float* ws = p.ws + ((uint64_t)min(what, 2u) * c.count + first) * p.D + i;
         float s = 0.0f;
         if (i < p.D)
-#pragma unroll 4
-            for (uint32_t k = warp; k < n; k += 8) s += ws[(uint64_t)k * p.D];
+#pragma unroll 8
+            for (uint32_t k = warp; k < n; k += kSumWarps) s += ws[(uint64_t)k * p.D];
         __syncthreads();
         part[warp][lane] = s;
         __syncthreads();
         if (warp != 0 || i >= p.D) continue;
-        for (int k = 1; k < 8; ++k) s += part[k][lane];
+#pragma unroll
+        for (uint32_t k = 1; k < kSumWarps; ++k) s += part[k][lane];
         if (what == 0)
             p.dw_pre[i] = s;
         else if (what == 1)
@@ -616,15 +616,16 @@ cudaError_t forward_launch(const Forward& p, const Shape& sh, cudaStream_t s) {
                   p, sh.ctas);
 }
 
-// 8 channels a thread up to 2048 channels, 16 up to 8192 in a CTA of up to 512
-// threads, then two CTAs.  As many CTAs on an SM as about 85 registers a thread
+// 8 channels a thread up to 2048 channels, then 16: one CTA up to 6144, above
+// that two to four of up to 256 threads (one of 512 leaves an SM a single row at
+// a time: 2000 x 8192 53 us).  As many CTAs on an SM as about 85 registers a thread
 // allow (with 64 they spill, with more too few rows are on their way).
 template <class R, int V, int GATE>
 cudaError_t forward_gated(const Forward& p, cudaStream_t s) {
     if (p.D <= 2048) return forward_launch<R, V, 8, 256, 4, GATE>(p, Shape(p.D, 8, 512), s);
     if (p.D <= 4096) return forward_launch<R, V, 16, 256, 3, GATE>(p, Shape(p.D, 16, 512), s);
     if (p.D <= 6144) return forward_launch<R, V, 16, 384, 2, GATE>(p, Shape(p.D, 16, 512), s);
-    return forward_launch<R, V, 16, 512, 1, GATE>(p, Shape(p.D, 16, 512), s);
+    return forward_launch<R, V, 16, 256, 3, GATE>(p, Shape(p.D, 16, 256), s);
 }
 
 template <class R, int V>
@@ -692,7 +693,7 @@ cudaError_t backward(const Backward& p, bool fp32, cudaStream_t s) {
     Chunks sums = c;
     if (!shared_gate) sums.gates = 0;
     const uint32_t rows = 2 + sums.gates;
-    return launch(sum_chunks, dim3((p.D + 31) / 32, rows < 32768 ? rows : 32768), 256, 1, s, p, sums);
+    return launch(sum_chunks, dim3((p.D + 31) / 32, rows < 32768 ? rows : 32768), 32 * kSumWarps, 1, s, p, sums);
 }
 
 }  // namespace norm

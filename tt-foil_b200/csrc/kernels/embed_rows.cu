@@ -9,7 +9,7 @@
 //     memory.  Meanwhile the other SMs write the zeros of the table's rows that
 //     no token names (each CTA looks through the ids for its rows), so the
 //     table is written once.
-//  2. sum_runs: CTAs take kRun consecutive sorted tokens, add the rows of one
+//  2. sum_runs: CTAs take a run of 8 to 32 consecutive sorted tokens, add the rows of one
 //     id in registers in that order and write an id's sum to the table where
 //     all of its tokens are in the run; the sums of the first and the last id,
 //     where they go on beyond it, go to the workspace.
@@ -168,8 +168,9 @@ cudaError_t lookup_launch(const Lookup& p, cudaStream_t s) {
 }
 
 // -------------------------------------------------------------------- sort ---
-constexpr uint32_t kRun = 32;         // sorted tokens of a run
+constexpr uint32_t kMaxRun = 32;      // sorted tokens of a run, at most
 constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
+constexpr uint32_t kSortAhead = 8;  // rounds of 32 tokens of a warp whose keys are on their way
 constexpr uint32_t kMaxBits = 9, kMaxRadix = 1u << kMaxBits;
 // A warp's counts of each digit, every CTA's, and the scan's; or the marks of
 // a clearing CTA's rows.
@@ -177,7 +178,7 @@ constexpr uint32_t kSortSmem = (kSortWarps * kMaxRadix + kSortCtas * kMaxRadix +
 constexpr uint32_t kMarkRows = kSortSmem * 8 / 32 * 32;  // rows that one CTA can clear
 
 struct Plan {
-    uint32_t runs, slabs;              // runs of tokens, column slabs of a run
+    uint32_t run, runs, slabs;         // tokens of a run, runs, column slabs of a run
     uint32_t ctas, clear;              // CTAs of the sort, CTAs that clear rows
     uint32_t passes, bits;             // passes of `bits` bits
     uint32_t *key0, *token0, *key1, *token1;  // buffers of the sort, in turn
@@ -188,10 +189,14 @@ uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
 
 Plan make_plan(const Gradient& p, uint64_t* bytes) {
     Plan q{};
-    q.runs = (p.T + kRun - 1) / kRun;
+    // Short runs where there are few tokens, so that they fill the SMs.
+    q.run = kMaxRun;
+    while (q.run > 8 && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
+    q.runs = (p.T + q.run - 1) / q.run;
     // One CTA sorts few tokens as fast.  Clusters of 4 leave 128 SMs to the
-    // zeros, of 8 only 112 (a cluster stays inside a GPC).
-    q.ctas = p.T <= 4096 ? 1 : p.accumulate ? kSortCtas : kSortCtas / 2;
+    // zeros, of 8 only 112 (a cluster stays inside a GPC) but sort many tokens
+    // in half the time.
+    q.ctas = p.T <= 4096 ? 1 : p.accumulate || p.T > 32768 ? kSortCtas : kSortCtas / 2;
     uint32_t bits = 1;
     while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
     q.passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -272,12 +277,20 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p,
         };
         for (uint32_t d = lane; d < radix; d += 32u) mine[d] = 0u;
         __syncwarp();
-        for (uint32_t i0 = first; i0 < last; i0 += 32u) {
-            const uint32_t i = i0 + lane;
-            const uint32_t d = i < last ? key_of(i) >> shift & (radix - 1u) : ~0u;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d);
-            if (i < last && (peers & ((1u << lane) - 1u)) == 0u) mine[d] += __popc(peers);
-            __syncwarp();
+        for (uint32_t i0 = first; i0 < last; i0 += 32u * kSortAhead) {
+            uint32_t key[kSortAhead];
+#pragma unroll
+            for (uint32_t b = 0; b < kSortAhead; ++b)
+                key[b] = i0 + 32u * b + lane < last ? key_of(i0 + 32u * b + lane) : ~0u;
+#pragma unroll
+            for (uint32_t b = 0; b < kSortAhead; ++b) {
+                if (i0 + 32u * b >= last) break;  // the whole warp
+                const bool in = i0 + 32u * b + lane < last;
+                const uint32_t d = in ? key[b] >> shift & (radix - 1u) : ~0u;
+                const uint32_t peers = __match_any_sync(0xffffffffu, d);
+                if (in && (peers & ((1u << lane) - 1u)) == 0u) mine[d] += __popc(peers);
+                __syncwarp();
+            }
         }
         __syncthreads();
         // Digit tid: the tokens of the warps before each warp, and of the CTA.
@@ -325,20 +338,30 @@ __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens(const Gradient p,
             for (uint32_t w = 0; w < kSortWarps; ++w) count[w * kMaxRadix + tid] = n[w] + base;
         }
         __syncthreads();
-        for (uint32_t i0 = first; i0 < last; i0 += 32u) {
-            const uint32_t i = i0 + lane;
-            const uint32_t key = i < last ? key_of(i) : ~0u, d = i < last ? key >> shift & (radix - 1u) : ~0u;
-            const uint32_t token = i >= last ? 0u : pass ? __ldcg(token_in + i) : i;
-            const uint32_t peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1u);
-            uint32_t at = 0;
-            if (i < last) at = mine[d] + __popc(lower);
-            __syncwarp();
-            if (i < last) {
-                if (lower == 0u) mine[d] += __popc(peers);
-                key_out[at] = key;
-                token_out[at] = token;
+        for (uint32_t i0 = first; i0 < last; i0 += 32u * kSortAhead) {
+            uint32_t key[kSortAhead], token[kSortAhead];
+#pragma unroll
+            for (uint32_t b = 0; b < kSortAhead; ++b) {
+                const uint32_t i = i0 + 32u * b + lane;
+                key[b] = i < last ? key_of(i) : ~0u;
+                token[b] = i >= last ? 0u : pass ? __ldcg(token_in + i) : i;
             }
-            __syncwarp();
+#pragma unroll
+            for (uint32_t b = 0; b < kSortAhead; ++b) {
+                if (i0 + 32u * b >= last) break;  // the whole warp
+                const bool in = i0 + 32u * b + lane < last;
+                const uint32_t d = in ? key[b] >> shift & (radix - 1u) : ~0u;
+                const uint32_t peers = __match_any_sync(0xffffffffu, d), lower = peers & ((1u << lane) - 1u);
+                uint32_t at = 0;
+                if (in) at = mine[d] + __popc(lower);
+                __syncwarp();
+                if (in) {
+                    if (lower == 0u) mine[d] += __popc(peers);
+                    key_out[at] = key[b];
+                    token_out[at] = token[b];
+                }
+                __syncwarp();
+            }
         }
         sync_all();
     }
@@ -349,15 +372,15 @@ constexpr uint32_t kAhead = 8;  // rows of tokens on their way
 
 template <class I, int V>
 __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Plan q) {
-    __shared__ uint32_t key[kRun + 2], token[kRun];
+    __shared__ uint32_t key[kMaxRun + 2], token[kMaxRun];
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
-    const uint32_t run = (uint32_t)(blockIdx.x / q.slabs), first = run * kRun, n = min(kRun, p.T - first);
+    const uint32_t run = (uint32_t)(blockIdx.x / q.slabs), first = run * q.run, n = min(q.run, p.T - first);
     const uint32_t *keys = q.key, *tokens = q.token;
-    if (threadIdx.x < kRun + 2u) {  // the keys before and after the run too
+    if (threadIdx.x < q.run + 2u) {  // the keys before and after the run too
         const uint32_t i = first + threadIdx.x - 1u;
         key[threadIdx.x] = first + threadIdx.x >= 1u && i < p.T ? __ldcg(keys + i) : ~0u;
-        if (threadIdx.x >= 1u && threadIdx.x <= kRun && i < p.T) token[threadIdx.x - 1u] = __ldcg(tokens + i);
+        if (threadIdx.x >= 1u && threadIdx.x <= q.run && i < p.T) token[threadIdx.x - 1u] = __ldcg(tokens + i);
     }
     __syncthreads();
     const uint32_t col = (blockIdx.x % q.slabs * kThreads + threadIdx.x) * V;
@@ -403,50 +426,64 @@ __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Pla
     }
 }
 
-// blockIdx.x: a run whose last id begins there and goes on; blockIdx.y: 256
-// columns.  8 warps take every eighth part, their sums are added in order.
-constexpr uint32_t kJoinColumns = 256;
+// blockIdx.x: eight runs, of which those count whose last id begins there and
+// goes on; blockIdx.y: 256 columns.  8 warps take every eighth part, their sums
+// are added in order.
+constexpr uint32_t kJoinColumns = 256, kJoinRuns = 8;
 
 __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Plan q) {
     __shared__ float part[kThreads / 32][kJoinColumns];
+    __shared__ uint32_t ids[kJoinRuns], ends[kJoinRuns];  // the id (~0: nothing to do), the run after its last part
     griddep_wait();  // launched with programmatic stream serialization
     griddep_launch_dependents();
-    const uint32_t *keys = q.key, run = blockIdx.x, first = run * kRun, end = first + kRun;
-    if (end >= p.T) return;
-    const uint32_t id = __ldcg(keys + end - 1u), next = __ldcg(keys + end), begin = __ldcg(keys + first);
-    const uint32_t previous = first ? __ldcg(keys + first - 1u) : ~0u;
-    if (id >= p.V || next != id) return;
-    if (begin == id && previous == id) return;  // began earlier
-    // Runs after this one that begin with the id: lo begins with it, hi does
-    // not; 32 places between them at a time.
-    uint32_t lo = run + 1u, hi = q.runs;
-    while (hi - lo > 1u) {
-        const uint32_t step = (hi - lo + 32u) / 33u, at = lo + (threadIdx.x % 32u + 1u) * step;
-        const uint32_t in = __popc(__ballot_sync(0xffffffffu, at < hi && __ldcg(keys + (uint64_t)at * kRun) == id));
-        hi = min(hi, lo + (in + 1u) * step);
-        lo += in * step;
+    const uint32_t *keys = q.key, warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
+    // Warp w looks at run w.
+    {
+        const uint64_t run = (uint64_t)blockIdx.x * kJoinRuns + warp, first = run * q.run, end = first + q.run;
+        uint32_t found = ~0u, lo = (uint32_t)run + 1u, hi = q.runs;
+        if (end < p.T) {
+            const uint32_t id = __ldcg(keys + end - 1u), next = __ldcg(keys + end), begin = __ldcg(keys + first);
+            const uint32_t previous = first ? __ldcg(keys + first - 1u) : ~0u;
+            if (id < p.V && next == id && !(begin == id && previous == id)) found = id;
+        }
+        // Runs after this one that begin with the id: lo begins with it, hi does
+        // not; 32 places between them at a time.
+        while (found != ~0u && hi - lo > 1u) {
+            const uint32_t step = (hi - lo + 32u) / 33u, at = lo + (lane + 1u) * step;
+            const uint32_t in =
+                __popc(__ballot_sync(0xffffffffu, at < hi && __ldcg(keys + (uint64_t)at * q.run) == found));
+            hi = min(hi, lo + (in + 1u) * step);
+            lo += in * step;
+        }
+        if (lane == 0) ids[warp] = found, ends[warp] = hi;
     }
-    const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u, col = blockIdx.y * kJoinColumns + lane;
-    constexpr int kEach = kJoinColumns / 32;
-    float s[kEach] = {};
-    for (uint32_t r = run + warp; r < hi; r += kThreads / 32u) {
-        const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
-#pragma unroll
-        for (int j = 0; j < kEach; ++j)
-            if (col + 32u * j < p.D) s[j] += row[32 * j];
-    }
-#pragma unroll
-    for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = s[j];
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k < kJoinColumns; k += kThreads) {
-        const uint32_t i = blockIdx.y * kJoinColumns + k;
-        if (i >= p.D) return;
-        float sum = 0.0f;
-        for (uint32_t w = 0; w < kThreads / 32u; ++w) sum += part[w][k];
-        float* at = p.dtable + (uint64_t)id * p.ld_dtable + i;
-        *at = fmaf(p.scale, sum, p.accumulate ? *at : 0.0f);
+    const uint32_t col = blockIdx.y * kJoinColumns + lane;
+    constexpr int kEach = kJoinColumns / 32;
+    for (uint32_t w = 0; w < kJoinRuns; ++w) {
+        const uint32_t id = ids[w], run = blockIdx.x * kJoinRuns + w, hi = ends[w];
+        if (id == ~0u) continue;
+        float s[kEach] = {};
+        for (uint32_t r = run + warp; r < hi; r += kThreads / 32u) {
+            const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
+#pragma unroll
+            for (int j = 0; j < kEach; ++j)
+                if (col + 32u * j < p.D) s[j] += row[32 * j];
+        }
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = s[j];
+        __syncthreads();
+        const uint32_t i = blockIdx.y * kJoinColumns + threadIdx.x;
+        if (i < p.D) {
+            float sum = 0.0f;
+            for (uint32_t k = 0; k < kThreads / 32u; ++k) sum += part[k][threadIdx.x];
+            float* at = p.dtable + (uint64_t)id * p.ld_dtable + i;
+            *at = fmaf(p.scale, sum, p.accumulate ? *at : 0.0f);
+        }
+        __syncthreads();
     }
 }
+static_assert(kJoinColumns == kThreads && kJoinRuns == kThreads / 32, "a thread a column, a warp a run");
 
 template <int V>
 cudaError_t sort_launch(const Gradient& p, Plan& q, cudaStream_t s) {
@@ -506,7 +543,7 @@ cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
     w.use(p.dout, p.ld_dout, fp32 ? 4 : 2);
     e = fp32 ? sum_launch<float>(p, q, w.v, s) : sum_launch<uint16_t>(p, q, w.v, s);
     if (e != cudaSuccess || q.runs < 2) return e;
-    return launch(join_runs, dim3(q.runs, (p.D + kJoinColumns - 1) / kJoinColumns), kThreads, 0, 1, s, p, q);
+    return launch(join_runs, dim3((q.runs + kJoinRuns - 1) / kJoinRuns, (p.D + kJoinColumns - 1) / kJoinColumns), kThreads, 0, 1, s, p, q);
 }
 
 }  // namespace embed
