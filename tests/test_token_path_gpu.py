@@ -460,6 +460,17 @@ def test_block_norm_gradient_of_shared_gates(gate_rows):
     check_backward(p, saved, run_backward(p, saved))
 
 
+@pytest.mark.parametrize("T,D,gate_rows", [(2500, 1, 0), (77, 2, 1), (3, 8, 2), (19003, 24, 1), (700, 17, 700),
+                                           (3001, 40, 7), (2500, 64, 1000), (20001, 96, 0), (1999, 129, 1),
+                                           (1205, 250, 60), (2000, 256, 1)])
+def test_block_norm_of_narrow_rows(T, D, gate_rows):
+    """Several rows share a warp; the last CTA's teams are without tokens."""
+    p = Norm(T, D, D % 3 == 0, True, gate_rows, "sigmoid" if T % 2 else "none")
+    saved = run_forward(p)
+    check_forward(p, saved)
+    check_backward(p, saved, run_backward(p, saved))
+
+
 @pytest.mark.parametrize("want", [("dresid",), ("du",), ("dgate",), ("dw_post",), ("dw_pre",), ("du", "dw_pre")])
 @pytest.mark.parametrize("dh,dy", [(True, True), (True, False), (False, True)])
 def test_block_norm_gradient_parts(want, dh, dy):

@@ -119,11 +119,12 @@ __device__ __forceinline__ void store_plain(float* p, const float2 (&v)[V * NV /
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
 __device__ __forceinline__ float2 sigmoid2(float2 g) { return make_float2(sigmoid(g.x), sigmoid(g.y)); }
 
-// The threads that hold one row: a warp, a CTA, or the CTAs of a cluster.
+// The threads that hold one row: 4 to 32 lanes of a warp, a CTA, or the CTAs of
+// a cluster.
 struct Team {
     uint32_t size, rank;    // threads, this thread
     uint32_t lane;
-    uint32_t ctas;          // CTAs of a team (0: the team is a warp)
+    uint32_t ctas;          // CTAs of a team (0: the team is in a warp)
     uint32_t index, count;  // this team, teams of the grid
     float* shared;          // two sets of kSumFloats floats
     uint32_t flip;
@@ -136,6 +137,13 @@ struct Team {
     __device__ __forceinline__ void sum(float (&v)[N]) {
         constexpr uint32_t kAll = 0xffffffffu;
         float s;
+        if (size < 32u) {  // the warp's other teams may be elsewhere
+            const uint32_t mask = ((1u << size) - 1u) << (lane & ~(size - 1u));
+            for (uint32_t o = size / 2u; o; o >>= 1)
+#pragma unroll
+                for (int n = 0; n < N; ++n) v[n] += __shfl_xor_sync(mask, v[n], o);
+            return;
+        }
         if constexpr (N == 1) {
             s = v[0];
 #pragma unroll
@@ -183,13 +191,19 @@ struct Team {
     static constexpr uint32_t kMaxTeamWarps = 64, kSumFloats = 4 * kMaxTeamWarps;
 };
 
-__device__ __forceinline__ Team team_of(uint32_t ctas, float* shared) {
-    if (ctas == 0) {
-        const uint32_t per = blockDim.x / 32u;
-        return Team{32u, threadIdx.x % 32u, threadIdx.x % 32u, 0u, blockIdx.x * per + threadIdx.x / 32u, gridDim.x * per, shared, 0u};
+// A team as the host planned it: `ctas` CTAs, or (0) `lanes` lanes of a warp.
+struct TeamPlan {
+    uint32_t ctas, lanes;
+};
+__device__ __forceinline__ Team team_of(const TeamPlan& t, float* shared) {
+    const uint32_t lane = threadIdx.x % 32u;
+    if (t.ctas == 0) {
+        const uint32_t per = blockDim.x / t.lanes;
+        return Team{t.lanes, lane & (t.lanes - 1u), lane, 0u, blockIdx.x * per + threadIdx.x / t.lanes,
+                    gridDim.x * per, shared, 0u};
     }
-    return Team{ctas * blockDim.x, blockIdx.x % ctas * blockDim.x + threadIdx.x, threadIdx.x % 32u, ctas, blockIdx.x / ctas,
-                gridDim.x / ctas, shared, 0u};
+    return Team{t.ctas * blockDim.x, blockIdx.x % t.ctas * blockDim.x + threadIdx.x, lane, t.ctas,
+                blockIdx.x / t.ctas, gridDim.x / t.ctas, shared, 0u};
 }
 
 // Element of vector j of this thread.  Threads past D read the last vector
@@ -266,10 +280,10 @@ __device__ __forceinline__ float2 gate2(const Raw<uint16_t, V> (&r)[NV], int i) 
 }
 
 template <class R, int V, int NV, int THREADS, int CTAS, int GATE>
-__global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p, uint32_t team_ctas) {
+__global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p, const TeamPlan plan) {
     __shared__ float shared[2 * Team::kSumFloats];
-    Team team = team_of(team_ctas, shared);
-    if (team_ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
+    Team team = team_of(plan, shared);
+    if (plan.ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
     griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
     const float inv_d = 1.0f / (float)p.D;
@@ -319,21 +333,24 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
     }
 }
 
-// A row's team of E channels a thread in CTAs of at most `most` threads: a warp
-// (4 of them share a CTA), a CTA, or a cluster of CTAs.
+// A row's team of E channels a thread in CTAs of at most `most` threads: lanes
+// of a warp (a CTA has 128), a CTA, or a cluster of CTAs.
 constexpr uint32_t kBackwardThreads = 512;  // of an SM, by registers
 struct Shape {
-    uint32_t threads, ctas, teams;  // threads of a CTA, CTAs of a team (0: a warp), teams of a CTA
+    uint32_t threads, teams;  // threads and teams of a CTA
+    TeamPlan plan;
     Shape(uint32_t D, uint32_t E, uint32_t most) {
         const uint32_t team = (D + 32 * E - 1) / (32 * E) * 32;
-        ctas = team == 32 ? 0 : (team + most - 1) / most;
-        threads = team == 32 ? 128 : ((team + ctas - 1) / ctas + 31) / 32 * 32;
-        teams = ctas ? 1 : 4;
+        plan.ctas = team == 32 ? 0 : (team + most - 1) / most;
+        plan.lanes = 32;
+        while (team == 32 && plan.lanes > 4 && plan.lanes / 2 * E >= D) plan.lanes /= 2;
+        threads = plan.ctas ? ((team + plan.ctas - 1) / plan.ctas + 31) / 32 * 32 : 128;
+        teams = plan.ctas ? 1 : 128 / plan.lanes;
     }
     // CTAs (or clusters) that run at once with `per_sm` threads on an SM.
     uint32_t resident(uint32_t per_sm) const {
         const uint32_t sms = (uint32_t)foil_sm_count(), n = per_sm / threads ? per_sm / threads : 1;
-        return ctas > 1 ? foil_resident_clusters(ctas) * n : sms * n;
+        return plan.ctas > 1 ? foil_resident_clusters(plan.ctas) * n : sms * n;
     }
 };
 
@@ -345,6 +362,7 @@ struct Shape {
 // them in order.
 struct Chunks {
     uint32_t rows, count;     // tokens of a chunk, chunks
+    uint32_t parts;           // sums of dw_pre and dw_post: of a chunk, or of a CTA of several
     uint32_t per_gate;        // chunks of a gate row, 0: a chunk holds whole gate rows
     uint32_t gates;           // gate rows
 };
@@ -367,6 +385,7 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
         c.rows = gate_rows ? rows / gate_rows * gate_rows : rows;
         c.count = (T + c.rows - 1) / c.rows;
     }
+    c.parts = sh.plan.ctas ? c.count : (c.count + sh.teams - 1) / sh.teams;
     return c;
 }
 
@@ -375,18 +394,19 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
 // uhat, dw_post gains act A and dgate is act' w_post A), else a gate row for
 // each token.
 template <class R, int V, int NV, int THREADS, int GATE>
-__global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, uint32_t team_ctas) {
+__global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, const TeamPlan plan) {
     constexpr int kPairs = V * NV / 2;
     __shared__ float shared[2 * Team::kSumFloats];
     __shared__ float2 post_sum[GATE ? 1 : kPairs * THREADS];  // dw_post of the gate rows done, a slot for each thread
-    Team team = team_of(team_ctas, shared);
-    if (team_ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
+    Team team = team_of(plan, shared);
+    if (plan.ctas > 1) cluster_sync();  // every CTA of the team runs before its memory is written
     griddep_wait();                     // launched with programmatic stream serialization
     griddep_launch_dependents();
-    if (team.index >= c.count) return;  // whole warps, or nobody
-    // Tokens [t0, t1).
+    // Tokens [t0, t1); none past the last chunk.
     uint32_t t0, t1;
-    if (c.per_gate) {
+    if (team.index >= c.count) {
+        t0 = t1 = 0;
+    } else if (c.per_gate) {
         const uint64_t gate0 = (uint64_t)(team.index / c.per_gate) * p.gate_rows;
         const uint64_t end = min((uint64_t)p.T, gate0 + p.gate_rows);
         const uint64_t first = min(end, gate0 + (uint64_t)(team.index % c.per_gate) * c.rows);
@@ -460,7 +480,7 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
         }
         if (!p.gate || !p.dgate) return;
         if (c.per_gate)
-            store_plain<V, NV>(p.ws + (2ull * c.count + team.index) * p.D, dgate, team, p.D);
+            store_plain<V, NV>(p.ws + (2ull * c.parts + team.index) * p.D, dgate, team, p.D);
         else
             store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
     };
@@ -537,14 +557,37 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
         }
         if constexpr (!GATE)
             if (!p.gate || gate_left != p.gate_rows) end_gate();  // the last row's tokens go on in another chunk, or end
-    } else if (!GATE && c.per_gate && p.dgate) {
-        store_plain<V, NV>(p.ws + (2ull * c.count + team.index) * p.D, dw_post, team, p.D);  // no tokens: zeros
+    } else if (!GATE && c.per_gate && p.dgate && team.index < c.count) {
+        store_plain<V, NV>(p.ws + (2ull * c.parts + team.index) * p.D, dw_post, team, p.D);  // no tokens: zeros
     }
     if constexpr (!GATE)
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) dw_post[i] = post_sum[i * blockDim.x + threadIdx.x];
-    if (p.dw_pre) store_plain<V, NV>(p.ws + (uint64_t)team.index * p.D, dw_pre, team, p.D);
-    if (p.dw_post) store_plain<V, NV>(p.ws + ((uint64_t)c.count + team.index) * p.D, dw_post, team, p.D);
+    if (plan.ctas) {
+        if (p.dw_pre) store_plain<V, NV>(p.ws + (uint64_t)team.index * p.D, dw_pre, team, p.D);
+        if (p.dw_post) store_plain<V, NV>(p.ws + ((uint64_t)c.parts + team.index) * p.D, dw_post, team, p.D);
+        return;
+    }
+    // The sums of the CTA's teams, in order.
+    __shared__ float2 all[kPairs][128];
+    const uint32_t per = 128u / team.size;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        if (w ? !p.dw_post : !p.dw_pre) continue;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) all[i][threadIdx.x] = w ? dw_post[i] : dw_pre[i];
+        __syncthreads();
+        if (threadIdx.x < team.size) {  // the first team adds
+            float2 sum[kPairs];
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) sum[i] = all[i][threadIdx.x];
+            for (uint32_t k = 1; k < per; ++k)
+#pragma unroll
+                for (int i = 0; i < kPairs; ++i) sum[i] = add2(sum[i], all[i][k * team.size + threadIdx.x]);
+            store_plain<V, NV>(p.ws + ((uint64_t)w * c.parts + blockIdx.x) * p.D, sum, team, p.D);
+        }
+    }
 }
 
 // Adds the chunks' sums: blockIdx.y 0 and 1 dw_pre and dw_post, 2 + g gate row
@@ -558,8 +601,8 @@ __global__ void __launch_bounds__(32 * kSumWarps) sum_chunks(const Backward p, c
     const uint32_t lane = threadIdx.x % 32u, warp = threadIdx.x / 32u, i = blockIdx.x * 32u + lane;
     for (uint32_t what = blockIdx.y; what < 2u + c.gates; what += gridDim.y) {
         if ((what == 0 && !p.dw_pre) || (what == 1 && !p.dw_post)) continue;
-        const uint32_t first = what < 2u ? 0u : (what - 2u) * c.per_gate, n = what < 2u ? c.count : c.per_gate;
-        const float* ws = p.ws + ((uint64_t)min(what, 2u) * c.count + first) * p.D + i;
+        const uint32_t first = what < 2u ? 0u : (what - 2u) * c.per_gate, n = what < 2u ? c.parts : c.per_gate;
+        const float* ws = p.ws + ((uint64_t)min(what, 2u) * c.parts + first) * p.D + i;
         float s = 0.0f;
         if (i < p.D)
 #pragma unroll 8
@@ -587,8 +630,7 @@ struct Width {
         while (v > 1 && ((uintptr_t)p % (v * elem < 16 ? v * elem : 16) || ld % v)) v = v == 8 ? 2 : 1;
     }
     explicit Width(uint32_t D) {
-        // Few channels: narrower vectors keep a warp's lanes busy.
-        while (v > 1 && (D % v || D < 32u * v)) v = v == 8 ? 2 : 1;
+        while (v > 1 && D % v) v = v == 8 ? 2 : 1;
     }
 };
 
@@ -612,8 +654,8 @@ template <class R, int V, int E, int THREADS, int CTAS, int GATE>
 cudaError_t forward_launch(const Forward& p, const Shape& sh, cudaStream_t s) {
     const uint32_t resident = sh.resident(THREADS * CTAS);
     const uint32_t teams = (p.T + sh.teams - 1) / sh.teams < resident ? (p.T + sh.teams - 1) / sh.teams : resident;
-    return launch(forward_kernel<R, V, E / V, THREADS, CTAS, GATE>, dim3(teams * (sh.ctas ? sh.ctas : 1)), sh.threads, sh.ctas, s,
-                  p, sh.ctas);
+    const dim3 grid(teams * (sh.plan.ctas ? sh.plan.ctas : 1));
+    return launch(forward_kernel<R, V, E / V, THREADS, CTAS, GATE>, grid, sh.threads, sh.plan.ctas, s, p, sh.plan);
 }
 
 // 8 channels a thread up to 2048 channels, then 16: one CTA up to 6144, above
@@ -637,8 +679,8 @@ cudaError_t forward_typed(const Forward& p, cudaStream_t s) {
 template <class R, int V, int GATE>
 cudaError_t backward_launch(const Backward& p, const Chunks& c, cudaStream_t s) {
     const Shape sh(p.D, 8, 512);
-    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.ctas ? sh.ctas : 1));
-    return launch(backward_kernel<R, V, 8 / V, 512, GATE>, grid, sh.threads, sh.ctas, s, p, c, sh.ctas);
+    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.plan.ctas ? sh.plan.ctas : 1));
+    return launch(backward_kernel<R, V, 8 / V, 512, GATE>, grid, sh.threads, sh.plan.ctas, s, p, c, sh.plan);
 }
 
 template <class R, int V>
@@ -652,7 +694,7 @@ cudaError_t backward_typed(const Backward& p, const Chunks& c, cudaStream_t s) {
 uint64_t backward_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows) {
     if (T == 0 || D == 0) return 0;
     const Chunks c = plan_chunks(T, D, gate_rows);
-    return (uint64_t)c.count * D * 4 * (c.per_gate ? 3 : 2);
+    return (2ull * c.parts + (c.per_gate ? c.count : 0)) * D * 4;
 }
 
 cudaError_t forward(const Forward& p, bool fp32, cudaStream_t s) {

@@ -189,9 +189,10 @@ uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
 
 Plan make_plan(const Gradient& p, uint64_t* bytes) {
     Plan q{};
-    // Short runs where there are few tokens, so that they fill the SMs.
+    // Short runs where there are few tokens, so that they fill the SMs; one run
+    // where one can hold them, which needs no join.
     q.run = kMaxRun;
-    while (q.run > 8 && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
+    while (q.run > 8 && p.T > kMaxRun && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
     q.runs = (p.T + q.run - 1) / q.run;
     // One CTA sorts few tokens as fast.  Clusters of 4 leave 128 SMs to the
     // zeros, of 8 only 112 (a cluster stays inside a GPC) but sort many tokens
