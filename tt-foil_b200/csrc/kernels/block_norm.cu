@@ -5,10 +5,10 @@
 // Bound by HBM, closely followed by instruction issue: every tensor is read
 // and written once, with 10 (forward) to 30 instructions a channel.  A row lives
 // in the registers of one warp, one CTA or a cluster of CTAs (its team), 8 or 16
-// channels a thread; a team goes over many rows, the weights in its registers and
-// the next row on its way while the present one is worked on.  (A ring of three
-// rows in shared memory, tried: 10 to 50 % slower, for the instructions it
-// takes.)  Channels are moved in vectors of 16 bytes where D, the strides and
+// channels a thread; a team goes over many rows, the next ones on their way to L2
+// or to registers while the present one is worked on.  (A ring of three rows in
+// shared memory, tried: 10 to 50 % slower, for the instructions it takes.)
+// Channels are moved in vectors of 16 bytes where D, the strides and
 // the pointers allow, else of 4 bytes (even D), else one by one.
 #include "block_norm.cuh"
 
@@ -250,6 +250,23 @@ struct Input {
     }
 };
 
+// A row of a tensor towards L2: each of a team's first threads asks for one
+// tensor's, the whole 16-byte pieces of it.  Forward, 8192 x 5120: 121 us
+// without, 106 with.
+struct Ahead {
+    uint64_t at;            // row 0
+    uint32_t pitch, bytes;  // bytes 0: nothing to ask for
+    template <class T, int V, int NV>
+    __device__ __forceinline__ void use(const Input<T, V, NV>& in, uint32_t D) {
+        if (in.ld >= 1u << 30) return;
+        at = reinterpret_cast<uint64_t>(in.p), pitch = in.ld * (uint32_t)sizeof(T);
+        bytes = D * (uint32_t)sizeof(T) - (V == 8 ? 0u : 16u) & ~15u;
+    }
+    __device__ __forceinline__ void operator()(uint32_t row) const {
+        const uint64_t from = at + (uint64_t)row * pitch + 15u & ~15ull;
+        asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(from), "r"(bytes) : "memory");
+    }
+};
 // This thread's part of a row's sum of squares.
 template <int V, int NV>
 __device__ __forceinline__ float sum_squares(const float2 (&v)[V * NV / 2], const Team& t, uint32_t D) {
@@ -289,6 +306,12 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
     const float inv_d = 1.0f / (float)p.D;
     const Input<R, V, NV> resid_in(p.resid, p.ld_resid);
     const Input<uint16_t, V, NV> u_in(p.u, p.ld_u), gate_in(p.gate, p.ld_gate);
+    Ahead ahead{};
+    if (p.D >= 2048u) {
+        if (team.rank == 0 && p.resid) ahead.use(resid_in, p.D);
+        if (team.rank == 1 && p.u) ahead.use(u_in, p.D);
+        if (GATE && team.rank == 2 && p.gate_rows == 1) ahead.use(gate_in, p.D);
+    }
     for (uint64_t row = team.index; row < p.T; row += team.count) {
         const uint32_t t = (uint32_t)row;
         Raw<R, V> resid[NV];
@@ -296,6 +319,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) forward_kernel(const Forward p,
         u_in.load(u, t, team, p.D);
         resid_in.load(resid, t, team, p.D);
         if constexpr (GATE) gate_in.load(gate, p.gate_rows == 1 ? t : t / p.gate_rows, team, p.D);
+        if (ahead.bytes && row + team.count < p.T) ahead((uint32_t)(row + team.count));
         constexpr int kPairs = V * NV / 2;
         float k = p.scale;
         if (p.post) {
@@ -396,6 +420,15 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
 template <class R, int V, int NV, int THREADS, int GATE>
 __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, const TeamPlan plan) {
     constexpr int kPairs = V * NV / 2;
+    // The next row in registers where those suffice (4096 x 4096, bf16 in
+    // vectors: 59 us with, 69 without), else towards L2 only (fp32: 102 and 81
+    // us; 4000 x 4095 one by one: 162 and 102).
+    constexpr bool kRowAhead = sizeof(R) == 2 && (V == 8 || (V == 2 && !GATE));
+    // Rows asked for from L2.  Beside the row in registers it pays where a row
+    // takes a cluster (2000 x 8192 84 and 75 us), elsewhere it costs registers
+    // (16384 x 4096 without gates 168 and 178 us).
+    constexpr bool kAhead = !kRowAhead || GATE;
+    constexpr uint32_t kAheadBy = kRowAhead ? 3u : 2u, kAheadMin = kRowAhead ? 4097u : 256u;
     __shared__ float shared[2 * Team::kSumFloats];
     __shared__ float2 post_sum[GATE ? 1 : kPairs * THREADS];  // dw_post of the gate rows done, a slot for each thread
     Team team = team_of(plan, shared);
@@ -436,6 +469,19 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
     const float* const rstd_pre = p.dy ? p.rstd_pre : reinterpret_cast<const float*>(g_zeros);
     const float* const rstd_post = post ? p.rstd_post : &g_one;
     const uint32_t pre_step = p.dy ? 1u : 0u, post_step = post ? 1u : 0u;
+    // In shared memory: registers for it would spill others.
+    __shared__ Ahead ahead[5];
+    if (kAhead && threadIdx.x < 5u) {
+        Ahead a{};
+        if (p.D >= kAheadMin && team.rank < 5u) {
+            if (threadIdx.x == 0 && p.dy) a.use(dy_in, p.D);
+            if (threadIdx.x == 1 && p.dy) a.use(h_in, p.D);
+            if (threadIdx.x == 2 && p.u) a.use(u_in, p.D);
+            if (threadIdx.x == 3 && p.dh) a.use(dh_in, p.D);
+            if (GATE && threadIdx.x == 4) a.use(gate_in, p.D);
+        }
+        ahead[threadIdx.x] = a;
+    }
     auto fetch = [&](Row& x, uint32_t t) {
         dy_in.load(x.dy, t, team, p.D);
         h_in.load(x.h, t, team, p.D);
@@ -485,9 +531,9 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
     };
     // One token: x is its row, which arrived while the one before was worked
-    // on; the next one goes to `ahead`.
-    auto step = [&](const Row& x, Row& ahead, uint32_t t) {
-        if (t + 1u < t1) fetch(ahead, t + 1u);
+    // on; the one after it goes to `next`.
+    auto step = [&](const Row& x, Row& next, uint32_t t) {
+        if (kRowAhead && t + 1u < t1) fetch(next, t + 1u);
         // c1 = mean(a hhat) and c2 = mean(dp pv), dp = k (dh + rh (a - hhat c1))
         // with k = scale act: one round of sums, c2 = ru (S1 - c1 rh S2).
         const float ks = p.scale * x.ru;
@@ -535,6 +581,10 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
         store_row<V, NV>(p.dresid ? static_cast<R*>(p.dresid) + (uint64_t)t * (uint32_t)p.ld_dresid : nullptr, e, team,
                          p.D);
         store_row<V, NV>(p.du ? p.du + (uint64_t)t * (uint32_t)p.ld_du : nullptr, hh, team, p.D);
+        if (kAhead && threadIdx.x < 5u && t + kAheadBy < t1) {
+            const Ahead a = ahead[threadIdx.x];
+            if (a.bytes) a(t + kAheadBy);
+        }
         if constexpr (GATE) {
             if (p.dgate) store_row<V, NV>(p.dgate + (uint64_t)t * (uint32_t)p.ld_dgate, dgate, team, p.D);
         } else if (--gate_left == 0u) {
@@ -546,13 +596,15 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
     };
     if (t0 < t1) {
         Row a, b;
-        fetch(a, t0);
+        if (kRowAhead) fetch(a, t0);
         if constexpr (!GATE) {
             if (p.gate) gate_row = t0 / p.gate_rows, gate_left = p.gate_rows - t0 % p.gate_rows;
             start_gate();
         }
         for (uint32_t t = t0; t < t1; t += 2u) {
+            if (!kRowAhead) fetch(a, t);
             step(a, b, t);
+            if (!kRowAhead && t + 1u < t1) fetch(b, t + 1u);
             if (t + 1u < t1) step(b, a, t + 1u);
         }
         if constexpr (!GATE)
