@@ -422,10 +422,14 @@ FOIL_API int foil_w4_dequantize_tiles_dev(const void* packed, uint16_t* tiles, u
                                           uint32_t group, int32_t zeros, int32_t transpose, void* stream);
 
 /* y (M x N) = relu?(x (M x K) . W + bias) for a few rows, M from 1 to 64:
- * one pass over the 4-bit weights for every 16 rows (longer inputs: dequantise
- * and use foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or
- * NULL.  fp32 accumulation of unrounded weights, one rounding to bf16 at the
- * end.  M = 0 or N = 0 does nothing. */
+ * one pass over the 4-bit weights for up to 16 rows, and for up to 64 if x is
+ * 16-byte aligned and ld_x a multiple of 8 (longer inputs: dequantise and use
+ * foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or NULL.  fp32
+ * accumulation of unrounded weights, one rounding to bf16 at the end.  An
+ * infinity or NaN in a row of x makes that row's outputs infinite or NaN.  With
+ * more than 16 rows the sums of (q - z) x over a group are fp32 numbers before
+ * their scale: keep |x| between 2^-100 and 2^116 there (smaller values lose
+ * bits, sums of larger ones overflow).  M = 0 or N = 0 does nothing. */
 FOIL_API int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* packed, const uint16_t* bias,
                                 uint16_t* y, uint64_t ld_y, uint32_t M, uint32_t K, uint32_t N,
                                 uint32_t group, int32_t zeros, int32_t relu, void* stream);

@@ -174,6 +174,62 @@ def test_matvec_non_finite_rows_stay_apart():
     assert torch.isnan(y1[1]).all() and not torch.isfinite(y1[3]).any()
 
 
+# More than 16 rows, x in whole 16-byte pieces: one block of k and many, its
+# second half without values, columns past the last tile, splits of K.
+@pytest.mark.parametrize("group,zeros", [(32, False), (32, True), (64, False), (64, True), (128, False), (128, True)])
+@pytest.mark.parametrize("M,K,N", [(17, 8, 1), (64, 64, 16), (31, 72, 127), (33, 128, 128), (48, 136, 129), (32, 1024, 300),
+                                   (63, 1928, 40), (64, 4104, 1000), (18, 8192, 260), (50, 16384, 130)])
+def test_matvec_batches(M, K, N, group, zeros):
+    check_matvec(M, K, N, group, zeros, bias=N % 2 == 1, relu=K % 16 == 8, seed=M + K + N)
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 32768, 520), (64, 2048, 40000), (64, 256, 100000), (33, 4096, 4096)])
+def test_matvec_large_batches(M, K, N):
+    check_matvec(M, K, N, 64, True, bias=True, relu=False, seed=K)
+
+
+@pytest.mark.parametrize("x_off,ld_x,y_off,ld_y", [(8, 520, 3, 0), (16, 528, 0, 131), (0, 536, 5, 133)])
+@pytest.mark.parametrize("M", [20, 64])
+def test_matvec_batch_strides(M, x_off, ld_x, y_off, ld_y):
+    check_matvec(M, 515, 129, 64, True, bias=True, relu=False, x_off=x_off, ld_x=ld_x, y_off=y_off, ld_y=ld_y)
+
+
+def test_matvec_batch_rows_stand_alone_and_repeat():
+    """An infinity or a NaN stays in its row; the others' bits, and those of a
+    replayed graph, are the same; nor do weights past K and N matter."""
+    g = gen(11)
+    M, K, N, group = 50, 1000, 200, 64
+    codes, scales, zp = make_weights(g, K, N, group, True)
+    x = randn(g, M, K)
+    packed = pack(codes, scales, zp, group)
+    y = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(x.cuda(), packed, y, M, K, N, group, zeros=True)
+    bad = x.clone()
+    bad[3, 17], bad[40, 999] = float("nan"), float("inf")
+    xs, yb = bad.cuda(), torch.empty_like(y)
+    tf.w4_matvec(xs, packed, yb, M, K, N, group, zeros=True)
+    keep = [i for i in range(M) if i not in (3, 40)]
+    assert torch.equal(y[keep].view(torch.int16), yb[keep].view(torch.int16))
+    assert torch.isnan(yb[3]).all() and not torch.isfinite(yb[40]).any()
+    graph = torch.cuda.CUDAGraph()
+    again = torch.empty_like(y)
+    with torch.cuda.graph(graph):
+        for _ in range(3):
+            tf.w4_matvec(xs, packed, again, M, K, N, group, zeros=True)
+    xs.copy_(x)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y.view(torch.int16), again.view(torch.int16))
+    Kp, Np = 1024, 208
+    full_c = torch.randint(0, 16, (Np, Kp), generator=g, dtype=torch.uint8)
+    full_s = randn(g, Np, Kp // group, std=3.0)
+    full_z = torch.randint(0, 16, (Np, Kp // group), generator=g, dtype=torch.uint8)
+    full_c[:N, :K], full_s[:N, :scales.shape[1]], full_z[:N, :zp.shape[1]] = codes, scales, zp
+    tf.w4_matvec(x.cuda(), pack(full_c, full_s, full_z, group), again, M, K, N, group, zeros=True)
+    assert torch.equal(y.view(torch.int16), again.view(torch.int16))
+    assert tf.device_error() == 0
+
+
 @pytest.mark.parametrize("M,K,group,zeros", [(8, 300, 64, True), (13, 4200, 128, False), (16, 20000, 32, True)])
 def test_matvec_rows_of_very_different_size(M, K, group, zeros):
     """Rows scaled by powers of two from 2^-118 to 2^100: each within its own bound,

@@ -141,7 +141,7 @@ extern "C" int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* 
         const Span sx = matrix(what, x, ld_x, M, K, 2), sy = matrix(what, y, ld_y, M, N, 2);
         disjoint(what, {sy}, {sx, Span(packed, foil::w4::packed_bytes(w)), Span(bias, 2ull * N)});
         launched(what, foil::w4::matvec(x, ld_x, (const uint8_t*)packed, bias, y, ld_y, M, w, relu != 0,
-                                        (cudaStream_t)stream));
+                                        M > foil::w4::kWarpRows ? foil_error_word() : nullptr, (cudaStream_t)stream));
     });
 }
 
