@@ -874,11 +874,9 @@ static bool plan_matvec(Matvec& p, uint32_t bytes, uint32_t group, uint32_t sms)
 
 cudaError_t matvec(const uint16_t* x, uint64_t ld_x, const uint8_t* packed, const uint16_t* bias, uint16_t* y,
                    uint64_t ld_y, uint32_t M, const Weights& w, bool relu, uint32_t* err, cudaStream_t s) {
-    // More rows than two MMAs take: on tcgen05, which reads x in 16-byte pieces.
-    // Up to 32 rows two passes here are as fast where there are many weights
-    // (32 rows of 4096 x 8192: 19 us here, 15 there; of 8192 x 8192 29 and 26; of 8192 x
-    // 24576 61 and 75).
-    if (M > kWarpRows && (M > 32 || (uint64_t)w.K * w.N <= 1u << 25) && (uintptr_t)x % 16 == 0 && ld_x % 8 == 0)
+    // More rows than two of the warps' MMAs take: on tcgen05, which reads x in
+    // 16-byte pieces (32 rows of 4096 x 4096: 15 us in two passes here, 9 there).
+    if (M > kWarpRows && (uintptr_t)x % 16 == 0 && ld_x % 8 == 0)
         return matvec_batch(x, ld_x, packed, bias, y, ld_y, M, w, relu, err, s);
     Matvec p{};
     p.x = x, p.packed = packed, p.bias = bias, p.y = y, p.ld_x = ld_x, p.ld_y = ld_y, p.M = M, p.K = w.K, p.N = w.N;

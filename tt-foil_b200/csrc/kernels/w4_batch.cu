@@ -21,13 +21,14 @@
 //    order.  Two CTAs share an SM, so one's start and join overlap the other's
 //    products.
 //
-// 64 rows, us (the warps' MMAs): 4096 x 4096 13 (29), 16384 x 4096 35 (67),
-// 8192 x 24576 85 (118), 8192 x 65536 180 (282).  Bound by the instructions of
-// the conversion (310 a storage block, a quarter of them waits, copies and
-// barriers) and shared memory, where a block's 1 KB of codes is written and read
-// as 4 KB.  Tried: the weights' operand in TMEM instead, x by 4-byte copies in
-// the order of the weights' fragments: 87 to 99 us for 8192 x 24576; one CTA of 16
-// warps and 256 columns: 84, but 17 for 4096 x 4096.
+// 64 rows, us (the warps' MMAs): 4096 x 4096 11 (29), 16384 x 4096 26 (67),
+// 8192 x 24576 68 (117), 8192 x 65536 143 (280); 32 rows: 9 (15), 21 (34), 61 (60).
+// Bound by the instructions of the conversion (some 350 a storage block, of which
+// 130 make the operand and 40 add its products) and by shared memory, where a
+// block's 1 KB of codes is written and read as 4 KB.  Tried, for 64 rows of 8192 x
+// 24576 at a time when this took 85: the weights' operand in TMEM instead, x by
+// 4-byte copies in the order of the weights' fragments: 87 to 99; one CTA of 16
+// warps and 256 columns: 84, but 17 against 14 for 4096 x 4096.
 #include "w4.cuh"
 
 #include <cuda.h>
@@ -82,6 +83,37 @@ __device__ __forceinline__ void tmem_ld8(uint32_t at, float* v) {
     for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
 }
 
+// Shared memory by its own addresses (from generic ones: more instructions).
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t ld_shared_u16(uint32_t at) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_shared_u8(uint32_t at) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+    return v;
+}
+
+// True in one lane of a converged warp, always the same.
+__device__ __forceinline__ bool elect() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "elect.sync _|p, 0xffffffff;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(one));
+    return one != 0;
+}
+
 __device__ __forceinline__ uint32_t word(const uint4& v, uint32_t i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
@@ -112,8 +144,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     __shared__ volatile uint32_t abort_flag;
     uint8_t* const smem =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* const rings = smem + kStages * kStageBytes;
-    uint16_t* const scales = reinterpret_cast<uint16_t*>(rings + kWorkers * kRing * kBytes);
+    const uint32_t stages = smem_u32(smem), rings = stages + kStages * kStageBytes;
+    const uint32_t scales = rings + kWorkers * kRing * kBytes;
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
     const uint32_t rank = blockIdx.x % p.S, n0 = blockIdx.x / p.S * kColumns, m0 = blockIdx.y * MT;
     const uint32_t kb0 = rank * p.kb_each + min(rank, p.kb_more), nkb = p.kb_each + (rank < p.kb_more ? 1u : 0u);
@@ -152,19 +184,24 @@ __global__ void __launch_bounds__(kThreads, 2)
     // Workers: the thread's column of the CTA's, its first row of x.
     const uint32_t column = warp % 4u * 32u + lane, row0 = warp / 4u * kAcc;
     auto wait = [&](uint64_t* bar, uint32_t parity) {
+        // Most waits are short: without the clock and its instructions at first.
+        if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if (mbar_try_wait_sleep(bar, parity)) return true;
         return mbar_wait(bar, parity, &abort_flag, p.err, p.wait_ns);
     };
 
     if (warp < kWorkers) {
         const uint32_t g = lane / 4u, t = lane % 4u;
-        uint8_t* const ring = rings + warp * kRing * kBytes;
+        const uint32_t ring = rings + warp * kRing * kBytes;
         // Past the last tile: that one once more, not stored.
         const uint32_t tile = min(n0 / kBlockN + warp, p.tiles - 1u);
         const uint8_t* src = p.packed + ((uint64_t)tile * p.kb + kb0) * kBytes + lane * 16u;
         uint32_t left = nkb;
-        auto issue = [&](uint8_t* slot) {
+        auto issue = [&](uint32_t slot) {
             if (left) {
-                const uint32_t dst = smem_u32(slot) + lane * 16u;
+                const uint32_t dst = slot + lane * 16u;
                 cp_async16(dst, src, 16);
                 cp_async16(dst + 512u, src + 512, 16);
                 if (lane < (kBytes - kCodeBytes) / 16u) cp_async16(dst + kCodeBytes, src + kCodeBytes, 16);
@@ -181,7 +218,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             wait(&d_full[u % kUnits], u / kUnits & 1u);
             __syncwarp();
             tc_fence_after();
-            const float s = bf16_bits_to_f32(scales[(b % kScaleSlots * kGroups + gi) * kColumns + column]);
+            const float s = bf16_bits_to_f32(ld_shared_u16(scales + (b % kScaleSlots * kGroups + gi) * (kColumns * 2u) + column * 2u));
             const uint32_t at = tmem + (warp % 4u * 32u << 16) + u % kUnits * MT + row0;
             constexpr int kLoad = kAcc < 16 ? kAcc : 16;
 #pragma unroll
@@ -197,10 +234,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
                 }
 #pragma unroll
-                for (int i = 0; i < kLoad; i += 2) {
-                    const float2 sum = fma2(both(s), make_float2(v[i], v[i + 1]), make_float2(acc[c + i], acc[c + i + 1]));
-                    acc[c + i] = sum.x, acc[c + i + 1] = sum.y;
-                }
+                for (int i = 0; i < kLoad; ++i) acc[c + i] = fmaf(s, v[i], acc[c + i]);
             }
             tc_fence_before();
             __syncwarp();
@@ -221,50 +255,50 @@ __global__ void __launch_bounds__(kThreads, 2)
         // Odd columns take each two words in the other order, so that eight
         // lanes' 16-byte stores fall on distinct banks.
         const uint32_t odd = g & 1u;
-        uint8_t* slot = ring;
+        uint32_t eight;  // 16 + 8 twice, in one register for good
+        asm volatile("mov.b32 %0, 0x41c041c0;" : "=r"(eight));
+        uint32_t slot = ring;
         uint32_t stage = 0, phase = 1;  // phase of the stage's previous round
         for (uint32_t b = 0; b < nkb; ++b) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
             __syncwarp();  // every lane's copies have landed
-            const uint4 a4 = *reinterpret_cast<const uint4*>(slot + lane * 16u);
-            const uint4 c4 = *reinterpret_cast<const uint4*>(slot + 512u + lane * 16u);
+            const uint4 a4 = ld_shared_v4(slot + lane * 16u), c4 = ld_shared_v4(slot + 512u + lane * 16u);
             uint32_t za[ZEROS ? kGroups : 1], zb[ZEROS ? kGroups : 1];
             if constexpr (ZEROS) {
-                const uint8_t* z = slot + kCodeBytes + 32u * kGroups;
+                const uint32_t z = slot + kCodeBytes + 32u * kGroups;
 #pragma unroll
                 for (uint32_t i = 0; i < kGroups; ++i) {
                     const uint32_t at = (GROUP == 32 ? i ^ odd : i) * 16u + g;
-                    za[i] = 0x41804180u | (z[at] & 15u) * 0x00080008u;
-                    zb[i] = 0x41804180u | (z[at + 8u] & 15u) * 0x00080008u;
+                    za[i] = 0x41804180u | (ld_shared_u8(z + at) & 15u) * 0x00080008u;
+                    zb[i] = 0x41804180u | (ld_shared_u8(z + at + 8u) & 15u) * 0x00080008u;
                 }
             }
             if (lane < 2u * kGroups)  // 8 scales a lane
-                *reinterpret_cast<uint4*>(scales + (b % kScaleSlots * kGroups + lane / 2u) * kColumns + warp * 16u +
-                                          lane % 2u * 8u) =
-                    *reinterpret_cast<const uint4*>(slot + kCodeBytes + lane * 16u);
+                st_shared_v4(scales + (b % kScaleSlots * kGroups + lane / 2u) * (kColumns * 2u) + warp * 32u +
+                                 lane % 2u * 16u,
+                             ld_shared_v4(slot + kCodeBytes + lane * 16u));
             __syncwarp();  // every lane has read the slot
             issue(slot);
             slot = slot + kBytes == ring + kRing * kBytes ? ring : slot + kBytes;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
                 if (2u * b + h >= kStages) wait(&empty[stage], phase);
+                __syncwarp();
                 // 64 k of 128 rows in the 128-byte swizzle.
-                uint8_t* const rows = smem + stage * kStageBytes + warp * 2048u + g * 128u;
+                const uint32_t rows = stages + stage * kStageBytes + warp * 2048u + g * 128u;
                 const uint32_t at0 = ((odd * 4u + t) ^ g) * 16u;  // of the first word written; the other: 64 bytes off
 #pragma unroll
                 for (uint32_t s = 2 * h; s < 2 * h + 2; ++s) {
                     // Word s, or s ^ 1 in odd columns.
                     const uint32_t a = odd ? word(a4, s ^ 1u) : word(a4, s), c = odd ? word(c4, s ^ 1u) : word(c4, s);
                     const uint32_t gi = s * 32 / GROUP;
-                    const uint32_t z0 = ZEROS ? za[ZEROS ? gi : 0] : 0x41c041c0u, z1 = ZEROS ? zb[ZEROS ? gi : 0] : 0x41c041c0u;
-                    uint8_t* const to = rows + (at0 ^ s % 2u * 64u);
-                    *reinterpret_cast<uint4*>(to) =
-                        make_uint4(difference<0>(a, z0), difference<1>(a, z0), difference<2>(a, z0), difference<3>(a, z0));
-                    *reinterpret_cast<uint4*>(to + 1024u) =
-                        make_uint4(difference<0>(c, z1), difference<1>(c, z1), difference<2>(c, z1), difference<3>(c, z1));
+                    const uint32_t z0 = ZEROS ? za[ZEROS ? gi : 0] : eight, z1 = ZEROS ? zb[ZEROS ? gi : 0] : eight;
+                    const uint32_t to = rows + (at0 ^ s % 2u * 64u);
+                    st_shared_v4(to, make_uint4(difference<0>(a, z0), difference<1>(a, z0), difference<2>(a, z0),
+                                                difference<3>(a, z0)));
+                    st_shared_v4(to + 1024u, make_uint4(difference<0>(c, z1), difference<1>(c, z1),
+                                                        difference<2>(c, z1), difference<3>(c, z1)));
                 }
-                // Written by the generic proxy, read by the MMA's.
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&full[stage]);
                 if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -275,31 +309,41 @@ __global__ void __launch_bounds__(kThreads, 2)
         take_half(nkb - 1u, 1u);
         asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (warp == kMmaWarp) {
-        if (lane == 0) {
-            constexpr uint64_t kmaj = smem_desc_sw128_kmajor();
-            uint32_t stage = 0, phase = 0;
-            bool ok = true;
-            for (uint32_t b = 0; b < nkb && ok; ++b) {
+        // One lane of the warp issues; all wait, so that the others' way is the same.
+        const bool one = elect();
+        constexpr uint64_t kmaj = smem_desc_sw128_kmajor();
+        uint32_t stage = 0, phase = 0;
+        bool ok = true;
+        for (uint32_t b = 0; b < nkb && ok; ++b) {
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    ok = ok && wait(&full[stage], phase) && wait(&x_full[stage], phase);
-                    if (!ok) break;
-                    const uint32_t w_at = smem_u32(smem + stage * kStageBytes) >> 4, x_at = w_at + (kWBytes >> 4);
-                    const uint64_t w_desc = kmaj | (uint64_t)(w_at & 0x3fffu), x_desc = kmaj | (uint64_t)(x_at & 0x3fffu);
+            for (uint32_t h = 0; h < 2; ++h) {
+                ok = ok && wait(&full[stage], phase) && wait(&x_full[stage], phase);
+                // W was written by the generic proxy, the MMA reads through the async
+                // one.  (A fence by every writer: 75 us instead of 68, 64 rows of 8192 x 24576.)
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                const uint32_t w_at = stages + stage * kStageBytes >> 4, x_at = w_at + (kWBytes >> 4);
+                const uint64_t w_desc = kmaj | (uint64_t)(w_at & 0x3fffu), x_desc = kmaj | (uint64_t)(x_at & 0x3fffu);
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; ++k) {  // 16 k each
-                        const uint32_t in = (4 * h + k) % (GROUP / 16);  // the group
-                        const uint32_t u = b * kGroups + (4 * h + k) / (GROUP / 16);
-                        if (in == 0 && u >= kUnits) ok = ok && wait(&d_empty[u % kUnits], (u / kUnits - 1u) & 1u);
-                        if (in == 0 || k == 0) tc_fence_after();
-                        tc_mma(tmem + u % kUnits * MT, w_desc + k * 2u, x_desc + k * 2u, instruction(MT), in ? 1u : 0u);
-                        if (in == GROUP / 16 - 1) tc_commit(&d_full[u % kUnits]);
+                for (uint32_t k0 = 0; k0 < 4; k0 += GROUP == 32 ? 2 : 4) {  // 16 k each
+                    const uint32_t in = (4 * h + k0) % (GROUP / 16);  // the group
+                    const uint32_t u = b * kGroups + (4 * h + k0) / (GROUP / 16);
+                    if (in == 0 && u >= kUnits) ok = ok && wait(&d_empty[u % kUnits], (u / kUnits - 1u) & 1u);
+                    ok = __all_sync(0xffffffffu, ok);
+                    tc_fence_after();
+                    if (one && ok) {
+#pragma unroll
+                        for (uint32_t k = k0; k < k0 + (GROUP == 32 ? 2 : 4); ++k)
+                            tc_mma(tmem + u % kUnits * MT, w_desc + k * 2u, x_desc + k * 2u, instruction(MT),
+                                   in == 0 && k == k0 ? 0u : 1u);
+                        if (GROUP < 128 || h == 1) tc_commit(&d_full[u % kUnits]);
+                        if (k0 + (GROUP == 32 ? 2 : 4) == 4) tc_commit(&empty[stage]);
                     }
-                    tc_commit(&empty[stage]);
-                    if (++stage == kStages) stage = 0, phase ^= 1u;
                 }
+                if (++stage == kStages) stage = 0, phase ^= 1u;
             }
-            // Every MMA of this thread ends before TMEM is released.
+        }
+        // Every MMA ends before TMEM is released.
+        if (one) {
             tc_commit(&drain);
             mbar_drain(&drain, 0, 100000000ull);
         }
@@ -308,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (; i < 2u * nkb; ++i) {
             if (i >= kStages && !wait(&empty[stage], phase)) break;
             mbar_expect_tx(&x_full[stage], MT * 128u);
-            tma_load_2d(smem_u32(smem + stage * kStageBytes + kWBytes), &map_x, (int32_t)(kb0 * kBlockK + i * 64u),
+            tma_load_2d(stages + stage * kStageBytes + kWBytes, &map_x, (int32_t)(kb0 * kBlockK + i * 64u),
                         (int32_t)m0, &x_full[stage]);
             if (++stage == kStages) stage = 0, phase ^= 1u;
         }
@@ -381,10 +425,10 @@ PFN_cuTensorMapEncodeTiled encoder() {
 }
 
 // CTAs that share K: the least estimated time, in us, two CTAs on an SM.  A CTA
-// takes 1.0 a block of k alone and 1.47 beside another, 2 to begin and end, and
-// 0.3 for each part to join (64 rows).  (64 rows of 4096 x 4096: 35, 21, 13 and 15
-// us with 1, 2, 4 and 8; of 8192 x 24576: 98, 85, 86, 101; estimates within a
-// quarter.)
+// takes 0.8 a block of k alone and 1.15 beside another, 2 to begin and end, and
+// 0.3 for each part to join (64 rows).  (64 rows of 4096 x 4096: 28, 17, 11 and 11
+// us with 1, 2, 4 and 8; of 8192 x 24576: 76, 67, 68, 84; estimates within a
+// fifth.)
 uint32_t split(uint32_t tiles, uint32_t kb, uint32_t mt) {
     const uint32_t sms = (uint32_t)foil_sm_count();
     uint32_t best = 1;
@@ -392,8 +436,8 @@ uint32_t split(uint32_t tiles, uint32_t kb, uint32_t mt) {
     for (uint32_t S = 1; S <= 8 && S <= kb; S *= 2) {
         const uint32_t blocks = (kb + S - 1) / S, ctas = tiles * S, last = ctas % (2 * sms);
         const float join = 2.0f + (S > 1 ? 0.3f * S * mt / 64 : 0.0f);
-        float t = (float)(ctas / (2 * sms)) * (join + 1.47f * blocks);
-        if (last) t += join + (last > sms ? 1.47f : 1.0f) * blocks;
+        float t = (float)(ctas / (2 * sms)) * (join + 1.15f * blocks);
+        if (last) t += join + (last > sms ? 1.15f : 0.8f) * blocks;
         if (S == 1 || t < least) best = S, least = t;
     }
     return best;
