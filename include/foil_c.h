@@ -372,11 +372,11 @@ FOIL_API int foil_matmul_tiles_noalloc_dev(const uint16_t* a, const uint16_t* b,
 /* Token-path operators: products of a few rows with 4-bit weights, the norms */
 /* around a residual block, embedding rows, and their gradients.  Row-major   */
 /* tensors (not tile streams) unless an argument says "tiles".  A row stride  */
-/* `ld_*` is in elements, 0 = dense.  Outputs must not overlap inputs or each */
-/* other except where stated (FOIL_ERR_INVALID).  No counterpart in the       */
-/* reference; their numeric types are its bf16 and fp32.  Like the other      */
-/* entry points, the first call on a device may allocate its error word: make */
-/* it before any stream capture.                                              */
+/* `ld_*` is in elements, below 2^32, 0 = dense.  Outputs must not overlap    */
+/* inputs or each other except where stated (FOIL_ERR_INVALID).  No           */
+/* counterpart in the reference; their numeric types are its bf16 and fp32.   */
+/* Like the other entry points, the first call on a device may allocate its   */
+/* error word: make it before any stream capture.                             */
 /* ------------------------------------------------------------------------ */
 
 /* 4-bit weights.  A weight matrix W (K x N, the B operand of the products
@@ -435,8 +435,8 @@ FOIL_API int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* pa
                                 uint32_t group, int32_t zeros, int32_t relu, void* stream);
 
 /* The norms after one block and before the next, fused with the block's gate,
- * its scale and the residual addition, for T tokens of D channels (D at most
- * 16384), N(v) = v / sqrt(mean(v^2) + eps):
+ * its scale and the residual addition, for T tokens of D channels (T at most
+ * 2^31, D at most 16384), N(v) = v / sqrt(mean(v^2) + eps):
  *
  *   p = post ? N(u) * w_post : u          the block's output u
  *   h = resid + scale * act(gate) * p     the residual stream
@@ -483,7 +483,7 @@ FOIL_API int foil_block_norm_grad_dev(const void* dh, uint64_t ld_dh, const uint
  * into a table of V rows of D bf16; out: bf16, or fp32 if `fp32` is non-zero.
  * A row whose id equals pad_id becomes zeros; so does one whose id is outside
  * 0 .. V - 1, which also sets FOIL_DEVERR_BAD_INDEX in the device error word.
- * V and T at most 2^24. */
+ * V and T at most 2^24, D at most 2^20 (here and in the gradient). */
 FOIL_API int foil_embed_rows_dev(const void* ids, int32_t id_bytes, const uint16_t* table, uint64_t ld_table,
                                  void* out, uint64_t ld_out, uint32_t T, uint32_t V, uint32_t D,
                                  int32_t fp32, float scale, int64_t pad_id, void* stream);

@@ -191,6 +191,19 @@ def test_embed_rows_refusals(L):
     assert grad(V=0) == 0 and grad(D=0) == 0
 
 
+def test_counts_that_32_bits_could_not_hold(L):
+    many = (1 << 31) + 1
+    refused(L, L.foil_block_norm_dev(*forward_args(T=many)), "2^31")
+    refused(L, L.foil_block_norm_grad_dev(*backward_args(T=many)), "2^31")
+    wide = (1 << 20) + 1
+    refused(L, L.foil_embed_rows_dev(at(0), 4, at(1), 0, at(2), 0, 1, 1, wide, 0, 1.0, -1, None), "2^20")
+    refused(L, L.foil_embed_rows_grad_dev(at(0), 4, at(2), 0, at(1), 0, 1, 1, wide, 0, 1.0, -1, 0, at(3), 1 << 40,
+                                          None), "2^20")
+    far = 1 << 32
+    refused(L, L.foil_block_norm_dev(*forward_args(ld_u=far)), "too large")
+    refused(L, L.foil_embed_rows_dev(at(0), 4, at(1), far, at(2), 0, 1, 1, 64, 0, 1.0, -1, None), "too large")
+
+
 def test_binding_refuses_tensors_it_cannot_describe():
     import torch
     import ttfoil

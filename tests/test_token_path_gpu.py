@@ -230,6 +230,35 @@ def test_matvec_batch_rows_stand_alone_and_repeat():
     assert tf.device_error() == 0
 
 
+def test_matvec_batches_at_once_and_between_other_products():
+    """Calls on two streams at once, and in line with the tile product, which
+    holds tensor memory too: the bits of a call by itself."""
+    g = gen(23)
+    M, K, N, group = 64, 2048, 4096, 128
+    codes, scales, _ = make_weights(g, K, N, group, False)
+    packed = pack(codes, scales, None, group)
+    x = randn(g, M, K).cuda()
+    alone = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(x, packed, alone, M, K, N, group)
+    a, b = tile(randn(g, 256, 512)).cuda(), tile(randn(g, 512, 256)).cuda()
+    ref = torch.empty(256 * 256, dtype=BF, device="cuda")
+    tf.matmul_tiles(a, b, ref, 8, 16, 8)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ys = [[torch.empty_like(alone) for _ in range(8)] for _ in streams]
+    cs = [torch.empty_like(ref) for _ in streams]
+    for i in range(8):
+        for s, y, c in zip(streams, ys, cs):
+            with torch.cuda.stream(s):
+                tf.w4_matvec(x, packed, y[i], M, K, N, group)
+                tf.matmul_tiles(a, b, c, 8, 16, 8)
+    torch.cuda.synchronize()
+    for y, c in zip(ys, cs):
+        assert all(torch.equal(v.view(torch.int16), alone.view(torch.int16)) for v in y)
+        assert torch.equal(c.view(torch.int16), ref.view(torch.int16))
+    assert tf.device_error() == 0
+
+
 @pytest.mark.parametrize("M,K,group,zeros", [(8, 300, 64, True), (13, 4200, 128, False), (16, 20000, 32, True)])
 def test_matvec_rows_of_very_different_size(M, K, group, zeros):
     """Rows scaled by powers of two from 2^-118 to 2^100: each within its own bound,

@@ -9,6 +9,7 @@ namespace foil {
 namespace norm {
 
 constexpr uint32_t kMaxD = 16384;
+constexpr uint32_t kMaxT = 1u << 31;  // tokens are counted in 32 bits
 
 struct Forward {
     const void* resid;

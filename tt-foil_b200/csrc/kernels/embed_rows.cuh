@@ -9,6 +9,7 @@ namespace foil {
 namespace embed {
 
 constexpr uint32_t kMaxRows = 1u << 24;  // T and V
+constexpr uint32_t kMaxD = 1u << 20;     // columns are counted in 32 bits, 16 Ki at a time
 
 struct Lookup {
     const void* ids;

@@ -1,6 +1,6 @@
 // C-ABI of the token-path operators (include/foil_c.h): argument checks, then
-// the launchers of kernels/w4.cu, kernels/block_norm.cu and
-// kernels/embed_rows.cu.
+// the launchers of kernels/w4.cu, kernels/w4_batch.cu, kernels/block_norm.cu
+// and kernels/embed_rows.cu.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -155,6 +155,7 @@ extern "C" int foil_block_norm_dev(const void* resid, uint64_t ld_resid, const u
     return guarded([&] {
         if (T == 0 || D == 0) return;
         if (D > foil::norm::kMaxD) invalid(what, "D must be at most 16384");
+        if (T > foil::norm::kMaxT) invalid(what, "T must be at most 2^31");
         if (!resid || (!h && !y)) invalid(what, "null pointer");
         if (!u && (post || w_post || gate || rstd_post)) invalid(what, "post norm or gate without the block's output");
         if (!post && (w_post || rstd_post)) invalid(what, "w_post or rstd_post without the post norm");
@@ -202,6 +203,7 @@ extern "C" int foil_block_norm_grad_dev(const void* dh, uint64_t ld_dh, const ui
     return guarded([&] {
         if (D == 0) return;
         if (D > foil::norm::kMaxD) invalid(what, "D must be at most 16384");
+        if (T > foil::norm::kMaxT) invalid(what, "T must be at most 2^31");
         if (!dresid && !du && !dgate && !dw_post && !dw_pre) invalid(what, "no output is wanted");
         if (!dh && !dy && T) invalid(what, "dh and dy are both null");
         if (dy && T && (!h || !rstd_pre)) invalid(what, "dy needs h and rstd_pre");
@@ -239,9 +241,10 @@ extern "C" int foil_block_norm_grad_dev(const void* dh, uint64_t ld_dh, const ui
 
 // --------------------------------------------------------- embedding rows ---
 namespace {
-void check_ids(const char* what, const void* ids, int32_t id_bytes, uint32_t T, uint32_t V) {
+void check_ids(const char* what, const void* ids, int32_t id_bytes, uint32_t T, uint32_t V, uint32_t D) {
     if (id_bytes != 4 && id_bytes != 8) invalid(what, "id_bytes must be 4 or 8");
     if (T > foil::embed::kMaxRows || V > foil::embed::kMaxRows) invalid(what, "T and V must be at most 2^24");
+    if (D > foil::embed::kMaxD) invalid(what, "D must be at most 2^20");
     if (T && !ids) invalid(what, "null pointer");
     if ((uintptr_t)ids % (uint32_t)id_bytes) invalid(what, "misaligned pointer");
 }
@@ -253,7 +256,7 @@ extern "C" int foil_embed_rows_dev(const void* ids, int32_t id_bytes, const uint
     const char* what = "foil_embed_rows_dev";
     return guarded([&] {
         if (T == 0 || D == 0) return;
-        check_ids(what, ids, id_bytes, T, V);
+        check_ids(what, ids, id_bytes, T, V, D);
         if (!out || (V && !table)) invalid(what, "null pointer");
         const Span st = matrix(what, table, ld_table, V, D, 2), so = matrix(what, out, ld_out, T, D, fp32 ? 4 : 2);
         disjoint(what, {so}, {st, Span(ids, (uint64_t)T * id_bytes)});
@@ -276,7 +279,7 @@ extern "C" int foil_embed_rows_grad_dev(const void* ids, int32_t id_bytes, const
     const char* what = "foil_embed_rows_grad_dev";
     return guarded([&] {
         if (V == 0 || D == 0) return;
-        check_ids(what, ids, id_bytes, T, V);
+        check_ids(what, ids, id_bytes, T, V, D);
         if (!dtable || (T && !dout)) invalid(what, "null pointer");
         const uint64_t need = foil::embed::gradient_ws_bytes(T, V, D);
         if (ws_bytes < need || (need && !ws) || !aligned16(ws)) invalid(what, "workspace too small or misaligned");
