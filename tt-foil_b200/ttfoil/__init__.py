@@ -319,9 +319,22 @@ def conv2d_chw(x, w, bias, y, N, Cin, H, W, Cout, KH, KW, stride, pad, relu=Fals
 
 # ------------------------------------------------------ token-path operators ---
 
-def _current_device():
-    import torch
-    return torch.cuda.current_device()
+# Their kernels take a few microseconds, so the calls below look at a tensor as
+# little as they can.
+
+def _place(stream):
+    """The current device, and the handle of `stream` or of its current stream."""
+    global _place_of
+    if _place_of is None:
+        import torch
+        _place_of = torch.cuda.current_device, getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    device = _place_of[0]()
+    if stream is None and _place_of[1] is not None:
+        return device, _place_of[1](device)
+    return device, _stream(stream)
+
+
+_place_of = None
 
 
 def _vec(t, device):
@@ -335,29 +348,31 @@ def _vec(t, device):
     return t.data_ptr()
 
 
-def _mat(t, ld, device):
-    """Pointer and row stride in elements of a matrix: the stride as given, else
-    that of a 2-D torch tensor, else 0 (dense)."""
+def _mat(t, ld, device, cols=None):
+    """Pointer and row stride in elements of a matrix (of `cols` columns): the
+    stride as given, else that of a 2-D torch tensor, else 0 (dense)."""
     if t is None or isinstance(t, int):
         return t, ld
     if t.get_device() != device:
         raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
-    if not ld:
-        if t.dim() == 2:
-            rows, cols = t.shape
-            step, unit = t.stride()
-            if (cols > 1 and unit != 1) or (rows > 1 and step < cols):
-                raise FoilError(1, "tt-foil: rows of a tensor must be contiguous and must not overlap")
-            ld = step if rows > 1 else 0
-        elif not t.is_contiguous():
-            raise FoilError(1, "tt-foil: a tensor must be contiguous, or a matrix with a row stride")
-    return t.data_ptr(), ld
+    if ld:
+        return t.data_ptr(), ld
+    shape = t.shape
+    if t.is_contiguous() and (len(shape) != 2 or shape[1] == cols):
+        return t.data_ptr(), 0
+    if len(shape) != 2:
+        raise FoilError(1, "tt-foil: a tensor must be contiguous, or a matrix with a row stride")
+    rows, cols = shape
+    step, unit = t.stride()
+    if (cols > 1 and unit != 1) or (rows > 1 and step < cols):
+        raise FoilError(1, "tt-foil: rows of a tensor must be contiguous and must not overlap")
+    return t.data_ptr(), step if rows > 1 else 0
 
 
 def _is_fp32(fp32, *tensors):
     """The residual stream's type: as given, else from the first torch tensor (float32 or 16-bit)."""
     for t in tensors:
-        if t is not None and not isinstance(t, int):
+        if not (t is None or isinstance(t, int)):
             wide = t.element_size() == 4
             if fp32 is not None and bool(fp32) != wide:
                 raise FoilError(1, "tt-foil: tensors of one type are mixed with another")
@@ -373,33 +388,33 @@ def w4_packed_bytes(K, N, group, zeros=False):
 def w4_pack(codes, scales, packed, K, N, group, zero_points=None, stream=None):
     """Codes (N x K, one byte each), scales (N x ceil(K / group) bf16) and zero
     points (alike, one byte each, or None) -> 4-bit storage."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     check(lib().foil_w4_pack_dev(_vec(codes, dev), _vec(scales, dev), _vec(zero_points, dev), _vec(packed, dev), K, N,
-                                 group, _stream(stream)))
+                                 group, stream))
 
 
 def w4_quantize_tiles(tiles, packed, Kt, Nt, group, zeros=False, stream=None):
     """Tile stream of Kt x Nt tiles -> 4-bit storage with a scale (and, with
     `zeros`, a zero point) for each `group` values of a column."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     check(lib().foil_w4_quantize_tiles_dev(_vec(tiles, dev), _vec(packed, dev), Kt, Nt, group, 1 if zeros else 0,
-                                           _stream(stream)))
+                                           stream))
 
 
 def w4_dequantize_tiles(packed, tiles, K, N, group, zeros=False, transpose=False, stream=None):
     """4-bit storage -> tile stream of the weights, or of their transpose."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     check(lib().foil_w4_dequantize_tiles_dev(_vec(packed, dev), _vec(tiles, dev), K, N, group, 1 if zeros else 0,
-                                             1 if transpose else 0, _stream(stream)))
+                                             1 if transpose else 0, stream))
 
 
 def w4_matvec(x, packed, y, M, K, N, group, zeros=False, bias=None, relu=False, ld_x=0, ld_y=0, stream=None):
     """y (M x N) = relu?(x (M x K) . W + bias) with 4-bit W, M at most 64."""
-    dev = _current_device()
-    x, ld_x = _mat(x, ld_x, dev)
-    y, ld_y = _mat(y, ld_y, dev)
+    dev, stream = _place(stream)
+    x, ld_x = _mat(x, ld_x, dev, K)
+    y, ld_y = _mat(y, ld_y, dev, N)
     check(lib().foil_w4_matvec_dev(x, ld_x, _vec(packed, dev), _vec(bias, dev), y, ld_y, M, K, N, group,
-                                   1 if zeros else 0, 1 if relu else 0, _stream(stream)))
+                                   1 if zeros else 0, 1 if relu else 0, stream))
 
 
 GATE_ACTS = {"none": 0, "sigmoid": 1}
@@ -417,17 +432,17 @@ def block_norm(resid, u, h, y, T, D, w_pre=None, post=False, w_post=None, gate=N
     """h = resid + scale * act(gate) * (post ? N(u) * w_post : u);
     y = N(h) * w_pre, with N(v) = v / sqrt(mean(v^2) + eps).  resid and h are
     bf16 or fp32 (taken from the tensors; `fp32` for raw pointers)."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     wide = _is_fp32(fp32, resid, h)
-    resid, ld_resid = _mat(resid, ld_resid, dev)
-    u, ld_u = _mat(u, ld_u, dev)
-    gate, ld_gate = _mat(gate, ld_gate, dev)
-    h, ld_h = _mat(h, ld_h, dev)
-    y, ld_y = _mat(y, ld_y, dev)
+    resid, ld_resid = _mat(resid, ld_resid, dev, D)
+    u, ld_u = _mat(u, ld_u, dev, D)
+    gate, ld_gate = _mat(gate, ld_gate, dev, D)
+    h, ld_h = _mat(h, ld_h, dev, D)
+    y, ld_y = _mat(y, ld_y, dev, D)
     check(lib().foil_block_norm_dev(resid, ld_resid, u, ld_u, 1 if post else 0, _vec(w_post, dev), gate, ld_gate,
                                     gate_rows, _gate_act(gate_act), _vec(w_pre, dev), h, ld_h, y, ld_y,
                                     _vec(rstd_post, dev), _vec(rstd_pre, dev), T, D, wide, scale, eps,
-                                    _stream(stream)))
+                                    stream))
 
 
 def block_norm_grad_ws_bytes(T, D, gate_rows=0):
@@ -441,22 +456,22 @@ def block_norm_grad(dh, dy, h, u, dresid, du, T, D, ws, rstd_pre=None, w_pre=Non
                     ld_du=0, ld_dgate=0, stream=None):
     """Gradients of block_norm from those of h (dh) and y (dy); outputs that
     are None are not made.  `ws`: a workspace of block_norm_grad_ws_bytes."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     wide = _is_fp32(fp32, dh, h, dresid)
     n = _ws_bytes(ws, ws_bytes)
-    dh, ld_dh = _mat(dh, ld_dh, dev)
-    dy, ld_dy = _mat(dy, ld_dy, dev)
-    h, ld_h = _mat(h, ld_h, dev)
-    u, ld_u = _mat(u, ld_u, dev)
-    gate, ld_gate = _mat(gate, ld_gate, dev)
-    dresid, ld_dresid = _mat(dresid, ld_dresid, dev)
-    du, ld_du = _mat(du, ld_du, dev)
-    dgate, ld_dgate = _mat(dgate, ld_dgate, dev)
+    dh, ld_dh = _mat(dh, ld_dh, dev, D)
+    dy, ld_dy = _mat(dy, ld_dy, dev, D)
+    h, ld_h = _mat(h, ld_h, dev, D)
+    u, ld_u = _mat(u, ld_u, dev, D)
+    gate, ld_gate = _mat(gate, ld_gate, dev, D)
+    dresid, ld_dresid = _mat(dresid, ld_dresid, dev, D)
+    du, ld_du = _mat(du, ld_du, dev, D)
+    dgate, ld_dgate = _mat(dgate, ld_dgate, dev, D)
     check(lib().foil_block_norm_grad_dev(
         dh, ld_dh, dy, ld_dy, h, ld_h, _vec(rstd_pre, dev), _vec(w_pre, dev), u, ld_u, 1 if post else 0,
         _vec(rstd_post, dev), _vec(w_post, dev), gate, ld_gate, gate_rows, _gate_act(gate_act), dresid, ld_dresid,
         du, ld_du, dgate, ld_dgate, _vec(dw_post, dev), _vec(dw_pre, dev), _vec(ws, dev), n, T, D, wide, scale,
-        _stream(stream)))
+        stream))
 
 
 def _ws_bytes(ws, ws_bytes):
@@ -479,12 +494,12 @@ def embed_rows(ids, table, out, T, V, D, scale=1.0, pad_id=-1, id_bytes=4, fp32=
                stream=None):
     """out[t] = scale * table[ids[t]]; zeros where ids[t] is pad_id.  A bad id
     gives zeros and DEVERR_BAD_INDEX (see device_error)."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     id_bytes, wide = _id_bytes(ids, id_bytes), _is_fp32(fp32, out)
-    table, ld_table = _mat(table, ld_table, dev)
-    out, ld_out = _mat(out, ld_out, dev)
+    table, ld_table = _mat(table, ld_table, dev, D)
+    out, ld_out = _mat(out, ld_out, dev, D)
     check(lib().foil_embed_rows_dev(_vec(ids, dev), id_bytes, table, ld_table, out, ld_out, T, V, D, wide, scale, pad_id,
-                                    _stream(stream)))
+                                    stream))
 
 
 def embed_rows_grad_ws_bytes(T, V, D):
@@ -497,12 +512,12 @@ def embed_rows_grad(ids, dout, dtable, T, V, D, ws, scale=1.0, pad_id=-1, accumu
     """dtable[v] (fp32) = scale * sum of dout[t] over ids[t] = v, or with
     `accumulate` added to what is there.  `ws`: a workspace of
     embed_rows_grad_ws_bytes."""
-    dev = _current_device()
+    dev, stream = _place(stream)
     id_bytes, wide, n = _id_bytes(ids, id_bytes), _is_fp32(fp32, dout), _ws_bytes(ws, ws_bytes)
-    dout, ld_dout = _mat(dout, ld_dout, dev)
-    dtable, ld_dtable = _mat(dtable, ld_dtable, dev)
+    dout, ld_dout = _mat(dout, ld_dout, dev, D)
+    dtable, ld_dtable = _mat(dtable, ld_dtable, dev, D)
     check(lib().foil_embed_rows_grad_dev(_vec(ids, dev), id_bytes, dout, ld_dout, dtable, ld_dtable, T, V, D, wide,
-                                         scale, pad_id, 1 if accumulate else 0, _vec(ws, dev), n, _stream(stream)))
+                                         scale, pad_id, 1 if accumulate else 0, _vec(ws, dev), n, stream))
 
 
 def matmul_tiles_host(device, a, b, c, Mt, Kt, Nt, bias=None, relu=False, chunk_rows=0):
