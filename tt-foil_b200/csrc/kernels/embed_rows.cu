@@ -431,6 +431,7 @@ __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Pla
 // goes on; blockIdx.y: 256 columns.  8 warps take every eighth part, their sums
 // are added in order.
 constexpr uint32_t kJoinColumns = 256, kJoinRuns = 8;
+constexpr uint32_t kJoinAhead = 4;  // parts of a warp on their way
 
 __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Plan q) {
     __shared__ float part[kThreads / 32][kJoinColumns];
@@ -465,11 +466,19 @@ __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Pl
         const uint32_t id = ids[w], run = blockIdx.x * kJoinRuns + w, hi = ends[w];
         if (id == ~0u) continue;
         float s[kEach] = {};
-        for (uint32_t r = run + warp; r < hi; r += kThreads / 32u) {
-            const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
+        for (uint32_t r0 = run + warp; r0 < hi; r0 += kJoinAhead * (kThreads / 32u)) {
+            float v[kJoinAhead][kEach];
 #pragma unroll
-            for (int j = 0; j < kEach; ++j)
-                if (col + 32u * j < p.D) s[j] += row[32 * j];
+            for (uint32_t k = 0; k < kJoinAhead; ++k) {
+                const uint32_t r = r0 + k * (kThreads / 32u);
+                const float* row = (r == run ? q.tail : q.head) + (uint64_t)r * p.D + col;
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) v[k][j] = r < hi && col + 32u * j < p.D ? row[32 * j] : 0.0f;
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kJoinAhead; ++k)
+#pragma unroll
+                for (int j = 0; j < kEach; ++j) s[j] += v[k][j];
         }
 #pragma unroll
         for (int j = 0; j < kEach; ++j) part[warp][lane + 32 * j] = s[j];
@@ -544,7 +553,8 @@ cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
     w.use(p.dout, p.ld_dout, fp32 ? 4 : 2);
     e = fp32 ? sum_launch<float>(p, q, w.v, s) : sum_launch<uint16_t>(p, q, w.v, s);
     if (e != cudaSuccess || q.runs < 2) return e;
-    return launch(join_runs, dim3((q.runs + kJoinRuns - 1) / kJoinRuns, (p.D + kJoinColumns - 1) / kJoinColumns), kThreads, 0, 1, s, p, q);
+    const dim3 grid((q.runs + kJoinRuns - 1) / kJoinRuns, (p.D + kJoinColumns - 1) / kJoinColumns);
+    return launch(join_runs, grid, kThreads, 0, 1, s, p, q);
 }
 
 }  // namespace embed

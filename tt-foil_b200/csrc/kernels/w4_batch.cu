@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kThreads, 2)
             wait(&d_full[u % kUnits], u / kUnits & 1u);
             __syncwarp();
             tc_fence_after();
-            const float s = bf16_bits_to_f32(ld_shared_u16(scales + (b % kScaleSlots * kGroups + gi) * (kColumns * 2u) + column * 2u));
+            const float s = bf16_bits_to_f32(
+                ld_shared_u16(scales + ((b % kScaleSlots * kGroups + gi) * kColumns + column) * 2u));
             const uint32_t at = tmem + (warp % 4u * 32u << 16) + u % kUnits * MT + row0;
             constexpr int kLoad = kAcc < 16 ? kAcc : 16;
 #pragma unroll
