@@ -7,8 +7,9 @@
 //
 //  * Eight warps read the storage blocks of 16 columns each through rings of
 //    their own (16-byte asynchronous copies) and write q - z, exact in bf16, to
-//    shared memory as the MMA's operand of 128 rows: K-major, 64 k a stage in
-//    the 128-byte swizzle.  A word of a storage block is 8 consecutive k of a
+//    shared memory as the MMA's operand of 128 rows: K-major in the 128-byte
+//    swizzle, 128 k a stage, or 64 where 64 rows leave no room for more (32 rows
+//    of 8192 x 24576: 61 us with 64, 56 with 128).  A word of a storage block is 8 consecutive k of a
 //    column, one 16-byte piece of that layout.  12 operations a word: shift,
 //    mask and 16 + q, minus 16 + z.
 //  * x comes by tensor copies, zeros past M and K, as the operand of 16, 32 or
@@ -22,7 +23,7 @@
 //    products.
 //
 // 64 rows, us (the warps' MMAs): 4096 x 4096 11 (29), 16384 x 4096 26 (67),
-// 8192 x 24576 68 (117), 8192 x 65536 143 (280); 32 rows: 9 (15), 21 (34), 61 (60).
+// 8192 x 24576 68 (117), 8192 x 65536 143 (280); 32 rows: 9 (15), 19 (34), 56 (60).
 // Bound by the instructions of the conversion (some 350 a storage block, of which
 // 130 make the operand and 40 add its products) and by shared memory, where a
 // block's 1 KB of codes is written and read as 4 KB.  Tried, for 64 rows of 8192 x
@@ -46,11 +47,14 @@ using namespace gemm;
 
 constexpr uint32_t kColumns = 128;   // of W a CTA takes: the MMA's rows
 constexpr uint32_t kWorkers = 8, kMmaWarp = 8, kCopyWarp = 9, kThreads = 320;
-constexpr uint32_t kStages = 3;      // of 64 k
-constexpr uint32_t kRing = 3;        // storage blocks of a warp on their way
+// Halves of 64 k in a stage, stages, storage blocks of a warp on their way: what
+// two CTAs of an SM have room for.
+__host__ __device__ constexpr uint32_t halves(uint32_t mt) { return mt == 64 ? 1 : 2; }
+__host__ __device__ constexpr uint32_t stages(uint32_t mt) { return mt == 64 ? 3 : 2; }
+__host__ __device__ constexpr uint32_t ring(uint32_t mt) { return mt == 64 ? 3 : 2; }
 constexpr uint32_t kUnits = 4;       // accumulators
 constexpr uint32_t kScaleSlots = 4;  // blocks whose scales are kept: warps are at most three blocks apart
-constexpr uint32_t kWBytes = kColumns * 128;
+constexpr uint32_t kWHalf = kColumns * 128;
 
 struct Batch {
     const uint8_t* packed;
@@ -62,9 +66,9 @@ struct Batch {
     uint32_t S, kb_each, kb_more;     // CTAs of a cluster, blocks of each, how many have one more
 };
 
-__host__ __device__ constexpr uint32_t stage_bytes(uint32_t mt) { return kWBytes + mt * 128u; }
+__host__ __device__ constexpr uint32_t stage_bytes(uint32_t mt) { return halves(mt) * (kWHalf + mt * 128u); }
 constexpr uint32_t smem_bytes(uint32_t mt, uint32_t group, uint32_t zeros) {
-    return 1024u + kStages * stage_bytes(mt) + kWorkers * kRing * block_bytes(group, zeros) +
+    return 1024u + stages(mt) * stage_bytes(mt) + kWorkers * ring(mt) * block_bytes(group, zeros) +
            kScaleSlots * (128u / group) * kColumns * 2u;
 }
 
@@ -136,7 +140,8 @@ template <int MT, int GROUP, bool ZEROS>
 __global__ void __launch_bounds__(kThreads, 2)
     batch_kernel(const Batch p, const __grid_constant__ CUtensorMap map_x) {
     constexpr uint32_t kBytes = block_bytes(GROUP, ZEROS), kGroups = 128 / GROUP;
-    constexpr uint32_t kStageBytes = stage_bytes(MT), kTmem = kUnits * MT;
+    constexpr uint32_t kStages = stages(MT), kRing = ring(MT), kHalves = halves(MT);
+    constexpr uint32_t kStageBytes = stage_bytes(MT), kWBytes = kHalves * kWHalf, kTmem = kUnits * MT;
     constexpr int kAcc = MT / 2;  // rows of x a thread holds
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kStages], x_full[kStages], empty[kStages], d_full[kUnits], d_empty[kUnits], drain;
@@ -144,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     __shared__ volatile uint32_t abort_flag;
     uint8_t* const smem =
         reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t stages = smem_u32(smem), rings = stages + kStages * kStageBytes;
+    const uint32_t base = smem_u32(smem), rings = base + kStages * kStageBytes;
     const uint32_t scales = rings + kWorkers * kRing * kBytes;
     const uint32_t warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
     const uint32_t rank = blockIdx.x % p.S, n0 = blockIdx.x / p.S * kColumns, m0 = blockIdx.y * MT;
@@ -194,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     if (warp < kWorkers) {
         const uint32_t g = lane / 4u, t = lane % 4u;
-        const uint32_t ring = rings + warp * kRing * kBytes;
+        const uint32_t slots = rings + warp * kRing * kBytes;
         // Past the last tile: that one once more, not stored.
         const uint32_t tile = min(n0 / kBlockN + warp, p.tiles - 1u);
         const uint8_t* src = p.packed + ((uint64_t)tile * p.kb + kb0) * kBytes + lane * 16u;
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        for (uint32_t i = 0; i < kRing; ++i) issue(ring + i * kBytes);
+        for (uint32_t i = 0; i < kRing; ++i) issue(slots + i * kBytes);
 
         // After a wait that ran out the workers go on, with whatever there is, to
         // the end.
@@ -258,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint32_t odd = g & 1u;
         uint32_t eight;  // 16 + 8 twice, in one register for good
         asm volatile("mov.b32 %0, 0x41c041c0;" : "=r"(eight));
-        uint32_t slot = ring;
+        uint32_t slot = slots;
         uint32_t stage = 0, phase = 1;  // phase of the stage's previous round
         for (uint32_t b = 0; b < nkb; ++b) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 1) : "memory");
@@ -280,13 +285,15 @@ __global__ void __launch_bounds__(kThreads, 2)
                              ld_shared_v4(slot + kCodeBytes + lane * 16u));
             __syncwarp();  // every lane has read the slot
             issue(slot);
-            slot = slot + kBytes == ring + kRing * kBytes ? ring : slot + kBytes;
+            slot = slot + kBytes == slots + kRing * kBytes ? slots : slot + kBytes;
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
-                if (2u * b + h >= kStages) wait(&empty[stage], phase);
-                __syncwarp();
+                if (h % kHalves == 0) {
+                    if (2u * b + h >= kStages * kHalves) wait(&empty[stage], phase);
+                    __syncwarp();
+                }
                 // 64 k of 128 rows in the 128-byte swizzle.
-                const uint32_t rows = stages + stage * kStageBytes + warp * 2048u + g * 128u;
+                const uint32_t rows = base + stage * kStageBytes + h % kHalves * kWHalf + warp * 2048u + g * 128u;
                 const uint32_t at0 = ((odd * 4u + t) ^ g) * 16u;  // of the first word written; the other: 64 bytes off
 #pragma unroll
                 for (uint32_t s = 2 * h; s < 2 * h + 2; ++s) {
@@ -300,9 +307,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                     st_shared_v4(to + 1024u, make_uint4(difference<0>(c, z1), difference<1>(c, z1),
                                                         difference<2>(c, z1), difference<3>(c, z1)));
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[stage]);
-                if (++stage == kStages) stage = 0, phase ^= 1u;
+                if (h % kHalves == kHalves - 1) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[stage]);
+                    if (++stage == kStages) stage = 0, phase ^= 1u;
+                }
                 if (b) take_half(b - 1u, h);
             }
         }
@@ -318,11 +327,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (uint32_t b = 0; b < nkb && ok; ++b) {
 #pragma unroll
             for (uint32_t h = 0; h < 2; ++h) {
-                ok = ok && wait(&full[stage], phase) && wait(&x_full[stage], phase);
+                if (h % kHalves == 0) ok = ok && wait(&full[stage], phase) && wait(&x_full[stage], phase);
                 // W was written by the generic proxy, the MMA reads through the async
                 // one.  (A fence by every writer: 75 us instead of 68, 64 rows of 8192 x 24576.)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                const uint32_t w_at = stages + stage * kStageBytes >> 4, x_at = w_at + (kWBytes >> 4);
+                const uint32_t w_at = base + stage * kStageBytes + h % kHalves * kWHalf >> 4;
+                const uint32_t x_at = base + stage * kStageBytes + kWBytes + h % kHalves * (MT * 128u) >> 4;
                 const uint64_t w_desc = kmaj | (uint64_t)(w_at & 0x3fffu), x_desc = kmaj | (uint64_t)(x_at & 0x3fffu);
 #pragma unroll
                 for (uint32_t k0 = 0; k0 < 4; k0 += GROUP == 32 ? 2 : 4) {  // 16 k each
@@ -337,10 +347,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                             tc_mma(tmem + u % kUnits * MT, w_desc + k * 2u, x_desc + k * 2u, instruction(MT),
                                    in == 0 && k == k0 ? 0u : 1u);
                         if (GROUP < 128 || h == 1) tc_commit(&d_full[u % kUnits]);
-                        if (k0 + (GROUP == 32 ? 2 : 4) == 4) tc_commit(&empty[stage]);
+                        if (k0 + (GROUP == 32 ? 2 : 4) == 4 && h % kHalves == kHalves - 1) tc_commit(&empty[stage]);
                     }
                 }
-                if (++stage == kStages) stage = 0, phase ^= 1u;
+                if (h % kHalves == kHalves - 1 && ++stage == kStages) stage = 0, phase ^= 1u;
             }
         }
         // Every MMA ends before TMEM is released.
@@ -350,11 +360,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
     } else if (warp == kCopyWarp && lane == 0) {
         uint32_t stage = 0, phase = 1, i = 0;
-        for (; i < 2u * nkb; ++i) {
+        for (; i < 2u / kHalves * nkb; ++i) {
             if (i >= kStages && !wait(&empty[stage], phase)) break;
-            mbar_expect_tx(&x_full[stage], MT * 128u);
-            tma_load_2d(stages + stage * kStageBytes + kWBytes, &map_x, (int32_t)(kb0 * kBlockK + i * 64u),
-                        (int32_t)m0, &x_full[stage]);
+            mbar_expect_tx(&x_full[stage], kHalves * MT * 128u);
+#pragma unroll
+            for (uint32_t h = 0; h < kHalves; ++h)
+                tma_load_2d(base + stage * kStageBytes + kWBytes + h * (MT * 128u), &map_x,
+                            (int32_t)(kb0 * kBlockK + (i * kHalves + h) * 64u), (int32_t)m0, &x_full[stage]);
             if (++stage == kStages) stage = 0, phase ^= 1u;
         }
         // Every copy ends before the block does.
