@@ -12,7 +12,7 @@
 //    of 8192 x 24576: 61 us with 64, 56 with 128).  A word of a storage block is 8 consecutive k of a
 //    column, one 16-byte piece of that layout.  12 operations a word: shift,
 //    mask and 16 + q, minus 16 + z.
-//  * x comes by tensor copies, zeros past M and K, as the operand of 16, 32 or
+//  * x comes by tensor copies, zeros past M and K, as the operand of 32, 48 or
 //    64 columns.
 //  * One thread issues tcgen05.mma 128 x MT x 16.  Each group of k has an
 //    accumulator of its own in TMEM (four in turn), which the eight warps read
@@ -23,7 +23,8 @@
 //    products.
 //
 // 64 rows, us (the warps' MMAs): 4096 x 4096 11 (29), 16384 x 4096 26 (67),
-// 8192 x 24576 68 (117), 8192 x 65536 143 (280); 32 rows: 9 (15), 19 (34), 56 (60).
+// 8192 x 24576 68 (117), 8192 x 65536 143 (280); 48 rows: 9.5 (22), 22 (51), 59 (88); 32
+// rows: 9 (15), 19 (34), 56 (60).
 // Bound by the instructions of the conversion (some 350 a storage block, of which
 // 130 make the operand and 40 add its products) and by shared memory, where a
 // block's 1 KB of codes is written and read as 4 KB.  Tried, for 64 rows of 8192 x
@@ -77,14 +78,19 @@ __host__ __device__ constexpr uint32_t instruction(uint32_t n) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-__device__ __forceinline__ void tmem_ld8(uint32_t at, float* v) {
-    uint32_t r[8];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "r"(at));
+// N (8 or 16) consecutive values of this thread's row.
+template <int N>
+__device__ __forceinline__ void tmem_values(uint32_t at, float* v) {
+    uint32_t r[16];
+    if constexpr (N == 16)
+        tmem_ld16(at, r);
+    else
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                     : "r"(at));
     tmem_ld_wait();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < N; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // Shared memory by its own addresses (from generic ones: more instructions).
@@ -141,7 +147,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     batch_kernel(const Batch p, const __grid_constant__ CUtensorMap map_x) {
     constexpr uint32_t kBytes = block_bytes(GROUP, ZEROS), kGroups = 128 / GROUP;
     constexpr uint32_t kStages = stages(MT), kRing = ring(MT), kHalves = halves(MT);
-    constexpr uint32_t kStageBytes = stage_bytes(MT), kWBytes = kHalves * kWHalf, kTmem = kUnits * MT;
+    constexpr uint32_t kStageBytes = stage_bytes(MT), kWBytes = kHalves * kWHalf;
+    constexpr uint32_t kTmem = MT == 32 ? 128 : 256;  // columns, a power of two
     constexpr int kAcc = MT / 2;  // rows of x a thread holds
     extern __shared__ uint8_t smem_raw[];
     __shared__ uint64_t full[kStages], x_full[kStages], empty[kStages], d_full[kUnits], d_empty[kUnits], drain;
@@ -226,21 +233,16 @@ __global__ void __launch_bounds__(kThreads, 2)
             const float s = bf16_bits_to_f32(
                 ld_shared_u16(scales + ((b % kScaleSlots * kGroups + gi) * kColumns + column) * 2u));
             const uint32_t at = tmem + (warp % 4u * 32u << 16) + u % kUnits * MT + row0;
-            constexpr int kLoad = kAcc < 16 ? kAcc : 16;
 #pragma unroll
-            for (int c = 0; c < kAcc; c += kLoad) {
-                float v[kLoad];
-                if constexpr (kLoad == 8) {
-                    tmem_ld8(at + c, v);
-                } else {
-                    uint32_t r[16];
-                    tmem_ld16(at + c, r);
-                    tmem_ld_wait();
+            for (int c = 0; c < kAcc; c += 16) {
+                float v[16];
+                if (c + 16 <= kAcc)
+                    tmem_values<16>(at + c, v);
+                else
+                    tmem_values<8>(at + c, v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
-                }
-#pragma unroll
-                for (int i = 0; i < kLoad; ++i) acc[c + i] = fmaf(s, v[i], acc[c + i]);
+                for (int i = 0; i < 16; ++i)
+                    if (c + i < kAcc) acc[c + i] = fmaf(s, v[i], acc[c + i]);
             }
             tc_fence_before();
             __syncwarp();
@@ -462,7 +464,7 @@ cudaError_t matvec_batch(const uint16_t* x, uint64_t ld_x, const uint8_t* packed
                          uint64_t ld_y, uint32_t M, const Weights& w, bool relu, uint32_t* err, cudaStream_t s) {
     const PFN_cuTensorMapEncodeTiled encode = encoder();
     if (!encode) return cudaErrorNotSupported;
-    const uint32_t mt = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+    const uint32_t mt = M <= 32 ? 32 : M <= 48 ? 48 : 64;
     Batch p{};
     p.packed = packed, p.bias = bias, p.y = y, p.err = err, p.ld_y = ld_y, p.wait_ns = foil_wait_limit_ns();
     p.M = M, p.N = w.N, p.kb = (w.K + kBlockK - 1) / kBlockK, p.tiles = (w.N + kBlockN - 1) / kBlockN, p.relu = relu;
@@ -476,7 +478,7 @@ cudaError_t matvec_batch(const uint16_t* x, uint64_t ld_x, const uint8_t* packed
                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return cudaErrorInvalidValue;
-    const BatchKernel kernel = mt == 16 ? pick<16>(w) : mt == 32 ? pick<32>(w) : pick<64>(w);
+    const BatchKernel kernel = mt == 32 ? pick<32>(w) : mt == 48 ? pick<48>(w) : pick<64>(w);
     const uint32_t smem = smem_bytes(mt, w.group, w.zeros);
     const cudaError_t e = foil_smem_optin(reinterpret_cast<const void*>(kernel), (int)smem);
     if (e != cudaSuccess) return e;
