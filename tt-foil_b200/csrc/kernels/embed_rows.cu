@@ -178,7 +178,7 @@ constexpr uint32_t kSortSmem = (kSortWarps * kMaxRadix + kSortCtas * kMaxRadix +
 constexpr uint32_t kMarkRows = kSortSmem * 8 / 32 * 32;  // rows that one CTA can clear
 
 struct Plan {
-    uint32_t run, runs, slabs;         // tokens of a run, runs, column slabs of a run
+    uint32_t run, runs, slabs, joined;  // tokens of a run, runs, column slabs of a run, runs a CTA joins
     uint32_t ctas, clear;              // CTAs of the sort, CTAs that clear rows
     uint32_t passes, bits;             // passes of `bits` bits
     uint32_t *key0, *token0, *key1, *token1;  // buffers of the sort, in turn
@@ -194,10 +194,10 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     q.run = kMaxRun;
     while (q.run > 8 && p.T > kMaxRun && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
     q.runs = (p.T + q.run - 1) / q.run;
-    // One CTA sorts few tokens as fast.  Clusters of 4 leave 128 SMs to the
+    // One CTA sorts few tokens as fast (2048 of them).  Clusters of 4 leave 128 SMs to the
     // zeros, of 8 only 112 (a cluster stays inside a GPC) but sort many tokens
     // in half the time.
-    q.ctas = p.T <= 4096 ? 1 : p.accumulate || p.T > 32768 ? kSortCtas : kSortCtas / 2;
+    q.ctas = p.T <= 2048 ? 1 : p.accumulate || p.T > 32768 ? kSortCtas : kSortCtas / 2;
     uint32_t bits = 1;
     while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
     q.passes = (bits + kMaxBits - 1) / kMaxBits;
@@ -427,8 +427,8 @@ __global__ void __launch_bounds__(kThreads) sum_runs(const Gradient p, const Pla
     }
 }
 
-// blockIdx.x: eight runs, of which those count whose last id begins there and
-// goes on; blockIdx.y: 256 columns.  8 warps take every eighth part, their sums
+// blockIdx.x: one or eight runs, of which those count whose last id begins there
+// and goes on; blockIdx.y: 256 columns.  8 warps take every eighth part, their sums
 // are added in order.
 constexpr uint32_t kJoinColumns = 256, kJoinRuns = 8;
 constexpr uint32_t kJoinAhead = 4;  // parts of a warp on their way
@@ -441,9 +441,9 @@ __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Pl
     const uint32_t *keys = q.key, warp = threadIdx.x / 32u, lane = threadIdx.x % 32u;
     // Warp w looks at run w.
     {
-        const uint64_t run = (uint64_t)blockIdx.x * kJoinRuns + warp, first = run * q.run, end = first + q.run;
+        const uint64_t run = (uint64_t)blockIdx.x * q.joined + warp, first = run * q.run, end = first + q.run;
         uint32_t found = ~0u, lo = (uint32_t)run + 1u, hi = q.runs;
-        if (end < p.T) {
+        if (warp < q.joined && end < p.T) {
             const uint32_t id = __ldcg(keys + end - 1u), next = __ldcg(keys + end), begin = __ldcg(keys + first);
             const uint32_t previous = first ? __ldcg(keys + first - 1u) : ~0u;
             if (id < p.V && next == id && !(begin == id && previous == id)) found = id;
@@ -462,8 +462,8 @@ __global__ void __launch_bounds__(kThreads) join_runs(const Gradient p, const Pl
     __syncthreads();
     const uint32_t col = blockIdx.y * kJoinColumns + lane;
     constexpr int kEach = kJoinColumns / 32;
-    for (uint32_t w = 0; w < kJoinRuns; ++w) {
-        const uint32_t id = ids[w], run = blockIdx.x * kJoinRuns + w, hi = ends[w];
+    for (uint32_t w = 0; w < q.joined; ++w) {
+        const uint32_t id = ids[w], run = blockIdx.x * q.joined + w, hi = ends[w];
         if (id == ~0u) continue;
         float s[kEach] = {};
         for (uint32_t r0 = run + warp; r0 < hi; r0 += kJoinAhead * (kThreads / 32u)) {
@@ -553,7 +553,12 @@ cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
     w.use(p.dout, p.ld_dout, fp32 ? 4 : 2);
     e = fp32 ? sum_launch<float>(p, q, w.v, s) : sum_launch<uint16_t>(p, q, w.v, s);
     if (e != cudaSuccess || q.runs < 2) return e;
-    const dim3 grid((q.runs + kJoinRuns - 1) / kJoinRuns, (p.D + kJoinColumns - 1) / kJoinColumns);
+    const uint32_t columns = (p.D + kJoinColumns - 1) / kJoinColumns;
+    // A run a CTA where those are few: an id's parts are found and added in a chain
+    // (3592 tokens of 439 channels 29 and 21 us), else eight, for the launch of so many
+    // CTAs (65536 of 1024 channels 104 and 96 us).
+    q.joined = (uint64_t)q.runs * columns <= 2048 ? 1 : kJoinRuns;
+    const dim3 grid((q.runs + q.joined - 1) / q.joined, columns);
     return launch(join_runs, grid, kThreads, 0, 1, s, p, q);
 }
 
