@@ -194,10 +194,11 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     q.run = kMaxRun;
     while (q.run > 8 && p.T > kMaxRun && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
     q.runs = (p.T + q.run - 1) / q.run;
-    // One CTA sorts few tokens as fast (2048 of them).  Clusters of 4 leave 128 SMs to the
-    // zeros, of 8 only 112 (a cluster stays inside a GPC) but sort many tokens
-    // in half the time.
-    q.ctas = p.T <= 2048 ? 1 : p.accumulate || p.T > 32768 ? kSortCtas : kSortCtas / 2;
+    // One CTA sorts few tokens as fast (2048 of them).  Clusters of 4 leave 128 SMs
+    // to the zeros, of 8 only 112 (a cluster stays inside a GPC) but sort in half the
+    // time: taken where the table has less than 16 KB a token (4 and 8 CTAs: 32768
+    // tokens, 32000 x 1024: 77 and 60 us; 8192 tokens, 32000 x 4096: 115 and 122).
+    q.ctas = p.T <= 2048 ? 1 : p.accumulate || (uint64_t)p.V * p.D <= 4096ull * p.T ? kSortCtas : kSortCtas / 2;
     uint32_t bits = 1;
     while (bits < 32 && (p.V >> bits)) ++bits;  // ids 0 .. V - 1, and V for the rows that do not count
     q.passes = (bits + kMaxBits - 1) / kMaxBits;
