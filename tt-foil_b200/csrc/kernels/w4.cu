@@ -188,6 +188,9 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
                     zero[j] = make_float2((float)__shfl_sync(0xffffffffu, c.zero, from),
                                           (float)__shfl_sync(0xffffffffu, c.zero, from + 2));
             }
+            // Without zero points |w / s| is below 7.2 where the reciprocal is a number (a
+            // scale above 2^-128 is within 2^-6 of max / 7).  Smaller scales, which divide,
+            // have few bits: w / s reaches 10 and is clamped.
             auto face_codes = [&](int f, auto divide) {
                 uint32_t word = 0;
 #pragma unroll
@@ -195,8 +198,11 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
                     const uint32_t v = word_of(x[f], j);
                     const float2 wf = make_float2(bf16_bits_to_f32(v & 0xffffu), __uint_as_float(v & 0xffff0000u));
                     float2 t = quotient(wf, s[j], inv[j]);
-                    if constexpr (decltype(divide)::value)
+                    if constexpr (decltype(divide)::value) {
                         t = make_float2(s[j].x > 0.0f ? wf.x / s[j].x : 0.0f, s[j].y > 0.0f ? wf.y / s[j].y : 0.0f);
+                        if constexpr (!ZEROS)
+                            t = make_float2(fminf(fmaxf(t.x, -8.0f), 7.0f), fminf(fmaxf(t.y, -8.0f), 7.0f));
+                    }
                     // To integers, ties to even: 1.5 * 2^23 leaves no fraction bits.
                     const float2 kRound = both(12582912.0f);
                     if constexpr (ZEROS) {
@@ -204,7 +210,7 @@ __global__ void __launch_bounds__(256) quantize_kernel(const uint16_t* __restric
                         t = make_float2(fminf(fmaxf(t.x, 0.0f), 15.0f), fminf(fmaxf(t.y, 0.0f), 15.0f));
                         t = add2(t, kRound);
                     } else {
-                        t = add2(t, both(12582920.0f));  // + 8; |t| < 7.04, no need to clamp
+                        t = add2(t, both(12582920.0f));  // + 8
                     }
                     const uint32_t codes = __byte_perm(__float_as_uint(t.x), __float_as_uint(t.y), 0x5410);
                     word |= (codes & 0x000f000fu) << (4 * j);
