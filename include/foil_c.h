@@ -444,8 +444,9 @@ FOIL_API int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* pa
  *
  * Weights that are NULL are ones.  gate: bf16 rows of D, token t takes row
  * t / gate_rows (1: a gate for each token, T: one vector for all); NULL: none.
- * act: FOIL_GATE_NONE or FOIL_GATE_SIGMOID.  resid and h: bf16, or fp32 if
- * `fp32` is non-zero.  u NULL: no branch (h = resid).  h or y may be NULL
+ * act: FOIL_GATE_NONE or FOIL_GATE_SIGMOID (within 2^-20 relative, values below
+ * 2^-126 as 0; its derivative in the gradient alike).  resid and h: bf16, or
+ * fp32 if `fp32` is non-zero.  u NULL: no branch (h = resid).  h or y may be NULL
  * (not wanted), not both.  rstd_post, rstd_pre: T floats each,
  * 1 / sqrt(mean + eps), for the gradient, or NULL.  Sums and the value that y
  * is made from are held in fp32, h is rounded once.  h may be resid and y may

@@ -114,10 +114,50 @@ __device__ __forceinline__ void store_plain(float* p, const float2 (&v)[V * NV /
     }
 }
 
-// At most 2^-17 relative off, to |g| = 88: __expf is within 2 + 1.173 |g| units
-// in the last place.
-__device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
-__device__ __forceinline__ float2 sigmoid2(float2 g) { return make_float2(sigmoid(g.x), sigmoid(g.y)); }
+// The logistic function of gates: act(g) = 1 / (1 + e) with e = exp(-g), and for its
+// derivative act(g) act(-g) the other factor is e act(g), without the cancellation
+// of 1 - act(g).  Gates are bf16, so e = 2^t (1 + c) with t = -g H exact (8 bits
+// times the 16 upper bits H of log2 e) and c = -g ln 2 (log2 e - H), below 2^-11, so
+// that what follows c does not count.  ex2.approx is within 2^-22, rcp.approx within
+// 2^-23; with the operations' roundings act and the derivative are within 2^-20
+// relative, to 0 below 2^-126.  (By expf and a division: 8192 x 5120 118 us, with
+// this 104.)
+constexpr float kLog2e = 47274.0f / 32768.0f, kRest = (float)((1.4426950408889634 - 47274.0 / 32768.0) * 0.6931471805599453);
+__device__ __forceinline__ float2 exp2(float2 x) {
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.x));
+    asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.y));
+    return x;
+}
+__device__ __forceinline__ float2 reciprocal2(float2 x) {
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.x));
+    asm("rcp.approx.ftz.f32 %0, %0;" : "+f"(x.y));
+    return x;
+}
+// g, at least -88 and at most 128; NaN stays.
+__device__ __forceinline__ float between(float g) {
+    asm("min.NaN.f32 %0, %0, 0f43000000;\n\tmax.NaN.f32 %0, %0, 0fc2b00000;" : "+f"(g));
+    return g;
+}
+// exp(-g) of gates 2 i and 2 i + 1, between exp(-128) = 0 and exp(88), a number
+// whose reciprocal is 0; NaN stays.
+template <int V, int NV>
+__device__ __forceinline__ float2 exp_minus2(const Raw<uint16_t, V> (&r)[NV], int i) {
+    float2 g = get2(r, i);
+    if constexpr (V == 1) {
+        g = make_float2(between(g.x), between(g.y));
+    } else {
+        uint32_t w = r[2 * i / V].w[i % (V / 2)];
+        asm("min.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0x43004300u));
+        asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(w) : "r"(0xc2b0c2b0u));
+        g = make_float2(bf16_bits_to_f32(w & 0xffffu), __uint_as_float(w & 0xffff0000u));
+    }
+    return mul2(exp2(mul2(g, both(-kLog2e))), fma2(g, both(-kRest), both(1.0f)));
+}
+__device__ __forceinline__ float2 act2(float2 e) { return reciprocal2(add2(e, both(1.0f))); }
+template <int V, int NV>
+__device__ __forceinline__ float2 sigmoid2(const Raw<uint16_t, V> (&r)[NV], int i) {
+    return act2(exp_minus2(r, i));
+}
 
 // The threads that hold one row: 4 to 32 lanes of a warp, a CTA, or the CTAs of
 // a cluster.
@@ -293,7 +333,7 @@ __device__ __forceinline__ float sum_squares(const float2 (&v)[V * NV / 2], cons
 enum { kNoGate = 0, kPlainGate = 1, kSigmoidGate = 2 };
 template <int GATE, int V, int NV>
 __device__ __forceinline__ float2 gate2(const Raw<uint16_t, V> (&r)[NV], int i) {
-    return GATE == kSigmoidGate ? sigmoid2(get2(r, i)) : get2(r, i);
+    return GATE == kSigmoidGate ? sigmoid2(r, i) : get2(r, i);
 }
 
 template <class R, int V, int NV, int THREADS, int CTAS, int GATE>
@@ -422,8 +462,8 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
     constexpr int kPairs = V * NV / 2;
     // The next row in registers where those suffice (4096 x 4096, bf16 in
     // vectors: 59 us with, 69 without), else towards L2 only (fp32: 102 and 81
-    // us; 4000 x 4095 one by one: 162 and 102).
-    constexpr bool kRowAhead = sizeof(R) == 2 && (V == 8 || (V == 2 && !GATE));
+    // us; 4000 x 4095 one by one: 162 and 102; bf16 with logistic gates: 86 and 72).
+    constexpr bool kRowAhead = sizeof(R) == 2 && ((V == 8 && GATE != kSigmoidGate) || (V == 2 && !GATE));
     // Rows asked for from L2.  Beside the row in registers it pays where a row
     // takes a cluster (2000 x 8192 84 and 75 us), elsewhere it costs registers
     // (16384 x 4096 without gates 168 and 178 us).
@@ -500,7 +540,7 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
             gw[i] = get2(wp, i);
-            if (p.gate) gw[i] = mul2(gw[i], p.gate_act ? sigmoid2(get2(g, i)) : get2(g, i));
+            if (p.gate) gw[i] = mul2(gw[i], p.gate_act ? sigmoid2(g, i) : get2(g, i));
         }
     };
     auto end_gate = [&] {
@@ -514,9 +554,10 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             dgate[i] = mul2(get2(wp, i), a);
             if (p.gate) {
                 float2 ga = get2(g, i);
-                if (p.gate_act) {  // the logistic function's derivative is g - g^2
-                    ga = sigmoid2(ga);
-                    dgate[i] = mul2(dgate[i], fma2(mul2(ga, ga), both(-1.0f), ga));
+                if (p.gate_act) {
+                    const float2 e = exp_minus2(g, i);
+                    ga = act2(e);
+                    dgate[i] = mul2(dgate[i], mul2(ga, mul2(ga, e)));
                 }
                 a = mul2(a, ga);
             }
@@ -538,7 +579,7 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
         // with k = scale act: one round of sums, c2 = ru (S1 - c1 rh S2).
         const float ks = p.scale * x.ru;
         const float2 rh = both(x.rh);
-        float2 e[kPairs], hh[kPairs], ga[GATE ? kPairs : 1];
+        float2 e[kPairs], hh[kPairs], ga[GATE ? kPairs : 1];  // ga: the gate, or exp(-gate)
         float2 s0 = both(0.0f), s1 = both(0.0f), s2 = both(0.0f);
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
@@ -549,8 +590,8 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             e[i] = fma2(rh, a, get2(x.dh, i));
             float2 k;
             if constexpr (GATE) {
-                ga[i] = gate2<GATE>(x.gate, i);
-                k = mul2(mul2(get2(x.u, i), get2(w_post, i)), ga[i]);
+                ga[i] = GATE == kSigmoidGate ? exp_minus2(x.gate, i) : get2(x.gate, i);
+                k = mul2(mul2(get2(x.u, i), get2(w_post, i)), GATE == kSigmoidGate ? act2(ga[i]) : ga[i]);
             } else {
                 k = mul2(get2(x.u, i), gw[i]);
             }
@@ -569,8 +610,9 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             e[i] = fma2(m1, hh[i], e[i]);
             const float2 u = get2(x.u, i), dz = mul2(e[i], k2);
             if constexpr (GATE) {
-                const float2 wp = get2(w_post, i), dp = mul2(dz, ga[i]);
-                dgate[i] = mul2(GATE == kSigmoidGate ? fma2(mul2(dp, ga[i]), both(-1.0f), dp) : dz, mul2(u, wp));
+                const float2 act = GATE == kSigmoidGate ? act2(ga[i]) : ga[i];
+                const float2 wp = get2(w_post, i), dp = mul2(dz, act);
+                dgate[i] = mul2(GATE == kSigmoidGate ? mul2(dp, mul2(ga[i], act)) : dz, mul2(u, wp));
                 dw_post[i] = fma2(dp, u, dw_post[i]);
                 hh[i] = fma2(m2, u, mul2(dp, wp));
             } else {
