@@ -92,3 +92,38 @@ def test_gates_without_end():
     assert du[0, 3] == 1 and du[0, 100] == 0 and du[1, 5] == 1
     assert torch.isnan(du[1, 263]) and torch.isnan(du).sum() == 1
     assert torch.isnan(dgate[1, 263]) and torch.isnan(dgate).sum() == 1
+
+
+# ------------------------------------------------------------ non-finite rows ---
+
+def kinds(t):
+    """0 for a number, 1 and 2 for an infinity by its sign, 3 for NaN."""
+    t = t.cpu().to(F64)
+    return torch.isnan(t) * 3 + torch.isposinf(t) * 1 + torch.isneginf(t) * 2
+
+
+# Threads past D: none, in a warp's teams, in a CTA, in a cluster; vectors of 8, 2, 1.
+ODD = [(24, False), (24, True), (34, False), (50, False), (258, False), (51, True), (200, False), (1000, True),
+       (2050, False), (2049, False), (4104, True), (4104, False), (8200, False), (5001, True)]
+
+
+@pytest.mark.parametrize("D,fp32", ODD)
+@pytest.mark.parametrize("where,gate_rows", [("dy", 0), ("dy", 1), ("h", 0), ("h", 2), ("dh", 0), ("dh", 1)])
+def test_gradient_of_an_infinity_in_the_last_channel(D, fp32, where, gate_rows):
+    """It makes infinities and NaN where the formula does, in its row only."""
+    T, row = 5, 2
+    p = Norm(T, D, fp32, True, gate_rows, "sigmoid" if gate_rows else "none", seed=3)
+    saved = run_forward(p)
+    base = run_backward(p, saved)
+    if where == "h":
+        saved["h"][row, D - 1] = math.inf
+    else:
+        getattr(p, where)[row, D - 1] = math.inf
+    out = run_backward(p, saved)
+    ref = grad64(p, saved["h"].cpu(), saved["rstd_pre"].cpu(), saved["rstd_post"].cpu())
+    assert torch.equal(kinds(out["dresid"]), kinds(ref["dresid"][0]))
+    if where == "dh":
+        assert torch.equal(kinds(out["du"]), kinds(ref["du"][0]))
+    keep = [t for t in range(T) if t != row]
+    for k in ("dresid", "du"):
+        assert torch.equal(out[k][keep], base[k][keep]), k

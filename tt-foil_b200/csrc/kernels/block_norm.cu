@@ -13,6 +13,7 @@
 #include "block_norm.cuh"
 
 #include <cstring>
+#include <type_traits>
 
 #include "gemm_ptx.cuh"
 
@@ -122,7 +123,8 @@ __device__ __forceinline__ void store_plain(float* p, const float2 (&v)[V * NV /
 // 2^-23; with the operations' roundings act and the derivative are within 2^-20
 // relative, to 0 below 2^-126.  (By expf and a division: 8192 x 5120 118 us, with
 // this 104.)
-constexpr float kLog2e = 47274.0f / 32768.0f, kRest = (float)((1.4426950408889634 - 47274.0 / 32768.0) * 0.6931471805599453);
+constexpr float kLog2e = 47274.0f / 32768.0f;
+constexpr float kRest = (float)((1.4426950408889634 - 47274.0 / 32768.0) * 0.6931471805599453);
 __device__ __forceinline__ float2 exp2(float2 x) {
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.x));
     asm("ex2.approx.ftz.f32 %0, %0;" : "+f"(x.y));
@@ -255,6 +257,12 @@ __device__ __forceinline__ uint32_t column(int j, const Team& t, uint32_t D) {
 template <int V>
 __device__ __forceinline__ bool inside(int j, const Team& t, uint32_t D) {
     return (j * t.size + t.rank) * V < D;
+}
+
+template <class T, int V>
+__device__ __forceinline__ void clear(Raw<T, V>& r) {
+#pragma unroll
+    for (int k = 0; k < Raw<T, V>::kWords; ++k) r.w[k] = 0u;
 }
 
 // bf16 weights of the thread's channels: ones where there are none, zeros past D.
@@ -457,18 +465,15 @@ Chunks plan_chunks(uint32_t T, uint32_t D, uint32_t gate_rows) {
 // the gate's part is taken out of the sums over its tokens: with A = sum dz
 // uhat, dw_post gains act A and dgate is act' w_post A), else a gate row for
 // each token.
-template <class R, int V, int NV, int THREADS, int GATE>
+// AHEAD: the next row arrives in registers while the present one is worked on.
+template <class R, int V, int NV, int THREADS, int GATE, bool AHEAD>
 __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, const TeamPlan plan) {
     constexpr int kPairs = V * NV / 2;
-    // The next row in registers where those suffice (4096 x 4096, bf16 in
-    // vectors: 59 us with, 69 without), else towards L2 only (fp32: 102 and 81
-    // us; 4000 x 4095 one by one: 162 and 102; bf16 with logistic gates: 86 and 72).
-    constexpr bool kRowAhead = sizeof(R) == 2 && ((V == 8 && GATE != kSigmoidGate) || (V == 2 && !GATE));
     // Rows asked for from L2.  Beside the row in registers it pays where a row
     // takes a cluster (2000 x 8192 84 and 75 us), elsewhere it costs registers
     // (16384 x 4096 without gates 168 and 178 us).
-    constexpr bool kAhead = !kRowAhead || GATE;
-    constexpr uint32_t kAheadBy = kRowAhead ? 3u : 2u, kAheadMin = kRowAhead ? 4097u : 256u;
+    constexpr bool kAhead = !AHEAD || GATE;
+    constexpr uint32_t kAheadBy = AHEAD ? 3u : 2u, kAheadMin = AHEAD ? 4097u : 256u;
     __shared__ float shared[2 * Team::kSumFloats];
     __shared__ float2 post_sum[GATE ? 1 : kPairs * THREADS];  // dw_post of the gate rows done, a slot for each thread
     Team team = team_of(plan, shared);
@@ -571,10 +576,20 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
         else
             store_row<V, NV>(p.dgate + (uint64_t)gate_row * (uint32_t)p.ld_dgate, dgate, team, p.D);
     };
+    // Threads past D read the last vector again, and if it is infinite or NaN no
+    // weight of zero keeps it out of the sums.  Cleared before it is used where the row
+    // has just been asked for; with the next row on its way that would wait for both
+    // (16384 x 4096: 214 us, this 171), so the sums go on without the last vector,
+    // the only one that can be outside there (see backward_launch).
+    const bool edge = !inside<V>(NV - 1, team, p.D);
     // One token: x is its row, which arrived while the one before was worked
     // on; the one after it goes to `next`.
-    auto step = [&](const Row& x, Row& next, uint32_t t) {
-        if (kRowAhead && t + 1u < t1) fetch(next, t + 1u);
+    auto step = [&](Row& x, Row& next, uint32_t t) {
+        if (AHEAD && t + 1u < t1) fetch(next, t + 1u);
+        if (!AHEAD && edge)
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+                if (!inside<V>(j, team, p.D)) clear(x.dy[j]), clear(x.h[j]), clear(x.u[j]), clear(x.dh[j]);
         // c1 = mean(a hhat) and c2 = mean(dp pv), dp = k (dh + rh (a - hhat c1))
         // with k = scale act: one round of sums, c2 = ru (S1 - c1 rh S2).
         const float ks = p.scale * x.ru;
@@ -586,6 +601,7 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             hh[i] = mul2(get2(x.h, i), rh);
             const float2 dy = get2(x.dy, i), a = mul2(dy, get2(w_pre, i));
             dw_pre[i] = fma2(dy, hh[i], dw_pre[i]);
+            const float2 s0_before = s0, s1_before = s1, s2_before = s2;
             s0 = fma2(a, hh[i], s0);
             e[i] = fma2(rh, a, get2(x.dh, i));
             float2 k;
@@ -597,8 +613,10 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
             }
             s1 = fma2(k, e[i], s1);
             s2 = fma2(k, hh[i], s2);
+            if (AHEAD && V == 2 && i == kPairs - 1 && edge) s0 = s0_before, s1 = s1_before, s2 = s2_before;
         }
         float s[3] = {sum2(s0), sum2(s1), sum2(s2)};
+        if (AHEAD && NV == 1 && edge) s[0] = s[1] = s[2] = 0.0f;
         team.sum(s);
         const float c1 = x.rh * s[0] * inv_d;
         const float c2 = post ? x.ru * x.ru * ks * (s[1] - c1 * s[2]) * inv_d : 0.0f;
@@ -638,15 +656,15 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
     };
     if (t0 < t1) {
         Row a, b;
-        if (kRowAhead) fetch(a, t0);
+        if (AHEAD) fetch(a, t0);
         if constexpr (!GATE) {
             if (p.gate) gate_row = t0 / p.gate_rows, gate_left = p.gate_rows - t0 % p.gate_rows;
             start_gate();
         }
         for (uint32_t t = t0; t < t1; t += 2u) {
-            if (!kRowAhead) fetch(a, t);
+            if (!AHEAD) fetch(a, t);
             step(a, b, t);
-            if (!kRowAhead && t + 1u < t1) fetch(b, t + 1u);
+            if (!AHEAD && t + 1u < t1) fetch(b, t + 1u);
             if (t + 1u < t1) step(b, a, t + 1u);
         }
         if constexpr (!GATE)
@@ -770,11 +788,33 @@ cudaError_t forward_typed(const Forward& p, cudaStream_t s) {
     return p.gate_act ? forward_gated<R, V, kSigmoidGate>(p, s) : forward_gated<R, V, kPlainGate>(p, s);
 }
 
+// The next row in registers where those suffice (4096 x 4096, bf16 in vectors of 8:
+// 59 us with, 69 without), else towards L2 only (fp32: 102 and 81 us; 4000 x 4095 one
+// by one: 162 and 102; bf16 with logistic gates: 86 and 72).
+template <class R, int V, int GATE>
+constexpr bool next_row_ahead() {
+    return sizeof(R) == 2 && ((V == 8 && GATE != kSigmoidGate) || (V == 2 && GATE == kNoGate));
+}
+
 template <class R, int V, int GATE>
 cudaError_t backward_launch(const Backward& p, const Chunks& c, cudaStream_t s) {
     const Shape sh(p.D, 8, 512);
-    const dim3 grid((c.count + sh.teams - 1) / sh.teams * (sh.plan.ctas ? sh.plan.ctas : 1));
-    return launch(backward_kernel<R, V, 8 / V, 512, GATE>, grid, sh.threads, sh.plan.ctas, s, p, c, sh.plan);
+    const uint32_t ctas = sh.plan.ctas ? sh.plan.ctas : 1;
+    const dim3 grid((c.count + sh.teams - 1) / sh.teams * ctas);
+    auto go = [&](auto ahead) {
+        return launch(backward_kernel<R, V, 8 / V, 512, GATE, decltype(ahead)::value>, grid, sh.threads, sh.plan.ctas,
+                      s, p, c, sh.plan);
+    };
+    if constexpr (!next_row_ahead<R, V, GATE>()) {
+        return go(std::false_type());
+    } else if constexpr (V == 8) {
+        return go(std::true_type());
+    } else {
+        // Every vector but a thread's last has to be inside: not so for some rows of
+        // fewer than 768 channels.
+        const uint32_t team = sh.plan.ctas ? ctas * sh.threads : sh.plan.lanes;
+        return (8 / V - 1) * V * team <= p.D ? go(std::true_type()) : go(std::false_type());
+    }
 }
 
 template <class R, int V>
