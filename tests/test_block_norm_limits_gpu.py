@@ -127,3 +127,17 @@ def test_gradient_of_an_infinity_in_the_last_channel(D, fp32, where, gate_rows):
     keep = [t for t in range(T) if t != row]
     for k in ("dresid", "du"):
         assert torch.equal(out[k][keep], base[k][keep]), k
+
+
+@pytest.mark.parametrize("D,fp32", ODD)
+@pytest.mark.parametrize("gate_rows", [0, 1, 2])
+def test_gradient_without_post_norm_does_not_look_at_the_output(D, fp32, gate_rows):
+    """du = scale act dh' where there is no post norm, whatever u holds."""
+    T = 5
+    p = Norm(T, D, fp32, False, gate_rows, "none", seed=5)
+    saved = run_forward(p)
+    base = run_backward(p, saved, want=("dresid", "du"))
+    p.u[2, D - 1], p.u[3, 0], p.u[4] = math.inf, math.nan, -math.inf
+    out = run_backward(p, saved, want=("dresid", "du"))
+    for k in ("dresid", "du"):
+        assert torch.isfinite(base[k]).all() and torch.equal(out[k], base[k]), k

@@ -638,6 +638,17 @@ __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, con
                 hh[i] = fma2(m2, u, mul2(dz, gw[i]));
             }
         }
+        // Without the post norm u has no part in du, but 0 times an infinity has: made
+        // anew in a row whose u is not finite (its sums are not, either).
+        if (!post && !(fabsf(s[1]) + fabsf(s[2]) < INFINITY))
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i) {
+                const float2 dz = mul2(e[i], k2);
+                if constexpr (GATE)
+                    hh[i] = mul2(mul2(dz, GATE == kSigmoidGate ? act2(ga[i]) : ga[i]), get2(w_post, i));
+                else
+                    hh[i] = mul2(dz, gw[i]);
+            }
         store_row<V, NV>(p.dresid ? static_cast<R*>(p.dresid) + (uint64_t)t * (uint32_t)p.ld_dresid : nullptr, e, team,
                          p.D);
         store_row<V, NV>(p.du ? p.du + (uint64_t)t * (uint32_t)p.ld_du : nullptr, hh, team, p.D);
