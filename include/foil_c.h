@@ -427,9 +427,9 @@ FOIL_API int foil_w4_dequantize_tiles_dev(const void* packed, uint16_t* tiles, u
  * foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or NULL.  fp32
  * accumulation of unrounded weights, one rounding to bf16 at the end.  An
  * infinity or NaN in a row of x makes that row's outputs infinite or NaN.  With
- * more than 16 rows the sums of (q - z) x over a group are fp32 numbers before
- * their scale: keep |x| between 2^-100 and 2^116 there (smaller values lose
- * bits, sums of larger ones overflow).  M = 0 or N = 0 does nothing. */
+ * more than 16 rows a group's sum of (q - z) x and the row's sum are fp32 numbers
+ * whose least step is 2^-138 (for values below 2^-115 that is less than 24 bits);
+ * no finite x overflows them.  M = 0 or N = 0 does nothing. */
 FOIL_API int foil_w4_matvec_dev(const uint16_t* x, uint64_t ld_x, const void* packed, const uint16_t* bias,
                                 uint16_t* y, uint64_t ld_y, uint32_t M, uint32_t K, uint32_t N,
                                 uint32_t group, int32_t zeros, int32_t relu, void* stream);

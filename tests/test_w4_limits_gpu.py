@@ -49,3 +49,69 @@ def test_quantize_groups_of_subnormal_weights(group, zeros):
     assert torch.equal(w.to(F64), units * 2.0 ** -133)  # whole multiples, up to 8 bits
     got = dequantize(quantize(w, group, zeros), K, N, group, zeros)
     assert torch.equal(got, quantized(w, group, zeros).to(BF))
+
+
+@pytest.mark.parametrize("M", [7, 16, 17, 33, 48, 64])
+@pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
+def test_matvec_rows_near_both_ends_of_the_range(M, group, zeros):
+    """Rows scaled by 2^-118 to 2^120, the ordinary ones among them with the bits
+    they have in ordinary company: a batch of any size holds what a row alone holds."""
+    g = gen(M + group)
+    K, N = 1320, 70
+    codes, scales, zp = make_weights(g, K, N, group, zeros)
+    w = real_weights(codes, scales, zp, group)
+    x = randn(g, M, K).clamp(-8, 8)
+    packed = pack(codes, scales, zp, group)
+    plain = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(x.cuda(), packed, plain, M, K, N, group, zeros=zeros)
+    powers = ([0, 60, -80, 119, -118, 0, 23, 110, -100, 100] * 7)[:M]
+    scale = torch.tensor([2.0 ** p for p in powers], dtype=F64)[:, None]
+    xs = (x.to(F64) * scale).to(BF)
+    y = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(xs.cuda(), packed, y, M, K, N, group, zeros=zeros)
+    close(y.cpu().to(F64) / scale, (xs.to(F64) / scale) @ w.t(),
+          matvec_slack(xs.to(F64) / scale, codes, scales, zp, group, w), BF)
+    for m in range(M):
+        if powers[m] == 0:
+            assert torch.equal(y[m].view(torch.int16), plain[m].view(torch.int16)), m
+
+
+@pytest.mark.parametrize("M", [1, 12, 17, 40, 64])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_matvec_of_the_largest_numbers(M, group):
+    """The largest bf16 number in every place against the largest codes: sums of a
+    group reach 15 group 2^128, the scales bring them back."""
+    K, N = 2 * group, 16
+    big = torch.finfo(BF).max
+    codes = torch.full((N, K), 15, dtype=torch.uint8)
+    scales = torch.full((N, 2), 2.0 ** -20, dtype=BF)
+    zp = torch.zeros(N, 2, dtype=torch.uint8)
+    x = torch.full((M, K), big, dtype=BF)
+    x[M // 2] *= -1
+    y = torch.empty(M, N, dtype=BF, device="cuda")
+    tf.w4_matvec(x.cuda(), pack(codes, scales, zp, group), y, M, K, N, group, zeros=True)
+    w = real_weights(codes, scales, zp, group)
+    ref = x.to(F64) @ w.t()
+    close(y, ref, matvec_slack(x, codes, scales, zp, group, w), BF)
+
+
+@pytest.mark.parametrize("M", [6, 16, 40, 64])
+def test_matvec_rows_do_not_depend_on_their_company(M):
+    """Another row's values change nothing of a row's bits in a batch of one size;
+    a row of a batch and the row by itself agree within both calls' bounds."""
+    g = gen(M)
+    K, N, group = 4104, 330, 32
+    codes, scales, zp = make_weights(g, K, N, group, True)
+    w = real_weights(codes, scales, zp, group)
+    packed = pack(codes, scales, zp, group)
+    x = randn(g, M, K)
+    a, b, one = (torch.empty(m, N, dtype=BF, device="cuda") for m in (M, M, 1))
+    tf.w4_matvec(x.cuda(), packed, a, M, K, N, group, zeros=True)
+    other = randn(g, M, K)
+    other[3] = x[3]
+    tf.w4_matvec(other.cuda(), packed, b, M, K, N, group, zeros=True)
+    assert torch.equal(a[3].view(torch.int16), b[3].view(torch.int16))
+    tf.w4_matvec(x[3:4].cuda(), packed, one, 1, K, N, group, zeros=True)
+    ref, slack = x[3:4].to(F64) @ w.t(), matvec_slack(x[3:4], codes, scales, zp, group, w)
+    close(one, ref, slack, BF)
+    close(a[3:4], ref, slack, BF)

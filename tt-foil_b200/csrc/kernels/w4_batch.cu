@@ -6,12 +6,12 @@
 // weights takes 16).  Here a CTA takes 128 columns and a share of K:
 //
 //  * Eight warps read the storage blocks of 16 columns each through rings of
-//    their own (16-byte asynchronous copies) and write q - z, exact in bf16, to
-//    shared memory as the MMA's operand of 128 rows: K-major in the 128-byte
-//    swizzle, 128 k a stage, or 64 where 64 rows leave no room for more (32 rows
-//    of 8192 x 24576: 61 us with 64, 56 with 128).  A word of a storage block is 8 consecutive k of a
-//    column, one 16-byte piece of that layout.  12 operations a word: shift,
-//    mask and 16 + q, minus 16 + z.
+//    their own (16-byte asynchronous copies) and write (q - z) 2^-11, exact in
+//    bf16, to shared memory as the MMA's operand of 128 rows: K-major in the
+//    128-byte swizzle, 128 k a stage, or 64 where 64 rows leave no room for more
+//    (32 rows of 8192 x 24576: 61 us with 64, 56 with 128).  A word of a storage
+//    block is 8 consecutive k of a column, one 16-byte piece of that layout.  12
+//    operations a word: shift, mask and 16 + q, minus 16 + z.
 //  * x comes by tensor copies, zeros past M and K, as the operand of 32, 48 or
 //    64 columns.
 //  * One thread issues tcgen05.mma 128 x MT x 16.  Each group of k has an
@@ -128,8 +128,12 @@ __device__ __forceinline__ uint32_t word(const uint4& v, uint32_t i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
-// Codes number I and I + 4 of a word minus the zero point, as bf16: 16 + q by
-// a mask, minus 16 + z, both exact.
+// Codes number I and I + 4 of a word minus the zero point, times 2^-11, as bf16:
+// (16 + q) 2^-11 by a mask, minus (16 + z) 2^-11, both exact.  Sums of a group stay
+// below 128 x 15 x 2^-11 < 1 times its largest x, so no finite x overflows them;
+// the 2^11 is put back at the end.
+constexpr uint32_t kSixteen = 0x3c003c00u;  // twice 16 x 2^-11, whose steps of one are bits 3 to 6
+constexpr float kUnit = 2048.0f;
 template <int I>
 __device__ __forceinline__ uint32_t difference(uint32_t w, uint32_t z16) {
     const uint32_t v = I == 0 ? w << 3 : w >> (4 * I - 3);
@@ -138,7 +142,7 @@ __device__ __forceinline__ uint32_t difference(uint32_t w, uint32_t z16) {
         "lop3.b32 t, %1, 0x00780078, %2, 0xea;\n\t"
         "sub.rn.bf16x2 %0, t, %3;\n\t}"
         : "=r"(r)
-        : "r"(v), "r"(0x41804180u), "r"(z16));
+        : "r"(v), "r"(kSixteen), "r"(z16));
     return r;
 }
 
@@ -263,8 +267,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         // Odd columns take each two words in the other order, so that eight
         // lanes' 16-byte stores fall on distinct banks.
         const uint32_t odd = g & 1u;
-        uint32_t eight;  // 16 + 8 twice, in one register for good
-        asm volatile("mov.b32 %0, 0x41c041c0;" : "=r"(eight));
+        uint32_t eight;  // (16 + 8) 2^-11 twice, in one register for good
+        asm volatile("mov.b32 %0, 0x3c403c40;" : "=r"(eight));
         uint32_t slot = slots;
         uint32_t stage = 0, phase = 1;  // phase of the stage's previous round
         for (uint32_t b = 0; b < nkb; ++b) {
@@ -277,8 +281,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                 for (uint32_t i = 0; i < kGroups; ++i) {
                     const uint32_t at = (GROUP == 32 ? i ^ odd : i) * 16u + g;
-                    za[i] = 0x41804180u | (ld_shared_u8(z + at) & 15u) * 0x00080008u;
-                    zb[i] = 0x41804180u | (ld_shared_u8(z + at + 8u) & 15u) * 0x00080008u;
+                    za[i] = kSixteen | (ld_shared_u8(z + at) & 15u) * 0x00080008u;
+                    zb[i] = kSixteen | (ld_shared_u8(z + at + 8u) & 15u) * 0x00080008u;
                 }
             }
             if (lane < 2u * kGroups)  // 8 scales a lane
@@ -384,6 +388,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     }
     auto put = [&](uint32_t n, uint32_t m, float v) {
         if (n >= p.N || m >= p.M) return;
+        v *= kUnit;
         if (p.bias) v += bf16_bits_to_f32(p.bias[n]);
         if (p.relu && v < 0.0f) v = 0.0f;
         p.y[m * p.ld_y + n] = (uint16_t)(cvt_bf16x2(v, 0.0f) & 0xffffu);
