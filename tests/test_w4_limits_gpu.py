@@ -51,6 +51,27 @@ def test_quantize_groups_of_subnormal_weights(group, zeros):
     assert torch.equal(got, quantized(w, group, zeros).to(BF))
 
 
+def test_quantize_groups_whose_range_overflows_stand_for_nan():
+    """lo and hi of one group are numbers, hi - lo is not: NaN as weights and in
+    products of few and of many rows; the other columns are as without it."""
+    g = gen(8)
+    K, group = 256, 64
+    w = randn(g, K, 64, std=0.05)
+    w[70, 3], w[100, 3] = 3.0e38, -3.0e38
+    packed = quantize(w, group, True)
+    got = dequantize(packed, K, 64, group, True)
+    bad = torch.zeros(K, 64, dtype=torch.bool)
+    bad[64:128, 3] = True
+    assert torch.isnan(got[bad]).all() and torch.isfinite(got[~bad]).all()
+    for M in (1, 5, 16, 17, 64):
+        y = torch.empty(M, 64, dtype=BF, device="cuda")
+        x = randn(g, M, K) * 2.0 ** torch.randint(-30, 31, (M, K), generator=g)  # sums that are not exact
+        tf.w4_matvec(x.to(BF).cuda(), packed, y, M, K, 64, group, zeros=True)
+        assert torch.isnan(y[:, 3]).all(), M
+        y[:, 3] = 0
+        assert torch.isfinite(y).all(), M
+
+
 @pytest.mark.parametrize("M", [7, 16, 17, 33, 48, 64])
 @pytest.mark.parametrize("group,zeros", [(32, True), (64, False), (128, True)])
 def test_matvec_rows_near_both_ends_of_the_range(M, group, zeros):

@@ -110,12 +110,14 @@ struct Column {
 template <bool ZEROS>
 __device__ __forceinline__ Column column_of(uint32_t hi, uint32_t lo) {
     Column c;
-    const bool bad = max(hi, lo) >= 0x7f80u;  // an infinity or NaN among them
     const float fh = bf16_bits_to_f32(hi), fl = bf16_bits_to_f32(lo);
-    c.s_bits = bad ? 0x7fc0u : f32_to_bf16_bits(ZEROS ? (fh + fl) / 15.0f : fmaxf(fh, fl) / 7.0f);
+    c.s_bits = f32_to_bf16_bits(ZEROS ? (fh + fl) / 15.0f : fmaxf(fh, fl) / 7.0f);
+    // An infinity or NaN among them, or a range that overflows: NaN, not an infinity,
+    // which times a sum that is not exactly zero would be one.
+    if (max(hi, lo) >= 0x7f80u || c.s_bits >= 0x7f80u) c.s_bits = 0x7fc0u;
     c.s = bf16_bits_to_f32(c.s_bits);
     c.zero = 8;
-    if (!(c.s > 0.0f) || !isfinite(c.s)) {
+    if (!(c.s > 0.0f)) {
         c.s = 0.0f, c.inv = 0.0f;  // every code is the zero point
         return c;
     }
