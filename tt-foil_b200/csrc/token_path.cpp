@@ -188,6 +188,7 @@ extern "C" int foil_block_norm_dev(const void* resid, uint64_t ld_resid, const u
 }
 
 extern "C" uint64_t foil_block_norm_grad_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows) {
+    if (T > foil::norm::kMaxT || D > foil::norm::kMaxD) return 0;
     return foil::norm::backward_ws_bytes(T, D, gate_rows);
 }
 
@@ -269,6 +270,7 @@ extern "C" int foil_embed_rows_dev(const void* ids, int32_t id_bytes, const uint
 }
 
 extern "C" uint64_t foil_embed_rows_grad_ws_bytes(uint32_t T, uint32_t V, uint32_t D) {
+    if (T > foil::embed::kMaxRows || V > foil::embed::kMaxRows || D > foil::embed::kMaxD) return 0;
     return foil::embed::gradient_ws_bytes(T, V, D);
 }
 
