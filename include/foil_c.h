@@ -467,8 +467,9 @@ FOIL_API int foil_block_norm_dev(const void* resid, uint64_t ld_resid, const uin
  * and with post also rstd_post: the forward call's outputs.  The sums over
  * tokens are made in a fixed order.  ws: workspace of at least
  * foil_block_norm_grad_ws_bytes(T, D, gate_rows or 0) bytes, 16-byte aligned;
- * calls that may run at the same time need one each.  The size query gives 0
- * outside the ranges of T and D above.  T = 0 writes zeros to dw_post and dw_pre. */
+ * calls that may run at the same time need one each.  The size for T is enough
+ * for fewer tokens too, also with another gate_rows if this one is above 1; it is
+ * 0 outside the ranges of T and D.  T = 0 writes zeros to dw_post and dw_pre. */
 FOIL_API uint64_t foil_block_norm_grad_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows);
 FOIL_API int foil_block_norm_grad_dev(const void* dh, uint64_t ld_dh, const uint16_t* dy, uint64_t ld_dy,
                                       const void* h, uint64_t ld_h, const float* rstd_pre,
@@ -496,9 +497,9 @@ FOIL_API int foil_embed_rows_dev(const void* ids, int32_t id_bytes, const uint16
  * as they are.  Tokens are sorted by id and the sums made in a fixed order:
  * the same call gives the same bits.  Rows with pad_id or a bad id count
  * nowhere, the latter setting FOIL_DEVERR_BAD_INDEX.  ws: workspace of at
- * least foil_embed_rows_grad_ws_bytes(T, V, D) bytes (0 outside the ranges of T,
- * V and D above), 16-byte aligned; calls that may run at the same time need one
- * each. */
+ * least foil_embed_rows_grad_ws_bytes(T, V, D) bytes, 16-byte aligned; calls
+ * that may run at the same time need one each.  The size for T is enough for
+ * fewer tokens too; it is 0 outside the ranges of T, V and D. */
 FOIL_API uint64_t foil_embed_rows_grad_ws_bytes(uint32_t T, uint32_t V, uint32_t D);
 FOIL_API int foil_embed_rows_grad_dev(const void* ids, int32_t id_bytes, const void* dout, uint64_t ld_dout,
                                       float* dtable, uint64_t ld_dtable, uint32_t T, uint32_t V,

@@ -28,3 +28,23 @@ def test_workspaces_at_the_ends_of_the_ranges():
             for D in (1, 1 << 20):
                 assert ttfoil.embed_rows_grad_ws_bytes(T, V, D) >= 16 * T
     assert ttfoil.embed_rows_grad_ws_bytes(0, 4, 4) == 0 and ttfoil.embed_rows_grad_ws_bytes(4, 0, 4) == 0
+
+
+@pytest.mark.parametrize("D", [8, 64, 250, 264, 2050, 4096, 8200, 16384])
+@pytest.mark.parametrize("gate_rows", [0, 1, 2, 37, 1000, 1 << 30])
+def test_block_norm_workspace_grows_with_the_tokens(D, gate_rows):
+    need = [ttfoil.block_norm_grad_ws_bytes(T, D, gate_rows) for T in range(1, 3000)]
+    assert all(a <= b for a, b in zip(need, need[1:]))
+    for T in (149, 297, 5000, 18945, 70001):
+        top = ttfoil.block_norm_grad_ws_bytes(T, D, gate_rows)
+        for t in (n for n in (1, 2, 3, 36, 37, 148, 296, T // 3, T // 2, T - 1) if n < T):
+            assert ttfoil.block_norm_grad_ws_bytes(t, D, gate_rows) <= top
+            if gate_rows > 1:  # one vector for all tokens: gate_rows follows T
+                assert ttfoil.block_norm_grad_ws_bytes(t, D, t) <= top
+
+
+@pytest.mark.parametrize("D", [1, 64, 2048, 2049, 4096, 10000, 1 << 18, 1 << 20])
+def test_embed_rows_workspace_grows_with_the_tokens(D):
+    need = [ttfoil.embed_rows_grad_ws_bytes(T, 65536, D) for T in range(1, 18000)]
+    assert all(a <= b for a, b in zip(need, need[1:]))
+    assert need[-1] <= ttfoil.embed_rows_grad_ws_bytes(1 << 24, 65536, D)

@@ -12,6 +12,7 @@
 // the pointers allow, else of 4 bytes (even D), else one by one.
 #include "block_norm.cuh"
 
+#include <algorithm>
 #include <cstring>
 #include <type_traits>
 
@@ -838,8 +839,15 @@ cudaError_t backward_typed(const Backward& p, const Chunks& c, cudaStream_t s) {
 
 uint64_t backward_ws_bytes(uint32_t T, uint32_t D, uint32_t gate_rows) {
     if (T == 0 || D == 0) return 0;
-    const Chunks c = plan_chunks(T, D, gate_rows);
-    return (2ull * c.parts + (c.per_gate ? c.count : 0)) * D * 4;
+    // Bounds of plan_chunks for T tokens or fewer.  There are at most `teams` chunks
+    // of T tokens, one token or more each; where gate rows are shared, at most `teams`
+    // of parts of them (the last gate row may have fewer tokens than chunks: 2 T), or
+    // less than twice `teams` of whole ones (a chunk is more than half of T / teams).
+    const Shape sh(D, 8, 512);
+    const uint64_t teams = (uint64_t)sh.resident(kBackwardThreads) * sh.teams, shared = gate_rows > 1;
+    const uint64_t count = std::min((1 + shared) * T, (1 + shared) * teams);
+    const uint64_t parts = sh.plan.ctas ? count : (count + sh.teams - 1) / sh.teams;
+    return (2 * parts + (shared ? std::min<uint64_t>(2ull * T, teams) : 0)) * D * 4;
 }
 
 cudaError_t forward(const Forward& p, bool fp32, cudaStream_t s) {

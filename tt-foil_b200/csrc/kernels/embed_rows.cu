@@ -18,6 +18,7 @@
 // every sum is fixed by the ids alone; there are no floating-point atomics.
 #include "embed_rows.cuh"
 
+#include <algorithm>
 #include <cstring>
 
 #include "gemm_ptx.cuh"
@@ -187,12 +188,26 @@ struct Plan {
 };
 uint64_t align16(uint64_t b) { return (b + 15u) / 16u * 16u; }
 
-Plan make_plan(const Gradient& p, uint64_t* bytes) {
+// Tokens of a run: short runs where there are few tokens, so that they fill the
+// SMs; one run where one can hold them, which needs no join.
+uint32_t run_length(uint32_t T, uint32_t D) {
+    uint32_t run = kMaxRun;
+    while (run > 8 && T > kMaxRun && (uint64_t)T * ((D + 2047) / 2048) < 512ull * run) run /= 2;
+    return run;
+}
+// The most runs of T tokens or fewer: of T, or of as many as have shorter runs.
+uint32_t most_runs(uint32_t T, uint32_t D) {
+    uint32_t most = 0;
+    for (uint32_t run = 8; run <= kMaxRun; run *= 2) {
+        const uint32_t t = std::min(T, (512u * 2 * run - 1) / ((D + 2047) / 2048));
+        for (uint32_t n : {t, T}) most = std::max(most, (n + run_length(n, D) - 1) / run_length(n, D));
+    }
+    return most;
+}
+
+Plan make_plan(const Gradient& p) {
     Plan q{};
-    // Short runs where there are few tokens, so that they fill the SMs; one run
-    // where one can hold them, which needs no join.
-    q.run = kMaxRun;
-    while (q.run > 8 && p.T > kMaxRun && (uint64_t)p.T * ((p.D + 2047) / 2048) < 512ull * q.run) q.run /= 2;
+    q.run = run_length(p.T, p.D);
     q.runs = (p.T + q.run - 1) / q.run;
     // One CTA sorts few tokens as fast (2048 of them).  Clusters of 4 leave 128 SMs
     // to the zeros, of 8 only 112 (a cluster stays inside a GPC) but sort in half the
@@ -206,7 +221,7 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     char* at = static_cast<char*>(p.ws);
     uint64_t off = 0;
     auto take = [&](uint64_t n) {
-        char* r = at ? at + off : nullptr;
+        char* r = at + off;
         off += align16(n);
         return r;
     };
@@ -214,7 +229,6 @@ Plan make_plan(const Gradient& p, uint64_t* bytes) {
     q.key1 = (uint32_t*)take(4ull * p.T), q.token1 = (uint32_t*)take(4ull * p.T);
     q.key = q.passes % 2 ? q.key1 : q.key0, q.token = q.passes % 2 ? q.token1 : q.token0;
     if (q.runs > 1) q.head = (float*)take(4ull * q.runs * p.D), q.tail = (float*)take(4ull * q.runs * p.D);
-    if (bytes) *bytes = off;
     return q;
 }
 
@@ -525,11 +539,9 @@ cudaError_t sum_launch(const Gradient& p, Plan q, int v, cudaStream_t s) {
 
 uint64_t gradient_ws_bytes(uint32_t T, uint32_t V, uint32_t D) {
     if (T == 0 || V == 0 || D == 0) return 0;
-    Gradient p{};
-    p.T = T, p.V = V, p.D = D;
-    uint64_t bytes = 0;
-    make_plan(p, &bytes);
-    return bytes;
+    // Enough for fewer tokens too, whose runs may be shorter.
+    const uint64_t runs = most_runs(T, D);
+    return 4 * align16(4ull * T) + (runs > 1 ? 2 * align16(4 * runs * D) : 0);
 }
 
 cudaError_t lookup(const Lookup& p, bool fp32, cudaStream_t s) {
@@ -546,7 +558,7 @@ cudaError_t gradient(const Gradient& p, bool fp32, cudaStream_t s) {
     if (p.T == 0)
         return p.accumulate ? cudaSuccess
                             : cudaMemset2DAsync(p.dtable, p.ld_dtable * 4, 0, (size_t)p.D * 4, p.V, s);
-    Plan q = make_plan(p, nullptr);
+    Plan q = make_plan(p);
     Width w(p.D);
     w.use(p.dtable, p.ld_dtable, 4);
     cudaError_t e = w.v == 8 ? sort_launch<8>(p, q, s) : w.v == 2 ? sort_launch<2>(p, q, s) : sort_launch<1>(p, q, s);
