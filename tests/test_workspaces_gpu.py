@@ -7,8 +7,8 @@ pytestmark = pytest.mark.gpu
 import torch  # noqa: E402
 
 import ttfoil as tf  # noqa: E402
-from test_token_path_gpu import (BF, F32, Norm, check_backward, close, embed_grad, embed_ref, gen, make_ids,  # noqa: E402
-                                 randn, run_backward, run_forward)
+from test_token_path_gpu import (BF, F32, Norm, check_backward, close, embed_grad, embed_ref, gen,  # noqa: E402
+                                 make_ids, randn, run_backward, run_forward)
 
 
 @pytest.fixture(autouse=True, scope="module")

@@ -337,44 +337,96 @@ def _place(stream):
 _place_of = None
 
 
-def _vec(t, device):
-    """Pointer of a dense argument: a torch tensor on `device`, an address or None."""
-    if t is None or isinstance(t, int):
-        return t
-    if t.get_device() != device:
-        raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
+# What a tensor's elements may be: the kind's own type, which the calls below look
+# for first, others that stand for it, and its name.
+class _Kind:
+    def __init__(self, name, *types):
+        self.name, self.types, self.own = name, types, None
+
+    def check(self, t):
+        if self.own is None:
+            import torch
+            self.types = tuple(getattr(torch, n) for n in self.types if hasattr(torch, n))
+            self.own = self.types[0]
+        if t.dtype not in self.types:
+            raise FoilError(1, f"tt-foil: a tensor is {t.dtype}, not {self.name}")
+
+
+_BF16 = _Kind("bf16 (or 16-bit integers)", "bfloat16", "int16", "uint16")
+_FP32 = _Kind("float32", "float32")
+_BYTES = _Kind("bytes", "uint8", "int8")
+_IDS = _Kind("32- or 64-bit integers", "int64", "int32", "uint32", "uint64")
+
+
+def _vec(t, device, kind=None, n=0):
+    """Pointer of a dense argument of at least `n` elements: a torch tensor on
+    `device`, an address or None."""
+    if t is None:
+        return None
+    try:
+        if t.get_device() != device:
+            raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
+    except AttributeError:
+        return t  # an address
     if not t.is_contiguous():
         raise FoilError(1, "tt-foil: a tensor must be contiguous")
+    if kind is not None and t.dtype is not kind.own:
+        kind.check(t)
+    if t.numel() < n:
+        raise FoilError(1, f"tt-foil: a tensor has {t.numel()} elements, {n} are needed")
     return t.data_ptr()
 
 
-def _mat(t, ld, device, cols=None):
-    """Pointer and row stride in elements of a matrix (of `cols` columns): the
+def _mat(t, ld, device, cols=None, rows=0, kind=None):
+    """Pointer and row stride in elements of a matrix of `rows` x `cols`: the
     stride as given, else that of a 2-D torch tensor, else 0 (dense)."""
-    if t is None or isinstance(t, int):
-        return t, ld
-    if t.get_device() != device:
-        raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
-    if ld:
-        return t.data_ptr(), ld
-    shape = t.shape
-    if t.is_contiguous() and (len(shape) != 2 or shape[1] == cols):
+    if t is None:
+        return None, ld
+    try:
+        if t.get_device() != device:
+            raise FoilError(1, "tt-foil: a tensor is not on the current CUDA device")
+    except AttributeError:
+        return t, ld  # an address
+    if kind is not None and t.dtype is not kind.own:
+        kind.check(t)
+    if not ld and t.shape == (rows, cols) and t.is_contiguous():
         return t.data_ptr(), 0
-    if len(shape) != 2:
-        raise FoilError(1, "tt-foil: a tensor must be contiguous, or a matrix with a row stride")
+    return t.data_ptr(), _stride(t, ld, cols, rows)
+
+
+def _stride(t, ld, cols, rows):
+    """A tensor's row stride in elements where it is not `rows` dense rows of `cols`."""
+    if ld:
+        if rows and t.storage_offset() + (rows - 1) * ld + cols > t.untyped_storage().nbytes() // t.element_size():
+            raise FoilError(1, f"tt-foil: {rows} x {cols} values with a row stride of {ld} pass a tensor's end")
+        return ld
+    shape = t.shape
+    dims = len(shape)
+    if t.is_contiguous() and (shape[1] == cols if dims == 2 else dims < 2 or not rows or shape[-1] == cols):
+        if rows and t.numel() < rows * cols:
+            raise FoilError(1, f"tt-foil: a tensor has {t.numel()} elements, {rows} x {cols} are needed")
+        return 0
+    if dims != 2:
+        raise FoilError(1, "tt-foil: a tensor must be contiguous rows, or a matrix with a row stride")
+    if rows and (shape[0] < rows or shape[1] < cols):
+        raise FoilError(1, f"tt-foil: a tensor is {shape[0]} x {shape[1]}, {rows} x {cols} are needed")
     rows, cols = shape
     step, unit = t.stride()
     if (cols > 1 and unit != 1) or (rows > 1 and step < cols):
         raise FoilError(1, "tt-foil: rows of a tensor must be contiguous and must not overlap")
-    return t.data_ptr(), step if rows > 1 else 0
+    return step if rows > 1 else 0
 
 
 def _is_fp32(fp32, *tensors):
-    """The residual stream's type: as given, else from the first torch tensor (float32 or 16-bit)."""
+    """The residual stream's type: as given, else from the first torch tensor (float32 or bf16)."""
     for t in tensors:
         if not (t is None or isinstance(t, int)):
-            wide = t.element_size() == 4
-            if fp32 is not None and bool(fp32) != wide:
+            own = t.dtype
+            wide = own is _FP32.own
+            if not wide and own is not _BF16.own:
+                wide = t.element_size() == 4
+                (_FP32 if wide else _BF16).check(t)
+            if fp32 is not None and bool(fp32) is not wide:
                 raise FoilError(1, "tt-foil: tensors of one type are mixed with another")
             fp32 = wide
     return 1 if fp32 else 0
@@ -385,36 +437,64 @@ def w4_packed_bytes(K, N, group, zeros=False):
     return int(lib().foil_w4_packed_bytes(K, N, group, 1 if zeros else 0))
 
 
+# Bytes of a storage block without and with zero points, for each group.
+_BLOCK_BYTES = {g: (1024 + 4096 // g, 1024 + 6144 // g) for g in (32, 64, 128)}
+
+
+def _packed(t, device, K, N, group, zeros):
+    """Pointer of 4-bit storage (the size of w4_packed_bytes; the call refuses other groups)."""
+    block = _BLOCK_BYTES.get(group)
+    return _vec(t, device, _BYTES, (N + 15 >> 4) * (K + 127 >> 7) * block[1 if zeros else 0] if block else 0)
+
+
+def _tiles(t, device, rows, cols):
+    """Pointer of a tile stream of rows x cols tiles."""
+    return _vec(t, device, _BF16, rows * cols * 1024)
+
+
 def w4_pack(codes, scales, packed, K, N, group, zero_points=None, stream=None):
     """Codes (N x K, one byte each), scales (N x ceil(K / group) bf16) and zero
     points (alike, one byte each, or None) -> 4-bit storage."""
     dev, stream = _place(stream)
-    check(lib().foil_w4_pack_dev(_vec(codes, dev), _vec(scales, dev), _vec(zero_points, dev), _vec(packed, dev), K, N,
-                                 group, stream))
+    groups = N * -(-K // group) if group > 0 else 0
+    rc = (_lib or lib()).foil_w4_pack_dev(
+        _vec(codes, dev, _BYTES, N * K), _vec(scales, dev, _BF16, groups), _vec(zero_points, dev, _BYTES, groups),
+        _packed(packed, dev, K, N, group, zero_points is not None), K, N, group, stream)
+    if rc:
+        check(rc)
 
 
 def w4_quantize_tiles(tiles, packed, Kt, Nt, group, zeros=False, stream=None):
     """Tile stream of Kt x Nt tiles -> 4-bit storage with a scale (and, with
     `zeros`, a zero point) for each `group` values of a column."""
     dev, stream = _place(stream)
-    check(lib().foil_w4_quantize_tiles_dev(_vec(tiles, dev), _vec(packed, dev), Kt, Nt, group, 1 if zeros else 0,
-                                           stream))
+    rc = (_lib or lib()).foil_w4_quantize_tiles_dev(
+        _tiles(tiles, dev, Kt, Nt), _packed(packed, dev, 32 * Kt, 32 * Nt, group, zeros), Kt, Nt, group,
+        1 if zeros else 0, stream)
+    if rc:
+        check(rc)
 
 
 def w4_dequantize_tiles(packed, tiles, K, N, group, zeros=False, transpose=False, stream=None):
     """4-bit storage -> tile stream of the weights, or of their transpose."""
     dev, stream = _place(stream)
-    check(lib().foil_w4_dequantize_tiles_dev(_vec(packed, dev), _vec(tiles, dev), K, N, group, 1 if zeros else 0,
-                                             1 if transpose else 0, stream))
+    rc = (_lib or lib()).foil_w4_dequantize_tiles_dev(
+        _packed(packed, dev, K, N, group, zeros), _tiles(tiles, dev, -(-K // 32), -(-N // 32)), K, N, group,
+        1 if zeros else 0, 1 if transpose else 0, stream)
+    if rc:
+        check(rc)
 
 
 def w4_matvec(x, packed, y, M, K, N, group, zeros=False, bias=None, relu=False, ld_x=0, ld_y=0, stream=None):
     """y (M x N) = relu?(x (M x K) . W + bias) with 4-bit W, M at most 64."""
     dev, stream = _place(stream)
-    x, ld_x = _mat(x, ld_x, dev, K)
-    y, ld_y = _mat(y, ld_y, dev, N)
-    check(lib().foil_w4_matvec_dev(x, ld_x, _vec(packed, dev), _vec(bias, dev), y, ld_y, M, K, N, group,
-                                   1 if zeros else 0, 1 if relu else 0, stream))
+    x, ld_x = _mat(x, ld_x, dev, K, M, _BF16)
+    y, ld_y = _mat(y, ld_y, dev, N, M, _BF16)
+    rc = (_lib or lib()).foil_w4_matvec_dev(
+        x, ld_x, _packed(packed, dev, K, N, group, zeros), _vec(bias, dev, _BF16, N), y, ld_y, M, K, N, group,
+        1 if zeros else 0, 1 if relu else 0, stream)
+    if rc:
+        check(rc)
 
 
 GATE_ACTS = {"none": 0, "sigmoid": 1}
@@ -426,6 +506,11 @@ def _gate_act(name):
     return GATE_ACTS[name]
 
 
+def _gates(T, gate_rows):
+    """Gate rows of T tokens."""
+    return T if gate_rows == 1 else -(-T // gate_rows) if gate_rows > 0 else 0
+
+
 def block_norm(resid, u, h, y, T, D, w_pre=None, post=False, w_post=None, gate=None, gate_rows=1, gate_act="none",
                scale=1.0, eps=1e-5, rstd_post=None, rstd_pre=None, fp32=None, ld_resid=0, ld_u=0, ld_gate=0, ld_h=0,
                ld_y=0, stream=None):
@@ -434,15 +519,18 @@ def block_norm(resid, u, h, y, T, D, w_pre=None, post=False, w_post=None, gate=N
     bf16 or fp32 (taken from the tensors; `fp32` for raw pointers)."""
     dev, stream = _place(stream)
     wide = _is_fp32(fp32, resid, h)
-    resid, ld_resid = _mat(resid, ld_resid, dev, D)
-    u, ld_u = _mat(u, ld_u, dev, D)
-    gate, ld_gate = _mat(gate, ld_gate, dev, D)
-    h, ld_h = _mat(h, ld_h, dev, D)
-    y, ld_y = _mat(y, ld_y, dev, D)
-    check(lib().foil_block_norm_dev(resid, ld_resid, u, ld_u, 1 if post else 0, _vec(w_post, dev), gate, ld_gate,
-                                    gate_rows, _gate_act(gate_act), _vec(w_pre, dev), h, ld_h, y, ld_y,
-                                    _vec(rstd_post, dev), _vec(rstd_pre, dev), T, D, wide, scale, eps,
-                                    stream))
+    resid, ld_resid = _mat(resid, ld_resid, dev, D, T)
+    u, ld_u = _mat(u, ld_u, dev, D, T, _BF16)
+    if gate is not None:
+        gate, ld_gate = _mat(gate, ld_gate, dev, D, _gates(T, gate_rows), _BF16)
+    h, ld_h = _mat(h, ld_h, dev, D, T)
+    y, ld_y = _mat(y, ld_y, dev, D, T, _BF16)
+    rc = (_lib or lib()).foil_block_norm_dev(
+        resid, ld_resid, u, ld_u, 1 if post else 0, _vec(w_post, dev, _BF16, D), gate, ld_gate, gate_rows,
+        _gate_act(gate_act), _vec(w_pre, dev, _BF16, D), h, ld_h, y, ld_y, _vec(rstd_post, dev, _FP32, T),
+        _vec(rstd_pre, dev, _FP32, T), T, D, wide, scale, eps, stream)
+    if rc:
+        check(rc)
 
 
 def block_norm_grad_ws_bytes(T, D, gate_rows=0):
@@ -459,34 +547,41 @@ def block_norm_grad(dh, dy, h, u, dresid, du, T, D, ws, rstd_pre=None, w_pre=Non
     dev, stream = _place(stream)
     wide = _is_fp32(fp32, dh, h, dresid)
     n = _ws_bytes(ws, ws_bytes)
-    dh, ld_dh = _mat(dh, ld_dh, dev, D)
-    dy, ld_dy = _mat(dy, ld_dy, dev, D)
-    h, ld_h = _mat(h, ld_h, dev, D)
-    u, ld_u = _mat(u, ld_u, dev, D)
-    gate, ld_gate = _mat(gate, ld_gate, dev, D)
-    dresid, ld_dresid = _mat(dresid, ld_dresid, dev, D)
-    du, ld_du = _mat(du, ld_du, dev, D)
-    dgate, ld_dgate = _mat(dgate, ld_dgate, dev, D)
-    check(lib().foil_block_norm_grad_dev(
-        dh, ld_dh, dy, ld_dy, h, ld_h, _vec(rstd_pre, dev), _vec(w_pre, dev), u, ld_u, 1 if post else 0,
-        _vec(rstd_post, dev), _vec(w_post, dev), gate, ld_gate, gate_rows, _gate_act(gate_act), dresid, ld_dresid,
-        du, ld_du, dgate, ld_dgate, _vec(dw_post, dev), _vec(dw_pre, dev), _vec(ws, dev), n, T, D, wide, scale,
-        stream))
+    dh, ld_dh = _mat(dh, ld_dh, dev, D, T)
+    dy, ld_dy = _mat(dy, ld_dy, dev, D, T, _BF16)
+    h, ld_h = _mat(h, ld_h, dev, D, T)
+    u, ld_u = _mat(u, ld_u, dev, D, T, _BF16)
+    dresid, ld_dresid = _mat(dresid, ld_dresid, dev, D, T)
+    du, ld_du = _mat(du, ld_du, dev, D, T, _BF16)
+    if gate is not None:
+        gates = _gates(T, gate_rows)
+        gate, ld_gate = _mat(gate, ld_gate, dev, D, gates, _BF16)
+        dgate, ld_dgate = _mat(dgate, ld_dgate, dev, D, gates, _BF16)
+    elif dgate is not None:
+        dgate, ld_dgate = _mat(dgate, ld_dgate, dev, D)
+    rc = (_lib or lib()).foil_block_norm_grad_dev(
+        dh, ld_dh, dy, ld_dy, h, ld_h, _vec(rstd_pre, dev, _FP32, T), _vec(w_pre, dev, _BF16, D), u, ld_u,
+        1 if post else 0, _vec(rstd_post, dev, _FP32, T), _vec(w_post, dev, _BF16, D), gate, ld_gate, gate_rows,
+        _gate_act(gate_act), dresid, ld_dresid, du, ld_du, dgate, ld_dgate, _vec(dw_post, dev, _FP32, D),
+        _vec(dw_pre, dev, _FP32, D), _vec(ws, dev), n, T, D, wide, scale, stream)
+    if rc:
+        check(rc)
 
 
 def _ws_bytes(ws, ws_bytes):
-    if ws_bytes is not None:
-        return ws_bytes
     if ws is None or isinstance(ws, int):
-        return 0
-    return ws.numel() * ws.element_size()
+        return ws_bytes or 0
+    n = ws.numel() * ws.element_size()
+    if ws_bytes is not None and ws_bytes > n:
+        raise FoilError(1, f"tt-foil: the workspace has {n} bytes, not {ws_bytes}")
+    return n if ws_bytes is None else ws_bytes
 
 
 def _id_bytes(ids, id_bytes):
     if isinstance(ids, int) or ids is None:
         return id_bytes
-    if ids.is_floating_point() or ids.element_size() not in (4, 8):
-        raise FoilError(1, "tt-foil: ids must be 32- or 64-bit integers")
+    if ids.dtype is not _IDS.own:
+        _IDS.check(ids)
     return ids.element_size()
 
 
@@ -496,10 +591,12 @@ def embed_rows(ids, table, out, T, V, D, scale=1.0, pad_id=-1, id_bytes=4, fp32=
     gives zeros and DEVERR_BAD_INDEX (see device_error)."""
     dev, stream = _place(stream)
     id_bytes, wide = _id_bytes(ids, id_bytes), _is_fp32(fp32, out)
-    table, ld_table = _mat(table, ld_table, dev, D)
-    out, ld_out = _mat(out, ld_out, dev, D)
-    check(lib().foil_embed_rows_dev(_vec(ids, dev), id_bytes, table, ld_table, out, ld_out, T, V, D, wide, scale, pad_id,
-                                    stream))
+    table, ld_table = _mat(table, ld_table, dev, D, V, _BF16)
+    out, ld_out = _mat(out, ld_out, dev, D, T)
+    rc = (_lib or lib()).foil_embed_rows_dev(
+        _vec(ids, dev, None, T), id_bytes, table, ld_table, out, ld_out, T, V, D, wide, scale, pad_id, stream)
+    if rc:
+        check(rc)
 
 
 def embed_rows_grad_ws_bytes(T, V, D):
@@ -514,10 +611,13 @@ def embed_rows_grad(ids, dout, dtable, T, V, D, ws, scale=1.0, pad_id=-1, accumu
     embed_rows_grad_ws_bytes."""
     dev, stream = _place(stream)
     id_bytes, wide, n = _id_bytes(ids, id_bytes), _is_fp32(fp32, dout), _ws_bytes(ws, ws_bytes)
-    dout, ld_dout = _mat(dout, ld_dout, dev, D)
-    dtable, ld_dtable = _mat(dtable, ld_dtable, dev, D)
-    check(lib().foil_embed_rows_grad_dev(_vec(ids, dev), id_bytes, dout, ld_dout, dtable, ld_dtable, T, V, D, wide,
-                                         scale, pad_id, 1 if accumulate else 0, _vec(ws, dev), n, stream))
+    dout, ld_dout = _mat(dout, ld_dout, dev, D, T)
+    dtable, ld_dtable = _mat(dtable, ld_dtable, dev, D, V, _FP32)
+    rc = (_lib or lib()).foil_embed_rows_grad_dev(
+        _vec(ids, dev, None, T), id_bytes, dout, ld_dout, dtable, ld_dtable, T, V, D, wide, scale, pad_id,
+        1 if accumulate else 0, _vec(ws, dev), n, stream)
+    if rc:
+        check(rc)
 
 
 def matmul_tiles_host(device, a, b, c, Mt, Kt, Nt, bias=None, relu=False, chunk_rows=0):
