@@ -23,3 +23,14 @@ def golden():
         return dict(np.load(os.path.join(GOLDEN, name + ".npz")))
 
     return load
+
+
+def pytest_collection_modifyitems(items):
+    """The drop-in runs execute binaries compiled from the reference's test
+    sources; without a reference tree there are none to run."""
+    if os.path.isdir(os.path.join(REPO, "oracle", "_ref", "droptests")):
+        return
+    skip = pytest.mark.skip(reason="oracle/_ref/droptests not built: it takes the reference's test sources")
+    for item in items:
+        if os.path.basename(str(item.fspath)) == "test_dropin_gpu.py":
+            item.add_marker(skip)
