@@ -141,3 +141,24 @@ def test_gradient_without_post_norm_does_not_look_at_the_output(D, fp32, gate_ro
     out = run_backward(p, saved, want=("dresid", "du"))
     for k in ("dresid", "du"):
         assert torch.isfinite(base[k]).all() and torch.equal(out[k], base[k]), k
+
+
+# --------------------------------------------------- many rows of one CTA's team ---
+
+@pytest.mark.parametrize("T,D", [(900, 2049), (1100, 2048), (700, 5120), (400, 8200), (330, 16384), (700, 3000)])
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("gate_rows", [1, 7])
+def test_forward_of_more_rows_than_teams(T, D, fp32, gate_rows):
+    """Teams of a CTA and of a cluster go on to other rows: sums in turn, rows asked
+    for ahead."""
+    p = Norm(T, D, fp32, True, gate_rows, "sigmoid")
+    check_forward(p, run_forward(p))
+
+
+@pytest.mark.parametrize("T,D", [(700, 2050), (500, 4096), (400, 4104), (300, 8200), (120, 16384), (250, 4097)])
+@pytest.mark.parametrize("fp32", [False, True])
+@pytest.mark.parametrize("gate_rows", [0, 1, 50])
+def test_gradient_of_more_rows_than_teams(T, D, fp32, gate_rows):
+    p = Norm(T, D, fp32, True, gate_rows, "sigmoid" if gate_rows == 1 else "none")
+    saved = run_forward(p)
+    check_backward(p, saved, run_backward(p, saved))
