@@ -327,7 +327,9 @@ def _place(stream):
     global _place_of
     if _place_of is None:
         import torch
-        _place_of = torch.cuda.current_device, getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        torch.cuda.current_device()  # sets CUDA up; from then on torch's own short cut does
+        _place_of = (getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device),
+                     getattr(torch._C, "_cuda_getCurrentRawStream", None))
     device = _place_of[0]()
     if stream is None and _place_of[1] is not None:
         return device, _place_of[1](device)
@@ -437,14 +439,13 @@ def w4_packed_bytes(K, N, group, zeros=False):
     return int(lib().foil_w4_packed_bytes(K, N, group, 1 if zeros else 0))
 
 
-# Bytes of a storage block without and with zero points, for each group.
-_BLOCK_BYTES = {g: (1024 + 4096 // g, 1024 + 6144 // g) for g in (32, 64, 128)}
+# Bytes of a storage block, by (group, zero points); 0 for groups that the call refuses.
+_BLOCK_BYTES = {(g, z): 1024 + (6144 if z else 4096) // g for g in (32, 64, 128) for z in (False, True)}
 
 
 def _packed(t, device, K, N, group, zeros):
-    """Pointer of 4-bit storage (the size of w4_packed_bytes; the call refuses other groups)."""
-    block = _BLOCK_BYTES.get(group)
-    return _vec(t, device, _BYTES, (N + 15 >> 4) * (K + 127 >> 7) * block[1 if zeros else 0] if block else 0)
+    """Pointer of 4-bit storage (the size of w4_packed_bytes)."""
+    return _vec(t, device, _BYTES, (N + 15 >> 4) * (K + 127 >> 7) * _BLOCK_BYTES.get((group, not not zeros), 0))
 
 
 def _tiles(t, device, rows, cols):
