@@ -422,9 +422,9 @@ FOIL_API int foil_w4_dequantize_tiles_dev(const void* packed, uint16_t* tiles, u
                                           uint32_t group, int32_t zeros, int32_t transpose, void* stream);
 
 /* y (M x N) = relu?(x (M x K) . W + bias) for a few rows, M from 1 to 64:
- * one pass over the 4-bit weights for up to 16 rows, and for up to 64 if x is
- * 16-byte aligned and ld_x a multiple of 8 (longer inputs: dequantise and use
- * foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or NULL.  fp32
+ * one pass over the 4-bit weights for up to 16 rows (8 with group 32, zero points
+ * and K above 31744), and for up to 64 if x is 16-byte aligned and ld_x a multiple
+ * of 8 (longer inputs: dequantise and use foil_matmul_tiles_dev).  K from 1 to 32768.  bias: N values or NULL.  fp32
  * accumulation of unrounded weights, one rounding to bf16 at the end.  An
  * infinity or NaN in a row of x makes that row's outputs infinite or NaN.  With
  * more than 16 rows a group's sum of (q - z) x and the row's sum are fp32 numbers

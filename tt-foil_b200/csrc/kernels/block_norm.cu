@@ -301,7 +301,7 @@ struct Input {
 
 // A row of a tensor towards L2: each of a team's first threads asks for one
 // tensor's, the whole 16-byte pieces of it.  Forward, 8192 x 5120: 121 us
-// without, 106 with.
+// without, 104 with.
 struct Ahead {
     uint64_t at;            // row 0
     uint32_t pitch, bytes;  // bytes 0: nothing to ask for
@@ -471,8 +471,8 @@ template <class R, int V, int NV, int THREADS, int GATE, bool AHEAD>
 __global__ void __launch_bounds__(THREADS) backward_kernel(const Backward p, const Chunks c, const TeamPlan plan) {
     constexpr int kPairs = V * NV / 2;
     // Rows asked for from L2.  Beside the row in registers it pays where a row
-    // takes a cluster (2000 x 8192 84 and 75 us), elsewhere it costs registers
-    // (16384 x 4096 without gates 168 and 178 us).
+    // takes a cluster (2000 x 8192: 78 us, 85 without), elsewhere it costs registers
+    // (16384 x 4096 without gates: 182 us, 167 without).
     constexpr bool kAhead = !AHEAD || GATE;
     constexpr uint32_t kAheadBy = AHEAD ? 3u : 2u, kAheadMin = AHEAD ? 4097u : 256u;
     __shared__ float shared[2 * Team::kSumFloats];
@@ -801,8 +801,9 @@ cudaError_t forward_typed(const Forward& p, cudaStream_t s) {
 }
 
 // The next row in registers where those suffice (4096 x 4096, bf16 in vectors of 8:
-// 59 us with, 69 without), else towards L2 only (fp32: 102 and 81 us; 4000 x 4095 one
-// by one: 162 and 102; bf16 with logistic gates: 86 and 72).
+// 59 us with, 70 without; 4099 x 2050 in vectors of 2: 57 and 66), else towards L2 only
+// (fp32: 98 us with, 80 without; 4000 x 4095 one by one: 160 and 101; bf16 with logistic
+// gates: 90 and 72).
 template <class R, int V, int GATE>
 constexpr bool next_row_ahead() {
     return sizeof(R) == 2 && ((V == 8 && GATE != kSigmoidGate) || (V == 2 && GATE == kNoGate));
